@@ -626,6 +626,54 @@ int mvf_adam_step(float* p, float* g, float* m, float* v, size_t n, float lr, fl
 int mvf_optim_set_width(int cus);
 
 /* ------------------------------------------------------------------------------------------------
+ * Token sequences with positions and a cache: the temporal encoder of models/utils.py:47-242 over videos of different lengths without
+ * padding, causal by token or by frame, trained on whole videos and run frame by frame on live ones (no counterpart in the reference,
+ * whose encoder is bidirectional over padded clips with an added one-axis sin/cos table, models/utils.py:113-145).
+ *
+ * dtype: MVF_F32, MVF_BF16 or MVF_F16 for all of q, k, v, gradients and caches; statistics and accumulation in fp32.
+ * Heads lie in tokens: element (token t, head h, channel d) at t * ld + h * hs + d, strides in ELEMENTS, every stride a multiple of 16
+ * bytes, pointers 16-byte aligned (a column slice of a fused q | k | v projection qualifies); outputs are contiguous.  Hq % Hk == 0: query
+ * head h reads key head h / (Hq / Hk).  Head size D: a multiple of 8, for attention up to 128 (MVF_ERR_UNSUPPORTED otherwise).
+ * `frame` = n > 0: the token at position p of its sequence sees the keys before (p / n + 1) n, i.e. its own and all earlier groups of n
+ * tokens (1: causal by token; the number of entities: causal by frame); 0: every key of the sequence.
+ * Device values that cannot be checked on the host do no harm: a row no sequence holds gets zeros, a page or a slot outside the cache is
+ * neither read nor written, a NaN or infinity of a key reaches only the rows that see that key.
+ * ---------------------------------------------------------------------------------------------- */
+/* Rotary positions with up to three axes (s1 = s2 = 0: one).  Pair p of a head turns by pos[t][axis] * freqs[p], pairs [0, s0) on axis 0,
+ * the next s1 on axis 1, the next s2 on axis 2; s0 + s1 + s2 <= D / 2, channels behind 2 (s0 + s1 + s2) stay.  interleaved: pair p is
+ * channels 2p, 2p + 1; otherwise p and p + (s0 + s1 + s2).  pos [T][axes] contiguous, pos_type 0 int32, 1 int64, 2 float.  freqs: double,
+ * device.  The angle is reduced in 64 bits.  inverse != 0 turns back: the gradient.  k may be NULL with Hk = 0. */
+int mvf_rotary(int dtype, const void* q, long ldq, long hsq, const void* k, long ldk, long hsk, const void* pos, int pos_type,
+               const double* freqs, int s0, int s1, int s2, int interleaved, int inverse, void* q_out, void* k_out, int T, int Hq,
+               int Hk, int D, hipStream_t stream);
+/* The same for new tokens of streams with a paged cache: q_out [T, Hq, D]; turned k and plain v go to row index[t] % page of page
+ * block_table[seq[t]][index[t] / page] of k_cache, v_cache [n_pages, page, Hk, D].  block_table [n_seqs][table_width].  A token whose seq,
+ * index or page lies outside (seq = -1: padding) is not written.  Two tokens of one slot: either may win. */
+int mvf_rotary_append(int dtype, const void* q, long ldq, long hsq, const void* k, long ldk, long hsk, const void* v, long ldv, long hsv,
+                      const void* pos, int pos_type, const double* freqs, int s0, int s1, int s2, int interleaved, void* q_out,
+                      void* k_cache, void* v_cache, const int* block_table, int table_width, int n_seqs, const int* seq,
+                      const int* index, int n_pages, int page, int T, int Hq, int Hk, int D, hipStream_t stream);
+/* Attention over packed sequences: sequence b holds rows cu_seqlens[b] .. cu_seqlens[b + 1] of the T rows (cu_seqlens [n_seqs + 1],
+ * ascending, device).  out [T, Hq, D].  stat: NULL, or [2][Hq][T] floats for the backward.  A row that sees no key (and one whose every
+ * score is -infinity) gets zeros. */
+int mvf_packed_attn_fwd(int dtype, const void* q, long ldq, long hsq, const void* k, long ldk, long hsk, const void* v, long ldv, long hsv,
+                        const int* cu_seqlens, int n_seqs, void* out, float* stat, int T, int Hq, int Hk, int D, int frame, float scale,
+                        hipStream_t stream);
+/* Its gradients: out, d_out [T, Hq, D], stat as the forward left it, delta: [Hq][T] floats of scratch; dq [T, Hq, D], dk, dv [T, Hk, D]
+ * (summed over the query heads of a group in a fixed order; no atomics). */
+int mvf_packed_attn_bwd(int dtype, const void* q, long ldq, long hsq, const void* k, long ldk, long hsk, const void* v, long ldv, long hsv,
+                        const int* cu_seqlens, int n_seqs, const void* out, const void* d_out, const float* stat, float* delta, void* dq,
+                        void* dk, void* dv, int T, int Hq, int Hk, int D, int frame, float scale, hipStream_t stream);
+/* Attention of the last n_new tokens of each of B streams, positions lengths[b] - n_new .. lengths[b] - 1, over the stream's pages.
+ * q: element (b, i, h, d) at b * q_batch + i * q_token + h * q_head + d; out [B, n_new, Hq, D]; block_table [B][table_width].  A position
+ * before 0 sees nothing (unless frame = 0) and gets zeros.  workspace: mvf_paged_attn_workspace_bytes (0: NULL will do), not shared between
+ * calls that can run at the same time. */
+size_t mvf_paged_attn_workspace_bytes(int B, int n_new, int Hq, int Hk, int D, int table_width, int page);
+int mvf_paged_attn(int dtype, const void* q, long q_batch, long q_token, long q_head, const void* k_cache, const void* v_cache,
+                   const int* block_table, const int* lengths, void* out, void* workspace, size_t ws_bytes, int B, int n_new, int Hq,
+                   int Hk, int D, int n_pages, int page, int table_width, int frame, float scale, hipStream_t stream);
+
+/* ------------------------------------------------------------------------------------------------
  * GPU-side view augmentation: one clip [T,3,H,W] of floats in [0,1] -> [T,3,S,S], normalised
  *   replaces: train.preproc_views (train.py:39-53) applying the ComposeOp of datasets/data_augment.py:372-413
  *   (random_resized_crop :287-317, flip :10-14, torchvision ColorJitter :340-352, torchvision GaussianBlur :357-365,

@@ -1,0 +1,571 @@
+"""Rotary positions, attention over packed sequences and attention over a paged cache (video_rep_learning_amd.ops) against their 64-bit
+statements (oracle/seq.py), within bounds that follow from the kernels' roundings; then what a user can do with them: other strides,
+padding, non-finite values where nobody looks, streams, graphs, and the four of them in a row."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+from oracle import seq as OS  # noqa: E402
+from video_rep_learning_amd import ops  # noqa: E402
+
+DEV = 'cuda'
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+IDS = ['fp32', 'bf16', 'fp16']
+
+
+def randn(*shape, dtype, seed, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(*shape, generator=g) * scale).to(dtype).to(DEV)
+
+
+def within(got, want, bound, what):
+    err = (got.detach().double().cpu() - want).abs()
+    over = err - bound
+    assert not torch.isnan(err).any() and (over <= 0).all(), '%s: off by %.3e where %.3e is allowed (worst of %d)' % (
+        what, err.flatten()[over.argmax()].item(), bound.flatten()[over.argmax()].item(), err.numel())
+
+
+def cum(lengths, first=0):
+    out = [first]
+    for n in lengths:
+        out.append(out[-1] + n)
+    return out
+
+
+def cu_tensor(c):
+    return torch.tensor(c, dtype=torch.int32, device=DEV)
+
+
+# ------------------------------------------------------------------------------------------------ rotary
+ROTARY = [  # tokens, hq, hk, d, sections, interleaved, pos dtype, far
+    (1, 1, 1, 8, (4,), False, torch.int32, 0),
+    (96, 8, 8, 32, (12, 4), False, torch.int64, 0),
+    (77, 12, 3, 64, (8, 12, 12), False, torch.int64, 10 ** 6),
+    (130, 5, 5, 40, (7, 6), True, torch.int32, 1000),
+    (33, 4, 2, 128, (16, 24, 24), True, torch.int64, 10 ** 9),
+    (19, 3, 1, 24, (5,), False, torch.float32, 0),
+    (64, 2, 2, 80, (3, 1, 1), True, torch.float32, 3000),
+    (5, 1, 1, 256, (100, 28), False, torch.int32, 7),
+]
+
+
+def positions(tokens, axes, dtype, far, seed):
+    g = torch.Generator().manual_seed(seed)
+    p = torch.randint(-5, 900, (tokens, axes), generator=g)
+    p[:, 0] += far
+    return (p.float() + torch.rand(tokens, axes, generator=g) if dtype == torch.float32 else p.to(dtype)).to(DEV)
+
+
+@pytest.mark.parametrize('dtype', DTYPES, ids=IDS)
+@pytest.mark.parametrize('t,hq,hk,d,sections,il,pdt,far', ROTARY)
+def test_rotary_and_its_gradient(dtype, t, hq, hk, d, sections, il, pdt, far):
+    qkv = randn(t, hq + 2 * hk, d, dtype=dtype, seed=1)
+    q, k = qkv[:, :hq].requires_grad_(), qkv[:, hq:hq + hk].detach().requires_grad_()
+    pos, freqs = positions(t, len(sections), pdt, far, 2), ops.rotary_freqs(sections)
+    yq, yk = ops.rotary(q, k, pos, freqs, sections, interleaved=il)
+    gq, gk = randn(t, hq, d, dtype=dtype, seed=3), randn(t, hk, d, dtype=dtype, seed=4)
+    dq, dk = torch.autograd.grad((yq, yk), (q, k), (gq, gk))
+    for x, y, inv, what in ((q, yq, False, 'q'), (k, yk, False, 'k'), (gq, dq, True, 'dq'), (gk, dk, True, 'dk')):
+        want = OS.rotate(x, pos, freqs, sections, il, inverse=inv)
+        within(y, want, OS.rotate_bound(x, want, sections, il, dtype), what)
+    only, none = ops.rotary(q.detach(), None, pos, freqs, sections, interleaved=il)
+    assert none is None and torch.equal(only, yq)
+
+
+def test_rotary_keeps_lengths_and_differences():
+    """Against differences: rotation is linear, so y(x + e) - y(x) is the gradient's transpose applied to e up to two roundings of each."""
+    t, h, d, sections = 20, 2, 16, (5, 3)
+    q = randn(t, h, d, dtype=torch.float32, seed=5).requires_grad_()
+    pos, freqs = positions(t, 2, torch.int64, 50, 6), ops.rotary_freqs(sections, base=500.0)
+    w = randn(t, h, d, dtype=torch.float32, seed=7)
+    y, _ = ops.rotary(q, None, pos, freqs, sections)
+    dq, = torch.autograd.grad(y, q, w)
+    e = randn(t, h, d, dtype=torch.float32, seed=8)
+    with torch.no_grad():
+        diff = ((ops.rotary(q + e, None, pos, freqs, sections)[0] - ops.rotary(q - e, None, pos, freqs, sections)[0]).double() * w.double()).sum() / 2
+    lin = (dq.double() * e.double()).sum()
+    mag = (w.double().abs() * (q.double().abs() + e.double().abs())).sum() * 4
+    assert abs(diff - lin) <= 16 * OS.U32 * mag
+
+
+def make_cache(pages, page, hk, d, dtype, seed):
+    return randn(pages, page, hk, d, dtype=dtype, seed=seed), randn(pages, page, hk, d, dtype=dtype, seed=seed + 1)
+
+
+@pytest.mark.parametrize('dtype', DTYPES, ids=IDS)
+@pytest.mark.parametrize('page,hq,hk,d,sections,il', [(16, 8, 8, 32, (12, 4), False), (7, 4, 2, 40, (20,), True), (1, 3, 1, 24, (3, 2, 1), False),
+                                                      (64, 6, 2, 128, (16, 24, 24), True)])
+def test_rotary_append_writes_its_slots_and_nothing_else(dtype, page, hq, hk, d, sections, il):
+    news, olds = [3, 0, 1, 21, 2], [0, 4, 2 * page, 5, page - 1]
+    width = max((a + b + page - 1) // page for a, b in zip(news, olds))
+    pages = 5 * width + 2
+    table = torch.randperm(pages, generator=torch.Generator().manual_seed(3))[:5 * width].view(5, width).int().to(DEV)
+    seq = [b for b, n in enumerate(news) for _ in range(n)] + [-1, 5, 2, 2, 0]                 # padding, no such stream,
+    index = [o + i for n, o in zip(news, olds) for i in range(n)] + [0, 0, -1, width * page, 2 ** 31 - 1]   # no such index
+    t = len(seq)
+    table[4, 0] = pages                       # a page outside the cache, and a negative one
+    table[4, width - 1] = -7
+    kc, vc = make_cache(pages, page, hk, d, dtype, 11)
+    want_k, want_v = kc.double().cpu(), vc.double().cpu()
+    qkv = randn(t, hq + 2 * hk, d, dtype=dtype, seed=12)
+    q, k, v = qkv[:, :hq], qkv[:, hq:hq + hk], qkv[:, hq + hk:]
+    pos, freqs = positions(t, len(sections), torch.int64, 100, 13), ops.rotary_freqs(sections)
+    qo = ops.rotary_append(q, k, v, pos, freqs, sections, kc, vc, table, torch.tensor(seq, dtype=torch.int32, device=DEV),
+                           torch.tensor(index, dtype=torch.int32, device=DEV), interleaved=il)
+    wq = OS.rotate(q, pos, freqs, sections, il)
+    within(qo, wq, OS.rotate_bound(q, wq, sections, il, dtype), 'q')
+    wk = OS.rotate(k, pos, freqs, sections, il)
+    wb = OS.rotate_bound(k, wk, sections, il, dtype)
+    bound = torch.zeros_like(want_k)
+    for i, (b, j) in enumerate(zip(seq, index)):
+        if 0 <= b < 5 and 0 <= j < width * page:
+            pg = int(table[b, j // page])
+            if 0 <= pg < pages:
+                want_k[pg, j % page], want_v[pg, j % page], bound[pg, j % page] = wk[i], v[i].double().cpu(), wb[i]
+    within(kc, want_k, bound, 'k cache')
+    assert torch.equal(vc.double().cpu(), want_v)
+
+
+# ------------------------------------------------------------------------------------------------ packed attention
+LENGTHS = {
+    'one': [1],
+    'short': [1, 0, 2, 31, 32, 33, 0, 5],
+    'edges': [63, 64, 65, 127, 129],
+    'long': [300, 1, 517],
+    'many': [3] * 70,
+}
+PACKED = [  # lengths, hq, hk, d, frame
+    ('one', 1, 1, 8, 1), ('one', 4, 2, 64, 0),
+    ('short', 8, 8, 32, 3), ('short', 4, 1, 40, 1), ('short', 3, 3, 96, 0),
+    ('edges', 2, 2, 64, 1), ('edges', 6, 2, 128, 1), ('edges', 2, 1, 80, 7),
+    ('long', 2, 2, 32, 6), ('long', 3, 1, 64, 0), ('long', 2, 2, 128, 100000),
+    ('many', 2, 2, 16, 1), ('many', 5, 5, 48, 2),
+]
+
+
+def run_packed(q, k, v, cu, frame, do, scale=None):
+    q, k, v = (x.detach().requires_grad_() for x in (q, k, v))
+    out = ops.packed_attention(q, k, v, cu, frame=frame, scale=scale)
+    return (out,) + torch.autograd.grad(out, (q, k, v), do)
+
+
+@pytest.mark.parametrize('dtype', DTYPES, ids=IDS)
+@pytest.mark.parametrize('lengths,hq,hk,d,frame', PACKED)
+def test_packed_attention_and_its_gradients(dtype, lengths, hq, hk, d, frame):
+    c = cum(LENGTHS[lengths])
+    t = c[-1]
+    q, k, v = (randn(t, h, d, dtype=dtype, seed=20 + i, scale=s) for i, (h, s) in enumerate(((hq, 1.5), (hk, 1.0), (hk, 1.0))))
+    do = randn(t, hq, d, dtype=dtype, seed=24)
+    got = run_packed(q, k, v, cu_tensor(c), frame, do)
+    want = OS.packed(q, k, v, c, frame, do=do)
+    for x, nm in zip(got, ('out', 'dq', 'dk', 'dv')):
+        assert x.dtype == dtype
+        within(x, want[nm], want[nm + '_b'], nm)
+    with torch.no_grad():
+        assert torch.equal(ops.packed_attention(q, k, v, cu_tensor(c), frame=frame), got[0])       # the same without statistics
+
+
+@pytest.mark.parametrize('dtype', DTYPES, ids=IDS)
+@pytest.mark.parametrize('frame', [0, 1, 4])
+def test_packed_attention_leaves_rows_of_no_sequence_alone(dtype, frame):
+    """Rows before the first and behind the last sequence hold NaN (uninitialised padding): zeros out, zero gradients, and the rows of
+    sequences come out as if the others were not there."""
+    c = cum([40, 0, 75], first=3)
+    t, hq, hk, d = c[-1] + 61, 4, 2, 64
+    q, k, v, do = (randn(t, h, d, dtype=dtype, seed=30 + i) for i, h in enumerate((hq, hk, hk, hq)))
+    for x in (q, k, v, do):
+        x[:3] = math.nan
+        x[c[-1]:] = math.nan
+    got = run_packed(q, k, v, cu_tensor(c), frame, do)
+    inner = slice(3, c[-1])
+    alone = run_packed(q[inner], k[inner], v[inner], cu_tensor([x - 3 for x in c]), frame, do[inner])
+    want = OS.packed(*(x[inner] for x in (q, k, v)), [x - 3 for x in c], frame, do=do[inner])
+    for x, y, nm in zip(got, alone, ('out', 'dq', 'dk', 'dv')):
+        assert (x[:3] == 0).all() and (x[c[-1]:] == 0).all(), nm
+        within(x[inner], want[nm], want[nm + '_b'], nm)
+        within(y, want[nm], want[nm + '_b'], nm)
+
+
+@pytest.mark.parametrize('dtype', DTYPES, ids=IDS)
+@pytest.mark.parametrize('bad', [math.nan, math.inf, -math.inf])
+def test_packed_attention_hides_what_a_row_does_not_see(dtype, bad):
+    """Non-finite keys and values of one token: the rows that see it change, no other row does -- not the earlier ones of the same tile,
+    not the next sequence's."""
+    c, hq, hk, d, at = cum([50, 70, 20]), 2, 1, 32, 50 + 37
+    t = c[-1]
+    q, k, v = (randn(t, h, d, dtype=dtype, seed=40 + i) for i, h in enumerate((hq, hk, hk)))
+    clean = OS.packed(q, k, v, c, 1)
+    sees = torch.zeros(t, dtype=torch.bool)
+    sees[at:c[2]] = True
+    v2 = v.clone()
+    v2[at, :, 5] = bad
+    out = ops.packed_attention(q, k, v2, cu_tensor(c), frame=1)
+    within(out[~sees], clean['out'][~sees], clean['out_b'][~sees], 'unseen value')
+    other = [i for i in range(d) if i != 5]
+    within(out[sees][..., other], clean['out'][sees][..., other], clean['out_b'][sees][..., other], 'other channels')
+    got = out[sees][..., 5].double().cpu()
+    assert torch.isnan(got).all() if math.isnan(bad) else (got == bad).all()
+    k2 = k.clone()
+    k2[at] = bad
+    out = ops.packed_attention(q, k2, v, cu_tensor(c), frame=1)
+    within(out[~sees], clean['out'][~sees], clean['out_b'][~sees], 'unseen key')
+    # two infinities of different sign meet
+    v2[at + 3, :, 5] = -bad
+    out = ops.packed_attention(q, k, v2, cu_tensor(c), frame=1)
+    assert torch.isnan(out[at + 3:c[2], :, 5]).all() and (math.isnan(bad) or not torch.isnan(out[at:at + 3, :, 5]).any())
+
+
+@pytest.mark.parametrize('dtype', DTYPES, ids=IDS)
+def test_packed_attention_gradients_hide_other_sequences(dtype):
+    """A sequence whose inputs or output gradients are not finite leaves its neighbours' gradients as they are."""
+    c, hq, hk, d = cum([45, 30, 90]), 4, 2, 64
+    t = c[-1]
+    q, k, v, do = (randn(t, h, d, dtype=dtype, seed=50 + i) for i, h in enumerate((hq, hk, hk, hq)))
+    want = OS.packed(q, k, v, c, 1, do=do)
+    keep = torch.ones(t, dtype=torch.bool)
+    keep[c[1]:c[2]] = False
+    for which in range(4):
+        xs = [x.clone() for x in (q, k, v, do)]
+        xs[which][c[1] + 4] = math.nan
+        xs[which][c[1] + 9] = math.inf
+        got = run_packed(xs[0], xs[1], xs[2], cu_tensor(c), 1, xs[3])
+        for x, nm in zip(got, ('out', 'dq', 'dk', 'dv')):
+            within(x[keep], want[nm][keep], want[nm + '_b'][keep], '%s with a bad %s' % (nm, 'qkvd'[which]))
+        # causal: what comes before the bad token inside its own sequence
+        within(got[0][c[1]:c[1] + 4], want['out'][c[1]:c[1] + 4], want['out_b'][c[1]:c[1] + 4], 'earlier rows')
+
+
+def test_packed_attention_gradient_against_differences():
+    """Central differences of the fp32 forward: f = sum w * out.  The forward is off by its bounds, so f by b = sum |w| bound, the quotient
+    by b / h; the step's own error is h^2 / 6 of the third derivative, taken from halving the step."""
+    c, hq, hk, d, frame = cum([17, 1, 30]), 2, 1, 16, 3
+    t = c[-1]
+    x = [randn(t, h, d, dtype=torch.float32, seed=60 + i, scale=0.7) for i, h in enumerate((hq, hk, hk))]
+    w = randn(t, hq, d, dtype=torch.float32, seed=64)
+    grads = run_packed(*x, cu_tensor(c), frame, w)[1:]
+    bound = (w.double().abs().cpu() * OS.packed(*x, c, frame)['out_b']).sum().item()
+
+    def f(xs):
+        return (ops.packed_attention(*xs, cu_tensor(c), frame=frame).double() * w.double()).sum().item()
+    for i in range(3):
+        e = randn(*x[i].shape, dtype=torch.float32, seed=70 + i)
+        quotient = []
+        for h in (2.0 ** -4, 2.0 ** -5):
+            quotient.append((f([y + h * e if j == i else y for j, y in enumerate(x)]) - f([y - h * e if j == i else y for j, y in enumerate(x)])) / (2 * h))
+        lin = (grads[i].double() * e.double()).sum().item()
+        # x +- h e rounds too: one step of 32 bits of x, carried by the gradient
+        rounding = (grads[i].double().abs() * x[i].double().abs()).sum().item() * 4 * OS.U32 * 2.0 ** 5
+        assert abs(quotient[1] - lin) <= abs(quotient[0] - quotient[1]) + 2 * bound * 2.0 ** 5 + rounding, (i, quotient, lin)
+
+
+@pytest.mark.parametrize('dtype', DTYPES, ids=IDS)
+def test_packed_attention_other_strides(dtype):
+    """Slices of a fused projection, heads before tokens, an odd start (copied), channels not contiguous (copied), broadcast keys."""
+    c, hq, hk, d = cum([33, 60]), 4, 2, 32
+    t = c[-1]
+    q, k, v, do = (randn(t, h, d, dtype=dtype, seed=80 + i) for i, h in enumerate((hq, hk, hk, hq)))
+    base = run_packed(q, k, v, cu_tensor(c), 1, do)
+    fused = torch.cat([q, k, v], 1)
+    tr = [x.transpose(0, 1).contiguous().transpose(0, 1) for x in (q, k, v)]
+    odd = [torch.cat([x.new_zeros(1), x.flatten()])[1:].view(x.shape) for x in (q, k, v)]
+    last = [x.transpose(1, 2).contiguous().transpose(1, 2) for x in (q, k, v)]
+    for xs in ((fused[:, :hq], fused[:, hq:hq + hk], fused[:, hq + hk:]), tr, odd, last):
+        got = run_packed(*xs, cu_tensor(c).long(), 1, do.transpose(0, 1).contiguous().transpose(0, 1))
+        assert all(torch.equal(a, b) for a, b in zip(base, got))
+    # one key head for all, broadcast by the caller: the gradient of the broadcast input is the sum of the heads'
+    one = randn(t, 1, d, dtype=torch.float32, seed=90).requires_grad_()
+    qf, vf, dof = q.float(), v.float(), do.float()
+    out = ops.packed_attention(qf, one.expand(t, hk, d), vf, cu_tensor(c), frame=1)
+    g, = torch.autograd.grad(out, one, dof)
+    want = OS.packed(qf, one.detach().expand(t, hk, d), vf, c, 1, do=dof)
+    within(g[:, 0], want['dk'].sum(1), want['dk_b'].sum(1) + OS.U32 * want['dk'].abs().sum(1), 'broadcast key')
+
+
+def test_packed_attention_nothing_to_do():
+    z = torch.zeros(0, 2, 32, device=DEV).requires_grad_()
+    out = ops.packed_attention(z, z, z, cu_tensor([0, 0]), frame=1)
+    out.sum().backward()
+    assert out.shape == (0, 2, 32) and z.grad.shape == (0, 2, 32)
+    q = randn(9, 2, 32, dtype=torch.float32, seed=1).requires_grad_()
+    out = ops.packed_attention(q, q, q, cu_tensor([0, 0, 0]), frame=0)         # rows, but no sequence holds them
+    out.sum().backward()
+    assert (out == 0).all() and (q.grad == 0).all()
+    y, _ = ops.rotary(z.detach(), None, torch.zeros(0, 1, dtype=torch.int64, device=DEV), ops.rotary_freqs((16,)), (16,))
+    assert y.shape == (0, 2, 32)
+
+
+def test_packed_attention_survives_bounds_out_of_order():
+    """Bounds that do not ascend or leave the rows give no meaningful rows, but nothing outside the operands is touched."""
+    q = randn(200, 2, 32, dtype=torch.bfloat16, seed=2).requires_grad_()
+    for c in ([50, 10, 300], [-40, 20, 10 ** 9], [200, 0, 200], [0, 2 ** 31 - 1, -2 ** 31]):
+        out = ops.packed_attention(q, q, q, cu_tensor(c), frame=3)
+        torch.autograd.grad(out, q, torch.ones_like(out))
+    torch.cuda.synchronize()
+
+
+def test_packed_attention_far_rows():
+    """Token strides that put the last rows behind 2^31 elements."""
+    t, h, d = 130, 1, 64
+    stride = (1 << 31) // 100 // 8 * 8
+    buf = torch.empty(stride * (t - 1) + 3 * d, device=DEV, dtype=torch.bfloat16)
+    q, k, v = (buf[i * d:].as_strided((t, h, d), (stride, d, 1)) for i in range(3))
+    dense = [randn(t, h, d, dtype=torch.bfloat16, seed=100 + i) for i in range(3)]
+    for x, y in zip((q, k, v), dense):
+        x.copy_(y)
+    cu = cu_tensor([0, 60, t])
+    assert torch.equal(ops.packed_attention(q, k, v, cu, frame=1), ops.packed_attention(*dense, cu, frame=1))
+
+
+# ------------------------------------------------------------------------------------------------ paged attention
+PAGED = [  # lengths, new, page, hq, hk, d, frame
+    ([1], 1, 16, 1, 1, 8, 1),
+    ([99], 3, 16, 8, 8, 32, 3),
+    ([0, 1, 2, 31, 32, 33, 64, 65], 1, 7, 4, 2, 40, 1),
+    ([5, 0, 130, 2], 3, 1, 6, 2, 64, 1),
+    ([700, 3, 257], 2, 24, 8, 1, 128, 0),
+    ([1300, 2600, 1], 1, 64, 16, 4, 128, 1),
+    ([90, 4], 6, 16, 16, 2, 96, 6),
+    ([4, 200], 5, 16, 40, 2, 80, 1),            # 100 rows of one key head: several tiles
+    ([3000], 1, 128, 2, 2, 64, 1),
+]
+
+
+def make_paged(lengths, new, page, hq, hk, d, dtype, seed, spare=2):
+    """Streams whose pages lie in a random order in a cache that holds NaN wherever no stream's key is."""
+    need = [-(-n // page) for n in lengths]
+    pages, width = sum(need) + spare, max(max(need), 1) + 1
+    order = torch.randperm(pages, generator=torch.Generator().manual_seed(seed)).tolist()
+    kc, vc = make_cache(pages, page, hk, d, dtype, seed)
+    used = torch.zeros(pages, page, dtype=torch.bool)
+    table = torch.full((len(lengths), width), -1, dtype=torch.int32)
+    for b, n in enumerate(lengths):
+        for j in range(need[b]):
+            pg = order.pop()
+            table[b, j] = pg
+            used[pg, :min(page, n - j * page)] = True
+    kc[~used.to(DEV)] = math.nan
+    vc[~used.to(DEV)] = math.nan
+    q = randn(len(lengths), new, hq, d, dtype=dtype, seed=seed + 5, scale=1.5)
+    return q, kc, vc, table.to(DEV), torch.tensor(lengths, dtype=torch.int32, device=DEV)
+
+
+@pytest.mark.parametrize('dtype', DTYPES, ids=IDS)
+@pytest.mark.parametrize('lengths,new,page,hq,hk,d,frame', PAGED)
+def test_paged_attention(dtype, lengths, new, page, hq, hk, d, frame):
+    q, kc, vc, table, lens = make_paged(lengths, new, page, hq, hk, d, dtype, 110)
+    out = ops.paged_attention(q, kc, vc, table, lens, frame=frame)
+    want, bound = OS.paged(q, kc, vc, table, lens, frame)
+    within(out, want, bound, 'out')
+    wide = torch.cat([table, torch.full((len(lengths), 700), -1, dtype=torch.int32, device=DEV)], 1)     # room for much longer streams
+    within(ops.paged_attention(q, kc, vc, wide, lens.long(), frame=frame), want, bound, 'wide table')
+    qt = q.transpose(1, 2).contiguous().transpose(1, 2)
+    assert torch.equal(ops.paged_attention(qt, kc, vc, table, lens, frame=frame), out)
+
+
+@pytest.mark.parametrize('dtype', DTYPES, ids=IDS)
+def test_paged_attention_bad_pages_and_lengths(dtype):
+    """Pages outside the cache hold no keys; a length beyond the table's pages is cut to them, a negative one is 0."""
+    q, kc, vc, table, _ = make_paged([200, 200, 64, 64], 1, 16, 4, 2, 32, dtype, 120)
+    table[0, 3] = kc.shape[0]
+    table[0, 7] = -5
+    table[1, :] = 2 ** 31 - 1
+    lens = torch.tensor([200, 200, -3, 10 ** 9], dtype=torch.int32, device=DEV)
+    out = ops.paged_attention(q, kc, vc, table, lens, frame=1)
+    want, bound = OS.paged(q, kc, vc, table, lens, 1)
+    within(out, want, bound, 'out')
+    assert (out[1] == 0).all() and (out[2] == 0).all()
+
+
+@pytest.mark.parametrize('dtype', DTYPES, ids=IDS)
+def test_paged_attention_hides_later_new_tokens(dtype):
+    """Of several new tokens the earlier ones do not see the later ones' keys, whatever these hold."""
+    q, kc, vc, table, lens = make_paged([67], 3, 16, 2, 2, 32, dtype, 130)
+    want, bound = OS.paged(q, kc, vc, table, lens, 1)
+    pg, row = int(table[0, 66 // 16]), 66 % 16
+    kc[pg, row], vc[pg, row] = math.nan, math.inf
+    out = ops.paged_attention(q, kc, vc, table, lens, frame=1)
+    within(out[:, :2], want[:, :2], bound[:, :2], 'earlier tokens')
+    assert torch.isnan(out[:, 2]).all()
+
+
+def test_paged_attention_far_pages():
+    """Pages behind 2^31 elements of the cache, written by rotary_append and read back."""
+    page, hk, d = 64, 8, 128
+    pages = (1 << 31) // (page * hk * d) + 5
+    kc, vc = (torch.empty(pages, page, hk, d, device=DEV, dtype=torch.bfloat16) for _ in range(2))
+    n = 150
+    table = torch.tensor([[pages - 1, 0, pages - 3]], dtype=torch.int32, device=DEV)
+    q, k, v = (randn(n, hk, d, dtype=torch.bfloat16, seed=140 + i) for i in range(3))
+    pos, freqs = torch.arange(n, device=DEV)[:, None].contiguous(), ops.rotary_freqs((64,))
+    seq, index = torch.zeros(n, dtype=torch.int32, device=DEV), torch.arange(n, dtype=torch.int32, device=DEV)
+    turned = ops.rotary_append(q, k, v, pos, freqs, (64,), kc, vc, table, seq, index)
+    out = ops.paged_attention(turned[-1:][None], kc, vc, table, torch.tensor([n], device=DEV), frame=1)
+    tq, tk = ops.rotary(q, k, pos, freqs, (64,))
+    assert torch.equal(tq, turned)
+    want = OS.packed(tq, tk, v, [0, n], 1)
+    within(out[0, 0], want['out'][-1], want['out_b'][-1], 'far pages')
+
+
+# ------------------------------------------------------------------------------------------------ the four of them in a row
+def project(x, w, hq, hk, d):
+    qkv = (x.float() @ w).to(x.dtype).view(x.shape[0], hq + 2 * hk, d)
+    return qkv[:, :hq], qkv[:, hq:hq + hk], qkv[:, hq + hk:]
+
+
+@pytest.mark.parametrize('dtype', DTYPES, ids=IDS)
+@pytest.mark.parametrize('ntok,page,hq,hk', [(3, 16, 8, 8), (1, 7, 4, 2)])
+def test_streaming_equals_the_whole_video(dtype, ntok, page, hq, hk):
+    """Two layers of attention, causal by frame, over three videos of different lengths at once (rotary + packed_attention) and frame by
+    frame over a paged cache (rotary_append + paged_attention): the second layer reads the first one's outputs, so both sides' bounds are
+    carried through one layer by the reference run on the first side's own first-layer output."""
+    d, sections, frames = 32, (12, 4), [9, 30, 1]
+    lengths = [f * ntok for f in frames]
+    c, t = cum(lengths), sum(lengths)
+    x = randn(t, hq * d, dtype=dtype, seed=150)
+    w = [randn(hq * d, (hq + 2 * hk) * d, dtype=torch.float32, seed=151 + i, scale=(hq * d) ** -0.5) for i in range(2)]
+    step = torch.cat([torch.arange(n) for n in lengths]).to(DEV)
+    pos = torch.stack([step // ntok, step % ntok], 1).contiguous()
+    freqs = ops.rotary_freqs(sections)
+    cu = cu_tensor(c)
+    whole, y, inputs = [], x, []
+    for i in range(2):
+        q, k, v = project(y, w[i], hq, hk, d)
+        q, k = ops.rotary(q, k, pos, freqs, sections)
+        inputs.append((q, k, v))
+        y = ops.packed_attention(q, k, v, cu, frame=ntok).view(t, hq * d)
+        whole.append(y)
+    width = -(-max(lengths) // page)
+    caches = [make_cache(3 * width, page, hk, d, dtype, 160 + 2 * i) for i in range(2)]
+    table = torch.randperm(3 * width, generator=torch.Generator().manual_seed(5)).view(3, width).int().to(DEV)
+    got = torch.zeros_like(x)
+    for f in range(max(frames)):
+        live = [b for b in range(3) if f < frames[b]]
+        rows = torch.tensor([c[b] + f * ntok + j for b in live for j in range(ntok)], device=DEV)
+        seq = torch.tensor([b for b in live for _ in range(ntok)], dtype=torch.int32, device=DEV)
+        index = step[rows].int()
+        lens = torch.full((len(live),), (f + 1) * ntok, dtype=torch.int32, device=DEV)
+        y = x[rows]
+        for i in range(2):
+            # the second layer starts from the whole run's first layer, so that the two sides differ by one layer's roundings
+            q, k, v = project(y if i == 0 else whole[0][rows], w[i], hq, hk, d)
+            q = ops.rotary_append(q, k, v, pos[rows], freqs, sections, *caches[i], table, seq, index)
+            out = ops.paged_attention(q.view(len(live), ntok, hq, d), *caches[i], table[live], lens, frame=ntok)
+            y = out.view(len(rows), hq * d)
+            if i == 0:
+                first = OS.packed(*inputs[0], c, ntok) if f == 0 else first
+                within(y.view(-1, hq, d), first['out'][rows.cpu()], 2 * first['out_b'][rows.cpu()] + 1e-6, 'first layer, frame %d' % f)
+        got[rows] = y
+    second = OS.packed(*inputs[1], c, ntok)
+    within(got.view(t, hq, d), second['out'], 2 * second['out_b'] + 1e-6, 'second layer')
+
+
+def test_training_through_rotary_and_attention():
+    """Gradients of a projection, rotary positions and attention in a row, against the same composition in 64 bits by autograd."""
+    hq, hk, d, sections, c = 4, 2, 32, (10, 6), cum([30, 7, 51])
+    t = c[-1]
+    x = randn(t, 64, dtype=torch.float32, seed=170)
+    w = randn(64, (hq + 2 * hk) * d, dtype=torch.float32, seed=171, scale=0.1).requires_grad_()
+    pos, freqs = positions(t, 2, torch.int64, 9, 172), ops.rotary_freqs(sections)
+    wo = randn(t, hq, d, dtype=torch.float32, seed=173)
+    q, k, v = project(x, w, hq, hk, d)
+    q, k = ops.rotary(q, k, pos, freqs, sections)
+    out = ops.packed_attention(q, k, v, cu_tensor(c), frame=3)
+    g, = torch.autograd.grad(out, w, wo)
+
+    w64 = w.detach().double().cpu().requires_grad_()
+    qkv = (x.double().cpu() @ w64).view(t, hq + 2 * hk, d)
+    ang = torch.cat([pos.cpu()[:, a:a + 1].double() * freqs.cpu()[s:s + m] for a, (s, m) in enumerate(((0, 10), (10, 6)))], 1)[:, None]
+
+    def turn(z):
+        a, b = z[..., :16], z[..., 16:]
+        return torch.cat([a * ang.cos() - b * ang.sin(), b * ang.cos() + a * ang.sin()], -1)
+    q64, k64, v64, loss = turn(qkv[:, :hq]), turn(qkv[:, hq:hq + hk]), qkv[:, hq + hk:], 0
+    for a, b in zip(c[:-1], c[1:]):
+        i = torch.arange(b - a)
+        mask = i[None] < (i[:, None] // 3 + 1) * 3
+        for h in range(hq):
+            s = (q64[a:b, h] @ k64[a:b, h // 2].t() * d ** -0.5).masked_fill(~mask, -math.inf)
+            loss = loss + ((s.softmax(1) @ v64[a:b, h // 2]) * wo[a:b, h].double().cpu()).sum()
+    g64, = torch.autograd.grad(loss, w64)
+    # every element is a sum over t rows of 32-bit quantities that carry some hundred roundings each (projection 64, score 32, softmax,
+    # products over the sequence): 2^-24 * 512 of the largest gradient
+    assert (g.double().cpu() - g64).abs().max().item() <= 512 * OS.U32 * g64.abs().max().item()
+
+
+# ------------------------------------------------------------------------------------------------ streams, graphs, repetition
+def test_same_bits_every_time():
+    c = cum([700, 3, 1000])
+    t = c[-1]
+    q, k, v, do = (randn(t, h, 64, dtype=torch.bfloat16, seed=180 + i) for i, h in enumerate((8, 2, 2, 8)))
+    a, b = (run_packed(q, k, v, cu_tensor(c), 1, do) for _ in range(2))
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+    p = make_paged([5000, 300], 1, 16, 8, 2, 64, torch.bfloat16, 190)
+    assert torch.equal(ops.paged_attention(*p, frame=1), ops.paged_attention(*p, frame=1))
+
+
+def test_another_stream():
+    p = make_paged([3000, 70], 1, 16, 8, 2, 64, torch.float32, 200)
+    want = ops.paged_attention(*p, frame=1)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        outs = [ops.paged_attention(*p, frame=1) for _ in range(3)]
+    outs.append(ops.paged_attention(*p, frame=1))              # at the same time on the default stream: workspaces of their own
+    torch.cuda.current_stream().wait_stream(s)
+    assert all(torch.equal(want, o) for o in outs)
+
+
+def test_graphs_replay_on_new_inputs():
+    """A streaming step (rotary_append + paged_attention) and a training step (forward and gradients) captured into two graphs, replayed in
+    turn with new inputs, new lengths and eager work between; each replay equals the eager result."""
+    hq, hk, d, page, B = 8, 2, 64, 16, 3
+    freqs, sections = ops.rotary_freqs((20, 12)), (20, 12)
+    kc, vc = make_cache(200, page, hk, d, torch.bfloat16, 210)
+    table = torch.randperm(200, generator=torch.Generator().manual_seed(1))[:180].view(3, 60).int().to(DEV)
+    qkv = torch.zeros(B, hq + 2 * hk, d, device=DEV, dtype=torch.bfloat16)
+    pos, index = torch.zeros(B, 2, dtype=torch.int64, device=DEV), torch.zeros(B, dtype=torch.int32, device=DEV)
+    seq, lens = torch.arange(B, dtype=torch.int32, device=DEV), torch.zeros(B, dtype=torch.int32, device=DEV)
+
+    def serve():
+        q = ops.rotary_append(qkv[:, :hq], qkv[:, hq:hq + hk], qkv[:, hq + hk:], pos, freqs, sections, kc, vc, table, seq, index)
+        return ops.paged_attention(q[:, None], kc, vc, table, lens, frame=1)
+    t = 150
+    xs = [torch.zeros(t, h, d, device=DEV, dtype=torch.float16).requires_grad_() for h in (hq, hk, hk)]
+    do, cu = torch.zeros(t, hq, d, device=DEV, dtype=torch.float16), cu_tensor([0, 1, 2])
+
+    def learn():
+        out = ops.packed_attention(*xs, cu, frame=1)
+        return (out.detach(),) + torch.autograd.grad(out, xs, do)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side), torch.no_grad():
+        serve()
+    with torch.cuda.stream(side):
+        learn()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    g1, g2 = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g1), torch.no_grad():
+        served = serve()
+    with torch.cuda.graph(g2):
+        learned = learn()
+    for i in range(4):
+        qkv.copy_(randn(B, hq + 2 * hk, d, dtype=torch.bfloat16, seed=220 + i))
+        index.copy_(torch.tensor([i, 200 * i, 900 - i], dtype=torch.int32))
+        pos.copy_(torch.stack([index.long() * 3, index.long()], 1))
+        lens.copy_(index + 1)
+        with torch.no_grad():
+            for x, h in zip(xs, (hq, hk, hk)):
+                x.copy_(randn(t, h, d, dtype=torch.float16, seed=230 + 7 * i + h))
+        do.copy_(randn(t, hq, d, dtype=torch.float16, seed=250 + i))
+        cu.copy_(torch.tensor([0, 20 * i + 1, t - i], dtype=torch.int32))
+        g1.replay()
+        g2.replay()
+        a, b = served.clone(), [x.clone() for x in learned]
+        torch.cuda.synchronize()
+        with torch.no_grad():
+            assert torch.equal(a, serve())
+        assert all(torch.equal(x, y) for x, y in zip(b, learn()))

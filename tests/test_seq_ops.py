@@ -1,0 +1,174 @@
+"""What the operators of token sequences refuse, checked without a GPU: argument checks of ops come before any launch, and so do those of the
+C entry points (their pointers are never read here)."""
+import ctypes
+
+import pytest
+import torch
+
+from video_rep_learning_amd import _lib, ops
+
+P = 4096            # an aligned address that nothing reads
+
+
+@pytest.fixture(scope='module')
+def lib():
+    import os
+    if not os.path.exists(_lib.LIB_PATH):
+        from video_rep_learning_amd.csrc import build
+        build.build()
+    return _lib.load()
+
+
+def heads(t=4, h=2, d=32, dtype=torch.float32):
+    return torch.zeros(t, h, d, dtype=dtype)
+
+
+def test_cpu_tensors_are_refused():
+    q, pos = heads(), torch.zeros(4, 1, dtype=torch.int64)
+    freqs = ops.rotary_freqs((16,), device='cpu')
+    cache, table, i = torch.zeros(2, 4, 2, 32), torch.zeros(1, 2, dtype=torch.int32), torch.zeros(4, dtype=torch.int32)
+    with pytest.raises(_lib.MvfError):
+        ops.rotary(q, q, pos, freqs, (16,))
+    with pytest.raises(_lib.MvfError):
+        ops.rotary_append(q, q, q, pos, freqs, (16,), cache, cache, table, i, i)
+    with pytest.raises(_lib.MvfError):
+        ops.packed_attention(q, q, q, torch.tensor([0, 4], dtype=torch.int32))
+    with pytest.raises(_lib.MvfError):
+        ops.paged_attention(q[None], cache, cache, table, torch.tensor([3]))
+
+
+@pytest.mark.parametrize('q,k', [(heads(d=12), heads(d=12)), (heads(h=3), heads(t=5)), (heads(), heads(d=64)), (torch.zeros(4, 32), heads()),
+                                 (heads(h=0), heads()), (heads(d=136), heads(d=136)[:3])])
+def test_shapes_are_refused(q, k):
+    with pytest.raises(ValueError):
+        ops.packed_attention(q, k, k, torch.tensor([0, 4], dtype=torch.int32))
+    with pytest.raises(ValueError):
+        ops.rotary(q, k, torch.zeros(q.shape[0], 1, dtype=torch.int64), ops.rotary_freqs((4,), device='cpu'), (4,))
+
+
+def test_paged_shapes_are_refused():
+    for q in (torch.zeros(1, 32), torch.zeros(1, 1, 2, 36), torch.zeros(1, 1, 2, 136), torch.zeros(1, 0, 2, 32)):
+        with pytest.raises(ValueError):
+            ops.paged_attention(q, torch.zeros(2, 4, 2, 32), torch.zeros(2, 4, 2, 32), torch.zeros(1, 2, dtype=torch.int32), torch.tensor([3]))
+
+
+@pytest.mark.parametrize('frame', [-1, 1.0, True, None, 2 ** 31])
+def test_frame_argument(frame):
+    with pytest.raises(ValueError):
+        ops._frame_arg(frame)
+
+
+@pytest.mark.parametrize('scale', [0.0, -1.0, float('nan'), float('inf')])
+def test_scale_argument(scale):
+    with pytest.raises(ValueError):
+        ops._scale_arg(scale, 64)
+
+
+@pytest.mark.parametrize('sections', [(), (0, 4), (-1,), (17,), (8, 8, 8), (1, 1, 1, 1)])
+def test_sections_argument(sections):
+    q = heads()
+    with pytest.raises(ValueError):
+        ops._rotary_args(torch.zeros(4, len(sections), dtype=torch.int64), torch.zeros(max(1, sum(sections)), dtype=torch.float64), sections, 4, 32, q)
+
+
+def test_positions_and_freqs_arguments():
+    q, f = heads(), ops.rotary_freqs((8, 8), device='cpu')
+    assert f.dtype == torch.float64 and f[0] == 1 and f[8] == 1
+    good = torch.zeros(4, 2, dtype=torch.int64)
+    for pos, freqs in ((good.double(), f), (good[:, :1], f), (good[:3], f), (good, f.float()), (good, f[:15])):
+        with pytest.raises(ValueError):
+            ops._rotary_args(pos, freqs, (8, 8), 4, 32, q)
+
+
+def test_cache_arguments():
+    q = heads()
+    ok = torch.zeros(2, 4, 2, 32)
+    ops._cache_args(q, ok, ok.clone())
+    for kc, vc in ((ok[0], ok), (ok, ok[:1]), (torch.zeros(2, 4, 3, 32),) * 2, (torch.zeros(2, 4, 2, 64),) * 2, (torch.zeros(0, 4, 2, 32),) * 2,
+                   (ok.transpose(1, 2).contiguous().transpose(1, 2), ok)):
+        with pytest.raises(ValueError):
+            ops._cache_args(q, kc, vc)
+
+
+def test_aligned_copies_only_what_it_must():
+    x = torch.zeros(6, 4, 32)
+    assert ops._aligned(x) is x and ops._aligned(x[:, 1:3]).data_ptr() == x[:, 1:3].data_ptr()
+    for y in (x.transpose(1, 2), torch.zeros(6 * 4 * 32 + 1)[1:].view(6, 4, 32), x[:, :1].expand(6, 4, 32), torch.zeros(6, 4, 34)[..., :32]):
+        z = ops._aligned(y)
+        assert z.data_ptr() != y.data_ptr() and z.data_ptr() % 16 == 0 and z.is_contiguous() and torch.equal(z, y)
+
+
+FWD = dict(dtype=_lib.BF16, q=P, ldq=64, hsq=32, k=P, ldk=64, hsk=32, v=P, ldv=64, hsv=32, cu=P, n=1, out=P, stat=None, T=4, Hq=2, Hk=2, D=32,
+           frame=1, scale=1.0)
+BAD_ATTN = [('dtype', 2), ('q', None), ('q', P + 8), ('k', None), ('v', None), ('cu', None), ('out', None), ('out', P + 4), ('ldq', 0), ('ldq', 63),
+            ('hsk', -32), ('ldv', 4), ('n', 0), ('T', 0), ('T', -1), ('Hq', 3), ('Hk', 0), ('frame', -1), ('scale', 0.0), ('scale', float('nan')),
+            ('scale', float('inf'))]
+
+
+@pytest.mark.parametrize('name,value', BAD_ATTN)
+def test_packed_entry_points_refuse(lib, name, value):
+    a = dict(FWD, **{name: value})
+    assert lib.mvf_packed_attn_fwd(*a.values(), None) == 10001
+    head = [a[n] for n in ('dtype', 'q', 'ldq', 'hsq', 'k', 'ldk', 'hsk', 'v', 'ldv', 'hsv', 'cu', 'n', 'out')]
+    tail = [a[n] for n in ('T', 'Hq', 'Hk', 'D', 'frame', 'scale')]
+    assert lib.mvf_packed_attn_bwd(*head, P, P, P, P, P, P, *tail, None) == 10001
+
+
+@pytest.mark.parametrize('d', [0, 12, 136, -8])
+def test_head_sizes_are_declined(lib, d):
+    assert lib.mvf_packed_attn_fwd(*dict(FWD, D=d).values(), None) == 10002
+    assert lib.mvf_paged_attn(_lib.F32, P, 64, 64, 32, P, P, P, P, P, None, 0, 1, 1, 2, 2, d, 1, 16, 1, 1, 1.0, None) == 10002
+
+
+@pytest.mark.parametrize('missing', range(6))
+def test_packed_backward_refuses_missing_buffers(lib, missing):
+    bufs = [P] * 6
+    bufs[missing] = None
+    head = [FWD[n] for n in ('dtype', 'q', 'ldq', 'hsq', 'k', 'ldk', 'hsk', 'v', 'ldv', 'hsv', 'cu', 'n', 'out')]
+    assert lib.mvf_packed_attn_bwd(*head, *bufs, 4, 2, 2, 32, 1, 1.0, None) == 10001
+
+
+ROT = dict(dtype=_lib.F32, q=P, ldq=64, hsq=32, k=P, ldk=64, hsk=32, pos=P, pos_type=0, freqs=P, s0=8, s1=4, s2=0, il=0, inv=0, qo=P, ko=P, T=4,
+           Hq=2, Hk=2, D=32)
+
+
+@pytest.mark.parametrize('name,value', [('dtype', 2), ('q', None), ('k', None), ('pos', None), ('pos_type', 3), ('freqs', None), ('s0', 0), ('s1', 9),
+                                        ('s2', -1), ('qo', None), ('ko', None), ('qo', P + 2), ('T', 0), ('Hq', 0), ('Hk', -1), ('ldq', 65),
+                                        ('hsk', 0), ('D', 0), ('D', 8192)])
+def test_rotary_entry_point_refuses(lib, name, value):
+    assert lib.mvf_rotary(*dict(ROT, **{name: value}).values(), None) == 10001
+
+
+def test_rotary_axes_have_to_follow_each_other(lib):
+    assert lib.mvf_rotary(*dict(ROT, s1=0, s2=4).values(), None) == 10001
+    assert lib.mvf_rotary(*dict(ROT, D=36).values(), None) == 10002
+
+
+def test_append_entry_point_refuses(lib):
+    ok = dict(dtype=_lib.F32, q=P, ldq=64, hsq=32, k=P, ldk=64, hsk=32, v=P, ldv=64, hsv=32, pos=P, pos_type=0, freqs=P, s0=8, s1=4, s2=0, il=0,
+              qo=P, kc=P, vc=P, table=P, width=2, n_seqs=1, seq=P, index=P, n_pages=4, page=16, T=4, Hq=2, Hk=2, D=32)
+    for name, value in (('v', None), ('v', P + 1), ('ldv', 3), ('qo', None), ('kc', None), ('vc', P + 8), ('table', None), ('width', 0), ('n_seqs', 0),
+                        ('seq', None), ('index', None), ('n_pages', 0), ('page', 0), ('Hk', 0), ('T', 0)):
+        assert lib.mvf_rotary_append(*dict(ok, **{name: value}).values(), None) == 10001, name
+
+
+PAGED = dict(dtype=_lib.F32, q=P, qb=64, qn=64, qh=32, kc=P, vc=P, table=P, lens=P, out=P, ws=P, ws_bytes=1 << 30, B=1, n=1, Hq=2, Hk=2, D=32,
+             n_pages=4, page=16, width=2, frame=1, scale=1.0)
+
+
+@pytest.mark.parametrize('name,value', [('dtype', 7), ('q', None), ('q', P + 4), ('kc', None), ('vc', P + 2), ('table', None), ('lens', None),
+                                        ('out', None), ('B', 0), ('n', 0), ('Hq', 3), ('Hk', 0), ('n_pages', 0), ('page', 0), ('width', 0),
+                                        ('frame', -2), ('scale', 0.0), ('qb', 2), ('width', 2 ** 28)])
+def test_paged_entry_point_refuses(lib, name, value):
+    assert lib.mvf_paged_attn(*dict(PAGED, **{name: value}).values(), None) == 10001
+
+
+def test_paged_workspace_is_asked_for_and_checked(lib):
+    size = lib.mvf_paged_attn_workspace_bytes(1, 1, 2, 2, 32, 4096, 16)
+    assert size > 0 and size % 4 == 0
+    long = dict(PAGED, width=4096)
+    assert lib.mvf_paged_attn(*dict(long, ws=None).values(), None) == 10001
+    assert lib.mvf_paged_attn(*dict(long, ws_bytes=size - 1).values(), None) == 10001
+    assert lib.mvf_paged_attn_workspace_bytes(1, 1, 3, 2, 32, 4096, 16) == 0
+    assert lib.mvf_paged_attn_workspace_bytes(64, 1, 8, 8, 128, 1, 16) == 0          # one page per stream: nothing to join
+    assert isinstance(ctypes.c_size_t(size).value, int)

@@ -14,7 +14,7 @@ EPI_STORE, EPI_GELU, EPI_RESID, EPI_PATCH = 0, 1, 2, 3
 _P, _I, _L, _Z, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_long, ctypes.c_size_t, ctypes.c_float
 
 # name -> argument kinds (p pointer, i int, l long, z size_t, f float, u uint64_t); every function returns int
-# except mvf_vit_workspace_bytes (size_t).  Kept in the order of include/mvf_hip.h.
+# except the workspace sizes (size_t).  Kept in the order of include/mvf_hip.h.
 SIGNATURES = {
     'mvf_vit_workspace_bytes': 'iiiii',
     'mvf_vit_fwd': 'pipipppziip',
@@ -120,6 +120,12 @@ SIGNATURES = {
     'mvf_grad_norm': 'pzpppp',
     'mvf_adam_step': 'ppppzfffffifpfip',
     'mvf_optim_set_width': 'i',
+    'mvf_rotary': 'ipllpll' + 'pip' + 'iiiii' + 'pp' + 'iiiip',
+    'mvf_rotary_append': 'ipllpllpll' + 'pip' + 'iiii' + 'ppp' + 'pii' + 'pp' + 'ii' + 'iiiip',
+    'mvf_packed_attn_fwd': 'ipllpllpll' + 'pi' + 'pp' + 'iiiiifp',
+    'mvf_packed_attn_bwd': 'ipllpllpll' + 'pi' + 'ppppppp' + 'iiiiifp',
+    'mvf_paged_attn_workspace_bytes': 'iiiiiii',
+    'mvf_paged_attn': 'iplllppppppz' + 'iiiiiiiiifp',
     'mvf_augment_workspace_bytes': 'iii',
     'mvf_augment_clips': 'ppiiiiippzp',
 }
@@ -221,7 +227,7 @@ def load():
         fn = getattr(lib, name)  # AttributeError if a declared symbol is not exported
         fn.argtypes = [_KIND[k] for k in sig]
         fn.restype = _Z if name in ('mvf_vit_workspace_bytes', 'mvf_bn_workspace_floats', 'mvf_augment_workspace_bytes',
-                                    'mvf_head_pack_elems') else _I
+                                    'mvf_head_pack_elems', 'mvf_paged_attn_workspace_bytes') else _I
     _lib = lib
     return lib
 

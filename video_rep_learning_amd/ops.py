@@ -2179,3 +2179,271 @@ def adam_step(p, g, m, v, lr, beta1, beta2, eps, weight_decay, step, clip=0.0, n
     """zero_grad: the kernel zeroes g as it consumes it (utils.optimizer.FusedAdam: the next zero_grad() becomes free)."""
     call('mvf_adam_step', ptr(p), ptr(g), ptr(m), ptr(v), p.numel(), lr, beta1, beta2, eps, weight_decay, step, clip,
          ptr(norm), gscale, int(zero_grad), stream())
+
+
+# ------------------------------------------------------------------------------------------------
+# Token sequences with positions and a cache: rotary positions, attention over packed sequences, attention over a paged cache
+# ------------------------------------------------------------------------------------------------
+_SEQ_DT = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
+_POS_DT = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
+
+
+def _seq_operands(first, *others):
+    """dtype code of the operands; all of them must be of one type and on one device."""
+    if not first.is_cuda:
+        raise _lib.MvfError('HIP op received a %s tensor (no CPU fallback)' % first.device)
+    code = _SEQ_DT.get(first.dtype)
+    if code is None:
+        raise ValueError('unsupported dtype %s: float32, bfloat16 or float16' % first.dtype)
+    for t in others:
+        if t.dtype != first.dtype:
+            raise ValueError('operands of different types: %s and %s' % (first.dtype, t.dtype))
+        if t.device != first.device:
+            raise _lib.MvfError('operands on different devices: %s and %s' % (first.device, t.device))
+    return code
+
+
+def _index_operand(t, like, shape, what):
+    """An int32 device tensor of the given shape (-1: any size), contiguous."""
+    if t.device != like.device:
+        raise _lib.MvfError('%s on %s, the operands on %s' % (what, t.device, like.device))
+    if t.dtype not in (torch.int32, torch.int64):
+        raise ValueError('%s must be int32 (or int64), got %s' % (what, t.dtype))
+    if t.dim() != len(shape) or any(n >= 0 and n != m for n, m in zip(shape, t.shape)):
+        raise ValueError('%s: expected shape %s, got %s' % (what, shape, tuple(t.shape)))
+    return t.to(torch.int32).contiguous()
+
+
+def _aligned(t):
+    """The tensor itself if its channels are contiguous and every other stride and the start are multiples of 16 bytes, else a copy."""
+    a = 16 // t.element_size()
+    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s > 0 and s % a == 0 for s in t.stride()[:-1]):
+        return t
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _heads(t, what, tokens=None, size=None):
+    if t.dim() != 3 or (tokens is not None and t.shape[0] != tokens) or (size is not None and t.shape[2] != size):
+        raise ValueError('%s: expected [%s, heads, %s], got %s' % (what, 'tokens' if tokens is None else tokens,
+                                                                 'head size' if size is None else size, tuple(t.shape)))
+    if t.shape[1] == 0 or t.shape[2] == 0 or t.shape[2] % 8:
+        raise ValueError('%s: at least one head of a size that is a multiple of 8, got %s' % (what, tuple(t.shape)))
+
+
+def _frame_arg(frame):
+    if not isinstance(frame, int) or isinstance(frame, bool) or not 0 <= frame < 2 ** 31:
+        raise ValueError('frame must be an int >= 0 (0: not causal), got %r' % (frame,))
+    return frame
+
+
+def _scale_arg(scale, d):
+    scale = d ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < 1e30:
+        raise ValueError('scale must be positive and finite, got %r' % (scale,))
+    return scale
+
+
+def _here(t):
+    """Launches go to the operands' device, whichever is current."""
+    return torch.cuda.device(t.device)
+
+
+def rotary_freqs(sections, base=10000.0, device='cuda'):
+    """Angles per unit of position, [sum(sections)] float64: pair j of an axis with n pairs has base ** (-j / n)."""
+    return torch.cat([float(base) ** (-torch.arange(n, dtype=torch.float64) / n) for n in sections]).to(device)
+
+
+def _rotary_args(pos, freqs, sections, tokens, size, like):
+    sections = tuple(int(n) for n in sections)
+    if not 1 <= len(sections) <= 3 or min(sections) <= 0 or 2 * sum(sections) > size:
+        raise ValueError('sections: pairs of one to three axes, at most %d in all, got %s' % (size // 2, sections))
+    if pos.device != like.device or freqs.device != like.device:
+        raise _lib.MvfError('pos on %s, freqs on %s, the operands on %s' % (pos.device, freqs.device, like.device))
+    if pos.dtype not in _POS_DT or tuple(pos.shape) != (tokens, len(sections)):
+        raise ValueError('pos: expected [%d, %d] of int32, int64 or float32, got %s %s' % (tokens, len(sections), tuple(pos.shape), pos.dtype))
+    if freqs.dtype != torch.float64 or tuple(freqs.shape) != (sum(sections),):
+        raise ValueError('freqs: expected [%d] float64, got %s %s' % (sum(sections), tuple(freqs.shape), freqs.dtype))
+    return pos.contiguous(), freqs.contiguous(), sections + (0,) * (3 - len(sections))
+
+
+def _rotary_call(q, k, pos, freqs, sections, interleaved, inverse):
+    q = _aligned(q)
+    k = _aligned(k) if k is not None else None
+    T, Hq, D = q.shape
+    qo = torch.empty(T, Hq, D, device=q.device, dtype=q.dtype)
+    ko = torch.empty(T, k.shape[1], D, device=q.device, dtype=q.dtype) if k is not None else None
+    if T == 0:
+        return qo, ko
+    with _here(q):
+        call('mvf_rotary', _SEQ_DT[q.dtype], q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr() if k is not None else None,
+             k.stride(0) if k is not None else 0, k.stride(1) if k is not None else 0, pos.data_ptr(), _POS_DT[pos.dtype], freqs.data_ptr(),
+             *sections, int(interleaved), int(inverse), qo.data_ptr(), ptr(ko), T, Hq, k.shape[1] if k is not None else 0, D, stream())
+    return qo, ko
+
+
+class _Rotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, pos, freqs, sections, interleaved):
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(pos, freqs)
+        ctx.cfg = (sections, interleaved)
+        return _rotary_call(q, k, pos, freqs, sections, interleaved, False)
+
+    @staticmethod
+    def backward(ctx, dq, dk):
+        pos, freqs = ctx.saved_tensors
+        a = (pos, freqs) + ctx.cfg + (True,)
+        if dq is None:
+            return None, _rotary_call(dk, None, *a)[0] if dk is not None else None, None, None, None, None
+        gq, gk = _rotary_call(dq, dk, *a)
+        return gq, gk, None, None, None, None
+
+
+def rotary(q, k, pos, freqs, sections, interleaved=False):
+    """Rotary positions with one to three axes (time, row, column; or time, entity): q [T, Hq, D], k [T, Hk, D] (or None) turned by
+    pos[t, axis] * freqs[pair] -> new (q, k).  `sections`: pairs of each axis, in the order of pos's columns; channels behind
+    2 * sum(sections) stay.  interleaved: a pair is two neighbouring channels, otherwise channels p and p + sum(sections).  pos [T, axes]
+    int32 / int64 / float32; freqs: rotary_freqs(sections).  fp32, bf16 or fp16; differentiable in q and k."""
+    _heads(q, 'q')
+    if k is not None:
+        _heads(k, 'k', q.shape[0], q.shape[2])
+        _seq_operands(q, k)
+    else:
+        _seq_operands(q)
+    pos, freqs, sections = _rotary_args(pos, freqs, sections, q.shape[0], q.shape[2], q)
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        return _Rotary.apply(q, k, pos, freqs, sections, bool(interleaved))
+    return _rotary_call(q, k, pos, freqs, sections, bool(interleaved), False)
+
+
+def _cache_args(q, k_cache, v_cache):
+    for c, what in ((k_cache, 'k_cache'), (v_cache, 'v_cache')):
+        if c.dim() != 4 or c.shape != k_cache.shape or c.shape[3] != q.shape[-1] or 0 in c.shape or q.shape[-2] % c.shape[2]:
+            raise ValueError('%s: expected [pages, page, key heads, %d], key heads dividing %d, got %s' % (
+                what, q.shape[-1], q.shape[-2], tuple(c.shape)))
+        if not c.is_contiguous() or c.data_ptr() % 16:
+            raise ValueError('%s must be contiguous and start at a multiple of 16 bytes' % what)
+
+
+def rotary_append(q, k, v, pos, freqs, sections, k_cache, v_cache, block_table, seq, index, interleaved=False):
+    """rotary() for new tokens of streams with a paged cache: returns the turned q; the turned k and v go into k_cache, v_cache
+    [pages, page, Hk, D] at index[t] of stream seq[t], i.e. row index % page of page block_table[seq, index // page].  A token whose seq
+    (-1: padding), index or page lies outside is not written.  For inference: no gradient."""
+    _heads(q, 'q')
+    _heads(k, 'k', q.shape[0], q.shape[2])
+    _heads(v, 'v', q.shape[0], q.shape[2])
+    code = _seq_operands(q, k, v, k_cache, v_cache)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        raise ValueError('rotary_append has no gradient: call it under torch.no_grad()')
+    _cache_args(q, k_cache, v_cache)
+    if k.shape[1] != k_cache.shape[2] or v.shape[1] != k_cache.shape[2]:
+        raise ValueError('k and v have %d and %d heads, the cache %d' % (k.shape[1], v.shape[1], k_cache.shape[2]))
+    T, Hq, D = q.shape
+    pos, freqs, sections = _rotary_args(pos, freqs, sections, T, D, q)
+    table = _index_operand(block_table, q, (-1, -1), 'block_table')
+    seq, index = _index_operand(seq, q, (T,), 'seq'), _index_operand(index, q, (T,), 'index')
+    q, k, v = _aligned(q), _aligned(k), _aligned(v)
+    qo = torch.empty(T, Hq, D, device=q.device, dtype=q.dtype)
+    if T == 0:
+        return qo
+    if 0 in table.shape:
+        raise ValueError('block_table is empty: %s' % (tuple(table.shape),))
+    with _here(q):
+        call('mvf_rotary_append', code, q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
+             v.stride(0), v.stride(1), pos.data_ptr(), _POS_DT[pos.dtype], freqs.data_ptr(), *sections, int(interleaved), qo.data_ptr(),
+             k_cache.data_ptr(), v_cache.data_ptr(), table.data_ptr(), table.shape[1], table.shape[0], seq.data_ptr(), index.data_ptr(),
+             k_cache.shape[0], k_cache.shape[1], T, Hq, k.shape[1], D, stream())
+    return qo
+
+
+def _packed_fwd(q, k, v, cu, frame, scale, need_stat):
+    T, Hq, D = q.shape
+    out = torch.empty(T, Hq, D, device=q.device, dtype=q.dtype)
+    stat = torch.empty(2, Hq, T, device=q.device, dtype=torch.float32) if need_stat else None
+    if T:
+        with _here(q):
+            call('mvf_packed_attn_fwd', _SEQ_DT[q.dtype], q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
+                 v.data_ptr(), v.stride(0), v.stride(1), cu.data_ptr(), cu.shape[0] - 1, out.data_ptr(), ptr(stat), T, Hq, k.shape[1], D,
+                 frame, scale, stream())
+    return out, stat
+
+
+class _PackedAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, cu, frame, scale):
+        q, k, v = _aligned(q), _aligned(k), _aligned(v)
+        out, stat = _packed_fwd(q, k, v, cu, frame, scale, True)
+        ctx.save_for_backward(q, k, v, cu, out, stat)
+        ctx.cfg = (frame, scale)
+        return out
+
+    @staticmethod
+    def backward(ctx, d_out):
+        q, k, v, cu, out, stat = ctx.saved_tensors
+        frame, scale = ctx.cfg
+        T, Hq, D = q.shape
+        d_out = d_out.contiguous()
+        if d_out.data_ptr() % 16:
+            d_out = d_out.clone()
+        dq, dk, dv = (torch.empty(x.shape, device=x.device, dtype=x.dtype) for x in (q, k, v))
+        if T:
+            with _here(q):
+                delta = torch.empty(Hq, T, device=q.device, dtype=torch.float32)
+                call('mvf_packed_attn_bwd', _SEQ_DT[q.dtype], q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
+                     v.data_ptr(), v.stride(0), v.stride(1), cu.data_ptr(), cu.shape[0] - 1, out.data_ptr(), d_out.data_ptr(),
+                     stat.data_ptr(), delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), T, Hq, k.shape[1], D, frame, scale,
+                     stream())
+        return dq, dk, dv, None, None, None
+
+
+def packed_attention(q, k, v, cu_seqlens, frame=0, scale=None):
+    """Self-attention over sequences of different lengths packed one behind the other: q [T, Hq, D], k, v [T, Hk, D] (Hq a multiple of
+    Hk: query head h reads key head h // (Hq // Hk)), sequence b in rows cu_seqlens[b] .. cu_seqlens[b + 1] -> [T, Hq, D].
+    frame = 0: a token sees its whole sequence; frame = n: its own and all earlier groups of n tokens of it (1: causal by token; the
+    number of entities: causal by frame).  Rows of no sequence give zeros and get zero gradients.  fp32, bf16 or fp16, D a multiple of 8
+    up to 128; scale: 1 / sqrt(D).  Differentiable in q, k, v, the same bits every time."""
+    _heads(q, 'q')
+    _heads(k, 'k', q.shape[0], q.shape[2])
+    _heads(v, 'v', q.shape[0], q.shape[2])
+    _seq_operands(q, k, v)
+    if k.shape[1] != v.shape[1] or q.shape[1] % k.shape[1]:
+        raise ValueError('%d query heads over %d key and %d value heads' % (q.shape[1], k.shape[1], v.shape[1]))
+    if q.shape[2] > 128:
+        raise ValueError('head size %d: at most 128' % q.shape[2])
+    cu = _index_operand(cu_seqlens, q, (-1,), 'cu_seqlens')
+    if cu.shape[0] < 2:
+        raise ValueError('cu_seqlens needs the bounds of at least one sequence, got %s' % (tuple(cu.shape),))
+    frame, scale = _frame_arg(frame), _scale_arg(scale, q.shape[2])
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return _PackedAttention.apply(q, k, v, cu, frame, scale)
+    return _packed_fwd(_aligned(q), _aligned(k), _aligned(v), cu, frame, scale, False)[0]
+
+
+def paged_attention(q, k_cache, v_cache, block_table, lengths, frame=1, scale=None):
+    """Attention of the last n tokens of each stream over its pages of the cache: q [B, n, Hq, D] are the queries of positions
+    lengths[b] - n .. lengths[b] - 1 (whose keys and values are in the cache already: rotary_append), k_cache, v_cache
+    [pages, page, Hk, D], block_table [B, pages of a stream], lengths [B] -> [B, n, Hq, D].  frame as in packed_attention; a stream of
+    length 0 gives zeros.  For inference: no gradient."""
+    if q.dim() != 4 or 0 in q.shape[1:] or q.shape[3] % 8 or q.shape[3] > 128:
+        raise ValueError('q: expected [streams, new tokens, heads, head size (a multiple of 8 up to 128)], got %s' % (tuple(q.shape),))
+    code = _seq_operands(q, k_cache, v_cache)
+    if torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad):
+        raise ValueError('paged_attention has no gradient: call it under torch.no_grad()')
+    _cache_args(q, k_cache, v_cache)
+    B, n, Hq, D = q.shape
+    table, lens = _index_operand(block_table, q, (B, -1), 'block_table'), _index_operand(lengths, q, (B,), 'lengths')
+    frame, scale = _frame_arg(frame), _scale_arg(scale, D)
+    out = torch.empty(B, n, Hq, D, device=q.device, dtype=q.dtype)
+    if B == 0:
+        return out
+    n_pages, page, Hk, width = k_cache.shape[0], k_cache.shape[1], k_cache.shape[2], table.shape[1]
+    if width == 0:
+        raise ValueError('block_table has no columns')
+    q = _aligned(q)
+    with _here(q):
+        need = _lib.load().mvf_paged_attn_workspace_bytes(B, n, Hq, Hk, D, width, page)
+        ws = torch.empty(need, device=q.device, dtype=torch.uint8) if need else None
+        call('mvf_paged_attn', code, q.data_ptr(), q.stride(0), q.stride(1), q.stride(2), k_cache.data_ptr(), v_cache.data_ptr(),
+             table.data_ptr(), lens.data_ptr(), out.data_ptr(), ptr(ws), need, B, n, Hq, Hk, D, n_pages, page, width, frame, scale, stream())
+    return out
