@@ -136,6 +136,7 @@ LENGTHS = {
     'edges': [63, 64, 65, 127, 129],
     'long': [300, 1, 517],
     'many': [3] * 70,
+    'wide': [300, 1, 0, 33, 129, 64, 517, 31] * 4,      # with 16 heads: enough rows for the form whose workgroups own 128
 }
 PACKED = [  # lengths, hq, hk, d, frame
     ('one', 1, 1, 8, 1), ('one', 4, 2, 64, 0),
@@ -143,6 +144,7 @@ PACKED = [  # lengths, hq, hk, d, frame
     ('edges', 2, 2, 64, 1), ('edges', 6, 2, 128, 1), ('edges', 2, 1, 80, 7),
     ('long', 2, 2, 32, 6), ('long', 3, 1, 64, 0), ('long', 2, 2, 128, 100000),
     ('many', 2, 2, 16, 1), ('many', 5, 5, 48, 2),
+    ('wide', 16, 16, 32, 1), ('wide', 16, 16, 64, 0), ('wide', 32, 16, 80, 3), ('wide', 16, 16, 128, 1), ('wide', 18, 9, 24, 0),
 ]
 
 
@@ -169,12 +171,12 @@ def test_packed_attention_and_its_gradients(dtype, lengths, hq, hk, d, frame):
 
 
 @pytest.mark.parametrize('dtype', DTYPES, ids=IDS)
-@pytest.mark.parametrize('frame', [0, 1, 4])
-def test_packed_attention_leaves_rows_of_no_sequence_alone(dtype, frame):
+@pytest.mark.parametrize('frame,behind,hq,hk', [(0, 61, 4, 2), (1, 61, 4, 2), (4, 61, 4, 2), (1, 4100, 16, 16)])
+def test_packed_attention_leaves_rows_of_no_sequence_alone(dtype, frame, behind, hq, hk):
     """Rows before the first and behind the last sequence hold NaN (uninitialised padding): zeros out, zero gradients, and the rows of
     sequences come out as if the others were not there."""
     c = cum([40, 0, 75], first=3)
-    t, hq, hk, d = c[-1] + 61, 4, 2, 64
+    t, d = c[-1] + behind, 64
     q, k, v, do = (randn(t, h, d, dtype=dtype, seed=30 + i) for i, h in enumerate((hq, hk, hk, hq)))
     for x in (q, k, v, do):
         x[:3] = math.nan
@@ -219,9 +221,10 @@ def test_packed_attention_hides_what_a_row_does_not_see(dtype, bad):
 
 
 @pytest.mark.parametrize('dtype', DTYPES, ids=IDS)
-def test_packed_attention_gradients_hide_other_sequences(dtype):
+@pytest.mark.parametrize('lengths,hq,hk', [([45, 30, 90], 4, 2), ([450, 35] + [100] * 37, 16, 16)], ids=['split', 'wide'])
+def test_packed_attention_gradients_hide_other_sequences(dtype, lengths, hq, hk):
     """A sequence whose inputs or output gradients are not finite leaves its neighbours' gradients as they are."""
-    c, hq, hk, d = cum([45, 30, 90]), 4, 2, 64
+    c, d = cum(lengths), 64
     t = c[-1]
     q, k, v, do = (randn(t, h, d, dtype=dtype, seed=50 + i) for i, h in enumerate((hq, hk, hk, hq)))
     want = OS.packed(q, k, v, c, 1, do=do)

@@ -24,13 +24,14 @@ struct PagedArgs {
   float c;
 };
 
-template <int DT, int DP>
+template <int DT, int DP, bool PAD>
 __global__ __launch_bounds__(64 * NW, 1) void paged_attn_kernel(PagedArgs a) {
   typedef Op<DT> O;
   typedef Img<O, DP> I;
-  constexpr int ROWF = DP + 4;                       // floats per row of the joining area
+  typedef Tiles<O, DP> S;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   __shared__ float s_m[NW][32], s_l[NW][32];
+  __shared__ int s_tab[NW][2][64];                    // page ids of a tile's 32 keys (twice)
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 31, hh = lane >> 5;
   const int split = blockIdx.x % a.splits, unit = blockIdx.x / a.splits;
@@ -47,6 +48,7 @@ __global__ __launch_bounds__(64 * NW, 1) void paged_attn_kernel(PagedArgs a) {
   int hi_all = m < a.R ? hi : 0x7fffffff;            // keys that every row sees
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) hi_all = min(hi_all, __shfl_xor(hi_all, o, 64));
+  hi_all = __builtin_amdgcn_readfirstlane(hi_all);
   typename O::Frag qf[DP / 16];
   {
     const char* src = a.q + b * a.qb + (long)min(mi, a.n - 1) * a.qn + (kh * a.g + m % a.g) * a.qh;
@@ -58,8 +60,9 @@ __global__ __launch_bounds__(64 * NW, 1) void paged_attn_kernel(PagedArgs a) {
       qf[ks] = f;
     }
   }
-  char* sk = smem + wave * 64 * I::RB;
-  char* sv = sk + 32 * I::RB;
+  if constexpr (PAD) clear_lds(smem, NW * S::NB * S::BUF);
+#pragma unroll
+  for (int ks = 0; ks < DP / 16; ++ks) asm volatile("" : "+v"(qf[ks]));      // landed before any DMA is in flight
   f32x16_t o[DP / 32];
 #pragma unroll
   for (int dt = 0; dt < DP / 32; ++dt) o[dt] = zero16();
@@ -69,35 +72,35 @@ __global__ __launch_bounds__(64 * NW, 1) void paged_attn_kernel(PagedArgs a) {
   const char* kb = a.k + (long)kh * a.D * O::SZ;
   const char* vb = a.v + (long)kh * a.D * O::SZ;
   const int* tab = a.table + (long)b * a.width;
+  const uint32_t lds = lds_addr(smem) + wave * S::NB * S::BUF, tlds = lds_addr(&s_tab[wave][0][0]);
+  const uint32_t rpart = I::row_part(lane), cpart = I::col_part(lane);
 
-  constexpr int NL = I::C / 2;                       // 16-byte pieces per lane of 32 rows
-  uint4 kr[NL], vr[NL];
-  uint32_t there = 0, there_next = 0;                // which of the tile's 32 keys exist
-  auto load = [&](int t) __attribute__((always_inline)) {
-    const int key = t * 32 + r;
-    long off = -1;
-    if (key < len) {
-      const int pg = tab[key / a.page];
-      if (pg >= 0 && pg < a.n_pages) off = ((long)pg * a.page + key % a.page) * row_bytes;
-    }
-    there_next = (uint32_t)__builtin_amdgcn_ballot_w64(off >= 0);
-    const int lo32 = (int)off, hi32 = (int)(off >> 32);
-#pragma unroll
-    for (int i = 0; i < NL; ++i) {
-      const int row = (i * 64 + lane) / I::C, ch = (i * 64 + lane) % I::C;
-      const long at = (long)(((uint64_t)(uint32_t)__shfl(hi32, row, 64) << 32) | (uint32_t)__shfl(lo32, row, 64));
-      kr[i] = vr[i] = make_uint4(0, 0, 0, 0);
-      if (at >= 0 && ch * 16 < a.D * O::SZ) {
-        kr[i] = *reinterpret_cast<const uint4*>(kb + at + ch * 16);
-        vr[i] = *reinterpret_cast<const uint4*>(vb + at + ch * 16);
-      }
-    }
+  auto ask_pages = [&](int t, int buf) __attribute__((always_inline)) {
+    dma4(reinterpret_cast<const float*>(tab + min((t * 32 + r) / a.page, a.width - 1)), tlds + buf * 256);
   };
-  auto tile = [&](auto mask_tag, int t) __attribute__((always_inline)) {
+  // where the tile's 32 keys lie, from the page ids; returns which of them exist (an absent one repeats one that does)
+  auto place = [&](int t, int pg, long& off) __attribute__((always_inline)) {
+    const int key = t * 32 + r;
+    const bool is = key < len && pg >= 0 && pg < a.n_pages;
+    const uint32_t there = (uint32_t)__builtin_amdgcn_ballot_w64(is);
+    off = is ? ((long)pg * a.page + key % a.page) * row_bytes : 0;
+    const int from = is ? r : there != 0 ? __builtin_ctz(there) : r;
+    off = (long)(((uint64_t)(uint32_t)__shfl((int)(off >> 32), from, 64) << 32) | (uint32_t)__shfl((int)off, from, 64));
+    return there;
+  };
+  auto ask_rows = [&](long off, int buf) __attribute__((always_inline)) {
+    const int lo32 = (int)off, hi32 = (int)(off >> 32);
+    S::template issue<PAD>(kb, vb, [&](int i, long& oa, long& ob) {
+      oa = ob = (long)(((uint64_t)(uint32_t)__shfl(hi32, i, 64) << 32) | (uint32_t)__shfl(lo32, i, 64));
+    }, a.D, lane, lds + buf * S::BUF);
+  };
+  bool bad = false;
+  auto tile = [&](auto mask_tag, int t, uint32_t there, uint32_t ik) __attribute__((always_inline)) {
     constexpr bool MASK = decltype(mask_tag)::value;
+    const uint32_t rp = launder(rpart), cp = launder(cpart);
     f32x16_t s = zero16();
 #pragma unroll
-    for (int ks = 0; ks < DP / 16; ++ks) s = O::mma(I::rows(sk, 0, ks, lane), qf[ks], s);
+    for (int ks = 0; ks < DP / 16; ++ks) s = O::mma(I::rows(ik, rp, ks), qf[ks], s);
     if constexpr (MASK) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
@@ -121,75 +124,92 @@ __global__ __launch_bounds__(64 * NW, 1) void paged_attn_kernel(PagedArgs a) {
       s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.c, st.nm));
       st.l += s[e];
     }
-#pragma unroll
-    for (int s2 = 0; s2 < 2; ++s2) {
-      const typename O::Frag p = O::pack(s, s2);
-#pragma unroll
-      for (int dt = 0; dt < DP / 32; ++dt) o[dt] = mma_weighted<O, MASK, false>(I::cols(sv, 16 * s2, dt, lane), p, o[dt]);
-    }
+    accumulate<O, DP>(o, s, ik + S::IMG, cp);
+    if constexpr (MASK) bad |= tile_nonfinite<O, DP>(ik + S::IMG, lane);
   };
-  int t = split * per + wave;
-  if (t < t_end) load(t);
-  for (; t < t_end; t += NW) {
-#pragma unroll
-    for (int i = 0; i < NL; ++i) {
-      const int row = (i * 64 + lane) / I::C, ch = (i * 64 + lane) % I::C;
-      *reinterpret_cast<uint4*>(sk + I::off(row, ch)) = kr[i];
-      *reinterpret_cast<uint4*>(sv + I::off(row, ch)) = vr[i];
+
+  // Per tile: its page ids are asked for two tiles ahead, its rows one tile ahead (where the buffers allow two tiles).
+  const int t0 = split * per + wave;
+  int buf = 0;
+  uint32_t there = 0, next = 0;
+  long off;
+  if (t0 < t_end) {
+    ask_pages(t0, 0);
+    ask_pages(t0 + NW, 1);
+    wait_dma<1>();
+    there = place(t0, s_tab[wave][0][lane], off);
+    ask_rows(off, 0);
+  }
+  for (int t = t0, i = 0; t < t_end; t += NW, ++i) {
+    const bool more = t + NW < t_end;
+    const uint32_t ik = lds + buf * S::BUF;
+    if (S::NB == 2 && more) {
+      wait_dma<S::NP>();                             // the next tile's page ids are older than this tile's rows
+      next = place(t + NW, s_tab[wave][(i + 1) & 1][lane], off);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      ask_pages(t + 2 * NW, i & 1);
+      ask_rows(off, buf ^ 1);
+      wait_dma<S::NP + 1>();
+    } else {
+      wait_dma<0>();
     }
-    there = there_next;
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the wave's own stores, before its other lanes read them
-    if (t + NW < t_end) load(t + NW);
-    if (there == 0xffffffffu && t * 32 + 32 <= hi_all) tile(std::false_type{}, t);
-    else tile(std::true_type{}, t);
+    if (there == 0xffffffffu && t * 32 + 32 <= hi_all) tile(std::false_type{}, t, there, ik);
+    else if (there != 0) tile(std::true_type{}, t, there, ik);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-  }
-  // ---- the four waves' parts ----
-  const float l = pair_sum(st.l);
-  __syncthreads();
-  float* so = reinterpret_cast<float*>(smem);           // [NW][32][ROWF]
-  if (hh == 0) { s_m[wave][r] = st.m == NEG_INF ? NEG_INF : -st.nm; s_l[wave][r] = l; }
-  if (r < rows) {
-#pragma unroll
-    for (int dt = 0; dt < DP / 32; ++dt)
-#pragma unroll
-      for (int g = 0; g < 4; ++g)
-        *reinterpret_cast<f32x4_t*>(so + (wave * 32 + r) * ROWF + 32 * dt + 8 * g + 4 * hh) =
-            (f32x4_t){o[dt][4 * g], o[dt][4 * g + 1], o[dt][4 * g + 2], o[dt][4 * g + 3]};
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < rows * (DP / 4); i += 64 * NW) {
-    const int row = i / (DP / 4), d = i % (DP / 4) * 4;
-    if (d >= a.D) continue;
-    float mx = NEG_INF;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) mx = fmaxf(mx, s_m[w][row]);
-    float sum = 0.f;
-    f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int w = 0; w < NW; ++w) {
-      const float f = s_m[w][row] == NEG_INF ? 0.f : __builtin_amdgcn_exp2f(s_m[w][row] - mx);
-      if (s_m[w][row] == NEG_INF && !(s_l[w][row] != s_l[w][row])) continue;
-      sum += f * s_l[w][row];
-      const f32x4_t x = *reinterpret_cast<const f32x4_t*>(so + (w * 32 + row) * ROWF + d);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[j] = fmaf(f, x[j], acc[j]);
+    if (S::NB == 2) {
+      buf ^= 1;
+    } else if (more) {
+      next = place(t + NW, s_tab[wave][(i + 1) & 1][lane], off);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      ask_pages(t + 2 * NW, i & 1);
+      ask_rows(off, 0);
     }
+    there = next;
+  }
+  if (bad) {                                          // a value that is not finite beside masked places: visible pairs only
+#pragma unroll
+    for (int dt = 0; dt < DP / 32; ++dt) o[dt] = zero16();
+    st = RowMax();
+#pragma unroll 1
+    for (int t = t0; t < t_end; t += NW)
+#pragma unroll 1
+      for (int key = t * 32; key < min(t * 32 + 32, len); ++key) {
+        const int pg = tab[key / a.page];
+        if (pg < 0 || pg >= a.n_pages) continue;
+        const long at = ((long)pg * a.page + key % a.page) * row_bytes;
+        const float s = slow_dot<O, DP>(qf, kb + at, a.D, hh);
+        if (key >= hi) continue;
+        const float to = fmaxf(st.m, s);
+        const float alpha = st.m == NEG_INF ? 0.f : __builtin_amdgcn_exp2f((st.m - to) * a.c);
+        st.m = to;
+        st.nm = to == NEG_INF ? 0.f : -to * a.c;
+        const float p = __builtin_amdgcn_exp2f(fmaf(s, a.c, st.nm));
+        st.l = fmaf(st.l, alpha, hh == 0 ? p : 0.f);
+#pragma unroll
+        for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[dt][e] *= alpha;
+        slow_add<O, DP>(o, p, vb + at, a.D, hh);
+      }
+  }
+  __syncthreads();
+  join_waves<DP>(reinterpret_cast<float*>(smem), s_m, s_l, o, st, rows, a.D, wave, lane,
+                 [&](int row, int d, const f32x4_t& acc, float mx, float l) {
     const int mm = m0 + row;
     if (a.splits == 1) {
-      const float inv = sum != 0.f ? 1.f / sum : 0.f;
-      typename O::E* dst = reinterpret_cast<typename O::E*>(a.out) + (((long)b * a.n + mm / a.g) * a.Hq + kh * a.g + mm % a.g) * a.D + d;
-      O::store4(dst, acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
+      const float inv = l != 0.f ? 1.f / l : 0.f;
+      O::store4(reinterpret_cast<typename O::E*>(a.out) + (((long)b * a.n + mm / a.g) * a.Hq + kh * a.g + mm % a.g) * a.D + d, acc[0] * inv,
+                acc[1] * inv, acc[2] * inv, acc[3] * inv);
     } else {
       const size_t prow = (((size_t)b * a.Hk + kh) * a.R + mm) * a.splits + split;
       *reinterpret_cast<f32x4_t*>(a.part + prow * a.D + d) = acc;
       if (d == 0) {
         float* ml = a.part + (size_t)a.B * a.Hk * a.R * a.splits * a.D + prow * 2;
         ml[0] = mx;
-        ml[1] = sum;
+        ml[1] = l;
       }
     }
-  }
+  });
 }
 
 // one workgroup per row: the splits' weights, then D channels x 8 groups of splits
@@ -242,13 +262,13 @@ int split_count(long units, long max_keys) {
   return (int)std::max(1l, std::min({std::max(fill, (max_keys + 1023) / 1024), most, 256l}));
 }
 
-template <int DT, int DP>
+template <int DT, int DP, bool PAD>
 int launch(const PagedArgs& a, hipStream_t st) {
-  typedef Img<Op<DT>, DP> I;
-  const size_t lds = std::max((size_t)NW * 64 * I::RB, (size_t)NW * 32 * (DP + 4) * 4);
+  typedef Tiles<Op<DT>, DP> S;
+  const size_t lds = std::max(NW * S::NB * S::BUF, JOIN_BYTES<DP>);
   static uint64_t attr = 0;
-  if (int rc = mvf_ensure_lds(reinterpret_cast<const void*>(paged_attn_kernel<DT, DP>), lds, attr)) return rc;
-  hipLaunchKernelGGL((paged_attn_kernel<DT, DP>), dim3((unsigned)a.B * a.Hk * a.rt * a.splits), dim3(64 * NW), lds, st, a);
+  if (int rc = mvf_ensure_lds(reinterpret_cast<const void*>(paged_attn_kernel<DT, DP, PAD>), lds, attr)) return rc;
+  hipLaunchKernelGGL((paged_attn_kernel<DT, DP, PAD>), dim3((unsigned)a.B * a.Hk * a.rt * a.splits), dim3(64 * NW), lds, st, a);
   MVF_LAUNCH_CHECK();
   if (a.splits > 1) {
     hipLaunchKernelGGL((paged_join_kernel<DT>), dim3((unsigned)a.B * a.Hk * a.R), dim3(256), 0, st, a);
@@ -256,9 +276,11 @@ int launch(const PagedArgs& a, hipStream_t st) {
   }
   return MVF_OK;
 }
+template <int DT, int DP>
+int launch_p(const PagedArgs& a, hipStream_t st) { return a.D == DP ? launch<DT, DP, false>(a, st) : launch<DT, DP, true>(a, st); }
 template <int DT>
 int launch_d(const PagedArgs& a, hipStream_t st) {
-  return a.D <= 32 ? launch<DT, 32>(a, st) : a.D <= 64 ? launch<DT, 64>(a, st) : a.D <= 96 ? launch<DT, 96>(a, st) : launch<DT, 128>(a, st);
+  return a.D <= 32 ? launch_p<DT, 32>(a, st) : a.D <= 64 ? launch_p<DT, 64>(a, st) : a.D <= 96 ? launch_p<DT, 96>(a, st) : launch_p<DT, 128>(a, st);
 }
 
 }  // namespace

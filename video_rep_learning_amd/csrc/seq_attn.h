@@ -19,6 +19,8 @@ namespace seq_attn {
 
 typedef __attribute__((ext_vector_type(16))) float f32x16_t;
 typedef __attribute__((ext_vector_type(8))) float f32x8_t;
+typedef __attribute__((ext_vector_type(4))) uint32_t u32x4_t;
+typedef __attribute__((ext_vector_type(2))) uint32_t u32x2_t;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float NEG_INF = -__builtin_huge_valf();
 
@@ -55,20 +57,23 @@ struct Op16 {
     for (int j = 0; j < 4; ++j) f.u[j] = pack16x2<F16>(x[8 * s + 2 * j], x[8 * s + 2 * j + 1]);
     return f.v;
   }
-  static constexpr uint32_t EXP = F16 ? 0x7c007c00u : 0x7f807f80u, ONE = F16 ? 0x04000400u : 0x00800080u;
-  static __device__ __forceinline__ bool any_nonfinite(const Frag& a) {
-    union { Frag v; uint32_t u[4]; } f;
-    f.v = a;
-    uint32_t bad = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) bad |= (f.u[j] & EXP) + ONE;     // an all-ones exponent carries into the sign bit
-    return (bad & 0x80008000u) != 0;
+  // a 16-byte chunk holds a NaN or an infinity: an all-ones exponent carries into the sign bit
+  static __device__ __forceinline__ bool nonfinite(const u32x4_t& x) {
+    constexpr uint32_t EXP = F16 ? 0x7c007c00u : 0x7f807f80u, ONE = F16 ? 0x04000400u : 0x00800080u;
+    return ((((x.x & EXP) + ONE) | ((x.y & EXP) + ONE) | ((x.z & EXP) + ONE) | ((x.w & EXP) + ONE)) & 0x80008000u) != 0;
+  }
+  // four elements as fp32
+  static __device__ __forceinline__ f32x4_t load4(const char* p) {
+    const u32x2_t u = *reinterpret_cast<const u32x2_t*>(p);
+    float x[4];
+    unpack16x2<F16>(u.x, x[0], x[1]);
+    unpack16x2<F16>(u.y, x[2], x[3]);
+    return (f32x4_t){x[0], x[1], x[2], x[3]};
   }
   static __device__ __forceinline__ float get(const Frag& a, int j) {
     const uint16_t x = (uint16_t)a[j];
     return F16 ? f16_to_f32(x) : bf16_to_f32(x);
   }
-  static __device__ __forceinline__ void set(Frag& a, int j, float x) { a[j] = (short)(F16 ? f32_to_f16(x) : f32_to_bf16(x)); }
   static __device__ __forceinline__ void store4(E* p, float a, float b, float c, float d) {
     *reinterpret_cast<uint2*>(p) = make_uint2(pack16x2<F16>(a, b), pack16x2<F16>(c, d));
   }
@@ -95,14 +100,12 @@ struct Op<MVF_F32> {
     for (int j = 0; j < 8; ++j) f[j] = x[8 * s + j];
     return f;
   }
-  static __device__ __forceinline__ bool any_nonfinite(const Frag& a) {
-    bool bad = false;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) bad |= !(fabsf(a[j]) < __builtin_huge_valf());
-    return bad;
+  static __device__ __forceinline__ bool nonfinite(const u32x4_t& x) {
+    constexpr uint32_t EXP = 0x7f800000u, ONE = 0x00800000u;
+    return ((((x.x & EXP) + ONE) | ((x.y & EXP) + ONE) | ((x.z & EXP) + ONE) | ((x.w & EXP) + ONE)) & 0x80000000u) != 0;
   }
+  static __device__ __forceinline__ f32x4_t load4(const char* p) { return *reinterpret_cast<const f32x4_t*>(p); }
   static __device__ __forceinline__ float get(const Frag& a, int j) { return a[j]; }
-  static __device__ __forceinline__ void set(Frag& a, int j, float x) { a[j] = x; }
   static __device__ __forceinline__ void store4(E* p, float a, float b, float c, float d) {
     *reinterpret_cast<float4*>(p) = make_float4(a, b, c, d);
   }
@@ -115,87 +118,211 @@ __device__ __forceinline__ f32x16_t zero16() {
   return z;
 }
 
-// acc + A . B where B holds weights that are exactly 0 in masked places and A the data those weights multiply.  0 * NaN is NaN, so a
-// NaN or infinity of a key that a row must not see would reach it through the product.  In tiles with masked places (SAFE) non-finite
-// data is therefore taken out of A and put back where its weight is not 0: counts of +inf, -inf and NaN per accumulator element come
-// out of one more product (at most 16 of each per step: 1, 64 and 4096 do not meet).  SIGNED: weights of both signs (the gradients'):
-// any of them makes the element NaN.
-template <class O, bool SAFE, bool SIGNED>
-__device__ __forceinline__ f32x16_t mma_weighted(const typename O::Frag& data, const typename O::Frag& w, const f32x16_t& acc) {
-  if constexpr (!SAFE) {
-    return O::mma(data, w, acc);
-  } else {
-    if (__builtin_amdgcn_ballot_w64(O::any_nonfinite(data)) == 0) return O::mma(data, w, acc);
-    typename O::Frag fin = data, mark, hit;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float x = O::get(data, j), p = O::get(w, j);
-      const bool bad = !(fabsf(x) < __builtin_huge_valf());
-      if (bad) O::set(fin, j, 0.f);
-      O::set(mark, j, !bad ? 0.f : (SIGNED || x != x) ? 4096.f : x > 0.f ? 1.f : 64.f);
-      O::set(hit, j, p == 0.f ? 0.f : 1.f);
-    }
-    f32x16_t out = O::mma(fin, w, acc);
-    const f32x16_t m = O::mma(mark, hit, zero16());
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const int n = (int)m[e];
-      const bool pos = (n & 63) != 0, neg = ((n >> 6) & 63) != 0;
-      if (n != 0) out[e] += (n >= 4096 || (pos && neg)) ? __builtin_nanf("") : pos ? __builtin_huge_valf() : -__builtin_huge_valf();
-    }
-    return out;
-  }
-}
-
 // ---------------------------------------------------------------------------------------------- LDS images
 // Rows of DP elements in 16-byte chunks, chunk c of row i stored at c ^ swz(i).  Two kinds of reads have to be free of bank conflicts:
 //   row fragments: ds_read_b128, 16 lanes at a time, one chunk of 16 different rows;
 //   transposed fragments: ds_read_b64_tr_b16, 32 lanes at a time, 4 consecutive rows x 64 bytes (4 aligned chunks).
 // A row of C chunks starts at chunk position C * i (mod 16, the 256 bytes of the banks); swz fills the positions that leaves.
+// An address inside an image is a lane part XOR a constant plus a constant, so one register per kind of read serves all fragments; launder()
+// keeps the compiler from holding every sum in a register of its own across the loop.
+typedef __attribute__((address_space(3))) const char* lds_t;
+__device__ __forceinline__ lds_t lds_at(uint32_t a) { return (lds_t)(uintptr_t)a; }
+__device__ __forceinline__ uint32_t lds_addr(const void* p) { return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)p; }
+template <class T>
+__device__ __forceinline__ T lds_read(uint32_t a) { return *reinterpret_cast<__attribute__((address_space(3))) const T*>(lds_at(a)); }
+__device__ __forceinline__ uint32_t launder(uint32_t x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
 template <class O, int DP>
 struct Img {
   static constexpr int RB = DP * O::SZ, C = RB / 16;
+  static constexpr int M = C == 4 || C == 12 ? 3 : C == 8 || C == 24 ? 7 : 15;       // chunk bits that swz touches
   static __device__ __forceinline__ int swz(int i) {
-    if constexpr (C == 4 || C == 12) return (i >> 2) & 3;
-    else if constexpr (C == 8 || C == 24) return (((i >> 1) & 1) << 2) | ((i >> 2) & 3);
+    if constexpr (M == 3) return (i >> 2) & 3;
+    else if constexpr (M == 7) return (((i >> 1) & 1) << 2) | ((i >> 2) & 3);
     else return ((i & 3) << 2) | ((i >> 2) & 3);
   }
   static __device__ __forceinline__ int off(int i, int c) { return i * RB + ((c ^ swz(i)) << 4); }
-  // A operand = 32 rows of the image from row0 on: lane (r, h) <- X[row0 + r][16 ks + 8h .. + 8]
-  static __device__ __forceinline__ typename O::Frag rows(const char* img, int row0, int ks, int lane) {
-    const int i = row0 + (lane & 31), h = lane >> 5;
+  // chunk c of a row whose lane part is `lane_part`: the low bits meet swz, the others are added
+  static __device__ __forceinline__ uint32_t at(uint32_t lane_part, int c, int x, uint32_t base) {
+    return (lane_part ^ (uint32_t)(((c & M) ^ x) << 4)) + base + (uint32_t)((c & ~M) << 4);
+  }
+  // A operand = 32 rows of the image from `img` on: lane (r, h) <- X[r][16 ks + 8h .. + 8]
+  static __device__ __forceinline__ uint32_t row_part(int lane) { return off(lane & 31, (lane >> 5) * (O::SZ / 2)); }
+  static __device__ __forceinline__ typename O::Frag rows(uint32_t img, uint32_t part, int ks) {
     if constexpr (O::SZ == 2) {
-      return *reinterpret_cast<const bf16x8_t*>(img + off(i, 2 * ks + h));
+      return lds_read<bf16x8_t>(at(part, 2 * ks, 0, img));
     } else {
-      const f32x4_t a = *reinterpret_cast<const f32x4_t*>(img + off(i, 4 * ks + 2 * h));
-      const f32x4_t b = *reinterpret_cast<const f32x4_t*>(img + off(i, 4 * ks + 2 * h + 1));
+      const f32x4_t a = lds_read<f32x4_t>(at(part, 4 * ks, 0, img)), b = lds_read<f32x4_t>(at(part, 4 * ks + 1, 0, img));
       return (f32x8_t){a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
     }
   }
-  // A operand = the image transposed, columns 32 dt .. + 32 on the rows, the 16 image rows from row0 on in the accumulators' order on k
-  static __device__ __forceinline__ typename O::Frag cols(const char* img, int row0, int dt, int lane) {
-    const int h = lane >> 5;
+  // A operand = the image transposed, columns 32 dt .. + 32 on the rows, rows 16 s .. + 16 of the image in the accumulators' order on k
+  static __device__ __forceinline__ uint32_t col_part(int lane) {
+    const int h = lane >> 5, li = lane & 15;
+    if constexpr (O::SZ == 2) return off(4 * h + (li >> 2), 2 * ((lane >> 4) & 1) + ((li & 3) >> 1)) + 8 * (li & 1);
+    else return off(4 * h, (lane & 31) >> 2) + 4 * (lane & 3);
+  }
+  static __device__ __forceinline__ typename O::Frag cols(uint32_t img, uint32_t part, int s, int dt) {
     if constexpr (O::SZ == 2) {
-      const int li = lane & 15, g = (lane >> 4) & 1;
       union { bf16x8_t v; bf16x4_t q[2]; } f;
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int i = row0 + 8 * j + 4 * h + (li >> 2), c = 4 * dt + 2 * g + ((li & 3) >> 1);
-        f.q[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) bf16x4_t*)(img + off(i, c) + 8 * (li & 1)));
-      }
+      for (int j = 0; j < 2; ++j)
+        f.q[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) bf16x4_t*)lds_at(
+            at(part, 4 * dt, 2 * j, img) + (16 * s + 8 * j) * RB));
       return f.v;
     } else {
       f32x8_t f;
-      const int d = 32 * dt + (lane & 31);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int i = row0 + (j < 4 ? 4 * h + j : 8 + 4 * h + j - 4);
-        f[j] = *reinterpret_cast<const float*>(img + off(i, d >> 2) + 4 * (d & 3));
+      for (int j = 0; j < 8; ++j) {     // row 16 s + 8 (j >> 2) + 4 h + (j & 3)
+        const int x = (M == 7 ? ((j >> 1) & 1) << 2 : (j & 3) << 2) ^ (2 * (j >> 2));
+        f[j] = lds_read<float>(at(part, 8 * dt, x, img) + (16 * s + 8 * (j >> 2) + (j & 3)) * RB);
       }
       return f;
     }
   }
 };
+
+// acc (rows d, columns owned) += X^T w over a 32-row tile X of an image, w its weights in accumulator order.  Weights are exactly 0 in masked
+// places, but 0 * NaN is NaN: through the product a NaN or infinity of a row would reach the columns that must not see it.  So in
+// tiles with masked places the kernels look for non-finite values, and a wave that met one goes over its rows again, element by
+// element and visible pairs only (their slow()), after the loop.
+template <class O, int DP>
+__device__ __forceinline__ void accumulate(f32x16_t (&acc)[DP / 32], const f32x16_t& w, uint32_t img, uint32_t part) {
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    const typename O::Frag b = O::pack(w, s);
+#pragma unroll
+    for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = O::mma(Img<O, DP>::cols(img, part, s, dt), b, acc[dt]);
+  }
+}
+template <class O, int DP>
+__device__ __forceinline__ bool tile_nonfinite(uint32_t img, int lane) {
+  typedef Img<O, DP> I;
+  bool bad = false;
+#pragma unroll 2
+  for (int i = 0; i < I::C / 2; ++i) bad |= O::nonfinite(lds_read<u32x4_t>(img + (i * 64 + lane) * 16));
+  return __builtin_amdgcn_ballot_w64(bad) != 0;
+}
+// the slow forms' pieces: a dot product of a row in fragments with a row in memory (whole in both lanes of a pair), and acc += w * row
+template <class O, int DP>
+__device__ __forceinline__ float slow_dot(const typename O::Frag (&f)[DP / 16], const char* row, int D, int hh) {
+  float s = 0.f;
+#pragma unroll
+  for (int ks = 0; ks < DP / 16; ++ks) {
+    const int d = 16 * ks + 8 * hh;
+    if (d < D) {
+      const typename O::Frag x = *reinterpret_cast<const typename O::Frag*>(row + d * O::SZ);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s = fmaf(O::get(f[ks], j), O::get(x, j), s);
+    }
+  }
+  return pair_sum(s);
+}
+template <class O, int DP>
+__device__ __forceinline__ void slow_add(f32x16_t (&acc)[DP / 32], float w, const char* row, int D, int hh) {
+#pragma unroll
+  for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int d = 32 * dt + 8 * g + 4 * hh;
+      if (d < D) {
+        const f32x4_t x = O::load4(row + d * O::SZ);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[dt][4 * g + j] = fmaf(w, x[j], acc[dt][4 * g + j]);
+      }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------- streaming
+// One LDS-DMA piece: 64 lanes x 16 bytes from per-lane addresses to 1 KiB of LDS at the wave-uniform byte address `lds`; a lane that
+// is switched off leaves its 16 bytes as they were.  Written in assembly because behind the builtin the compiler orders every later
+// transposing LDS read after ALL outstanding DMAs; the counted waits and barriers below order them.  (s_nop: no hazards are padded
+// around inline assembly.)
+__device__ __forceinline__ void dma16(const char* src, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(__builtin_amdgcn_readfirstlane(lds)) : "memory");
+}
+__device__ __forceinline__ void dma4(const float* src, uint32_t lds) {      // 64 lanes x 4 bytes
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 4\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(__builtin_amdgcn_readfirstlane(lds)) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void wait_dma() {           // all but the wave's last N pieces have landed, its LDS reads have too
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+}
+
+// A workgroup of four waves streams blocks of KB rows of two matrices (a and b) through a ring of three buffers: waves 0 and 1 fetch a's
+// pieces, waves 2 and 3 b's, block n + 2 is asked for right behind the one barrier of block n.  A row behind the last one repeats it;
+// chunks behind the row's D elements are not fetched (the caller cleared the buffers once).
+template <class O, int DP>
+struct Ring {
+  typedef Img<O, DP> I;
+  static constexpr int KB = I::RB <= 64 ? 128 : I::RB <= 128 ? 64 : 32;
+  static constexpr int IMG = KB * I::RB, BUF = 2 * IMG, NB = 3, PP = IMG / 2048;     // PP: pieces per wave and block
+  const char* p[PP];
+  long ld;
+  uint32_t on, lds;
+  __device__ __forceinline__ void start(const char* a, long lda, const char* b, long ldb, int row, int D, int wave, int lane, uint32_t lds0) {
+    ld = wave < 2 ? lda : ldb;
+    const char* base = (wave < 2 ? a : b) + (long)row * ld;
+    lds = lds0 + wave * PP * 1024;
+    on = 0;
+#pragma unroll
+    for (int j = 0; j < PP; ++j) {
+      const int idx = ((wave & 1) * PP + j) * 64 + lane, r = idx / I::C, ch = (idx % I::C) ^ I::swz(r);
+      p[j] = base + r * ld + ch * 16;
+      on |= (uint32_t)(ch * 16 < D * O::SZ) << j;
+    }
+  }
+  // block of rows [row, row + KB) of the rows before `end`, into buffer `buf`
+  template <bool PAD>
+  __device__ __forceinline__ void issue(int row, int end, int buf, int wave, int lane) {
+    const bool last = row + KB > end;
+    lane = launder(lane);
+#pragma unroll
+    for (int j = 0; j < PP; ++j) {
+      const char* q = p[j];
+      if (last) {
+        const int over = row + (((wave & 1) * PP + j) * 64 + lane) / I::C - (end - 1);
+        if (over > 0) q -= over * ld;
+      }
+      if (!PAD || ((on >> j) & 1)) dma16(q, lds + buf * BUF + j * 1024);
+      p[j] += KB * ld;
+    }
+  }
+};
+
+// A wave streams 32-row tiles of two matrices through buffers of its own (one or two): no barrier, nothing shared.
+template <class O, int DP>
+struct Tiles {
+  typedef Img<O, DP> I;
+  static constexpr int IMG = 32 * I::RB, BUF = 2 * IMG, NB = I::RB <= 256 ? 2 : 1, NP = I::C;    // NP: pieces per tile
+  template <bool PAD, class RowAt>      // RowAt(i): byte offsets of the tile's row i in a and in b
+  static __device__ __forceinline__ void issue(const char* a, const char* b, RowAt&& at, int D, int lane, uint32_t lds) {
+#pragma unroll
+    for (int j = 0; j < NP / 2; ++j) {
+      const int idx = j * 64 + lane, r = idx / I::C, ch = (idx % I::C) ^ I::swz(r);
+      long oa, ob;
+      at(r, oa, ob);
+      if (!PAD || ch * 16 < D * O::SZ) {
+        dma16(a + oa + ch * 16, lds + j * 1024);
+        dma16(b + ob + ch * 16, lds + IMG + j * 1024);
+      }
+    }
+  }
+};
+
+__device__ __forceinline__ void clear_lds(char* p, int bytes) {
+  for (int i = threadIdx.x * 16; i < bytes; i += blockDim.x * 16) *reinterpret_cast<uint4*>(p + i) = make_uint4(0, 0, 0, 0);
+  __syncthreads();
+}
+
+// blockIdx -> unit such that every XCD (workgroups go round them) gets a contiguous run of units: neighbours share keys and values
+__device__ __forceinline__ int xcd_unit(int units) {
+  const int per = (units + 7) >> 3, slot = blockIdx.x >> 3, u = (blockIdx.x & 7) * per + slot;
+  return slot < per && u < units ? u : -1;
+}
+static inline unsigned xcd_grid(long units) { return (unsigned)((units + 7) / 8 * 8); }
 
 // ---------------------------------------------------------------------------------------------- which rows meet
 struct Span { int lo, hi; };
@@ -257,5 +384,58 @@ struct RowMax {
     return true;
   }
 };
+
+// union of the four waves' spans (a barrier inside)
+__device__ __forceinline__ Span block_span(const WaveSpan& ws, int* s_span, int lane, int wave, int nw) {
+  if (lane == 0) { s_span[2 * wave] = ws.any.hi > 0 ? ws.any.lo : 0x7fffffff; s_span[2 * wave + 1] = ws.any.hi; }
+  __syncthreads();
+  Span s = {0x7fffffff, 0};
+  for (int w = 0; w < nw; ++w) { s.lo = min(s.lo, s_span[2 * w]); s.hi = max(s.hi, s_span[2 * w + 1]); }
+  // nothing: {0, 0}, so that sums with .lo stay in range
+  return {__builtin_amdgcn_readfirstlane(s.hi == 0 ? 0 : s.lo), __builtin_amdgcn_readfirstlane(s.hi)};
+}
+
+// Four waves hold partial softmaxes of the same 32 rows: sums o^T against their own maxima.  Joins them in LDS (fixed order) and hands
+// use(row, first channel of four, unnormalised sums, maximum in the exponent's units, sum of weights) for every row and channel.  All
+// threads; the caller's earlier LDS reads are behind a barrier.
+template <int DP>
+constexpr int JOIN_BYTES = 4 * 32 * (DP + 4) * 4;
+template <int DP, class Use>
+__device__ __forceinline__ void join_waves(float* so, float (*s_m)[32], float (*s_l)[32], const f32x16_t (&o)[DP / 32], const RowMax& st,
+                                           int rows, int D, int wave, int lane, Use&& use) {
+  constexpr int ROWF = DP + 4;
+  const int r = lane & 31, hh = lane >> 5;
+  const float l = pair_sum(st.l);
+  if (hh == 0) { s_m[wave][r] = st.m == NEG_INF ? NEG_INF : -st.nm; s_l[wave][r] = l; }
+  if (r < rows) {
+#pragma unroll
+    for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<f32x4_t*>(so + (wave * 32 + r) * ROWF + 32 * dt + 8 * g + 4 * hh) =
+            (f32x4_t){o[dt][4 * g], o[dt][4 * g + 1], o[dt][4 * g + 2], o[dt][4 * g + 3]};
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < rows * (DP / 4); i += 256) {
+    const int row = i / (DP / 4), d = i % (DP / 4) * 4;
+    if (d >= D) continue;
+    float mx = NEG_INF;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) mx = fmaxf(mx, s_m[w][row]);
+    float sum = 0.f;
+    f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float m = s_m[w][row], lw = s_l[w][row];
+      if (m == NEG_INF && lw == lw) continue;                 // saw nothing (a NaN sum with no maximum saw a NaN)
+      const float f = m == NEG_INF ? lw : __builtin_amdgcn_exp2f(m - mx);
+      sum = fmaf(f, lw, sum);
+      const f32x4_t x = *reinterpret_cast<const f32x4_t*>(so + (w * 32 + row) * ROWF + d);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[j] = fmaf(f, x[j], acc[j]);
+    }
+    use(row, d, acc, mx, sum);
+  }
+}
 
 }  // namespace seq_attn

@@ -3,6 +3,11 @@
 // Tiles are cut out of the packed rows, not out of each sequence: a tile may hold the end of one sequence and the start of the next,
 // every row has its own [lo, hi) of keys, and a tile walks the union.  So nothing but the number of rows sizes the grid (no host copy
 // of the lengths), empty sequences cost nothing, short ones share a tile, and rows behind the last sequence come out as zeros.
+//
+// Two forms of the same tile arithmetic:
+//   wide:   a workgroup owns 128 rows of one head (32 per wave) and its waves share each block of keys;
+//   split:  a workgroup owns 32 rows, each wave walks every fourth 32-key tile by itself, the four partial softmaxes are joined at the
+//           end: four times as many workgroups and a quarter of the dependent steps, for four times the key traffic.
 #include "mvf_hip_internal.h"
 #include "seq_attn.h"
 
@@ -15,46 +20,31 @@ struct FwdArgs {
   const int* cu;
   int n_seqs;
   char* out;                           // [T, Hq, D]
-  float* stat;                         // NULL, or [2][Hq][T]: see below
+  float* stat;                         // NULL, or [2][Hq][T]: see finish()
   int T, Hq, Hk, D, frame, ntiles;
   float c;                             // scale * log2(e)
 };
 
-// rows [row0, row0 + ROWS) of a strided matrix into an image; rows from `end` on and columns from D on are zeros
-template <class O, int DP, int ROWS>
-__device__ __forceinline__ void stage(char* img, const char* src, long ld, int row0, int end, int D, int tid, int nthreads) {
-  typedef Img<O, DP> I;
-  for (int i = tid; i < ROWS * I::C; i += nthreads) {
-    const int r = i / I::C, ch = i % I::C;
-    uint4 x = make_uint4(0, 0, 0, 0);
-    if (row0 + r < end && ch * 16 < D * O::SZ) x = *reinterpret_cast<const uint4*>(src + (long)(row0 + r) * ld + ch * 16);
-    *reinterpret_cast<uint4*>(img + I::off(r, ch)) = x;
-  }
-}
-
 template <int DT, int DP>
-__global__ __launch_bounds__(256, 1) void packed_attn_fwd_kernel(FwdArgs a) {
+struct Fwd {
   typedef Op<DT> O;
   typedef Img<O, DP> I;
-  constexpr int KROWS = 64;
-  extern __shared__ __attribute__((aligned(16))) char smem[];
-  __shared__ int s_span[8];
-  char* sk = smem;
-  char* sv = smem + KROWS * I::RB;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nw = blockDim.x >> 6;
-  const int r = lane & 31, hh = lane >> 5;
-  const int head = blockIdx.x % a.Hq, tile = a.ntiles - 1 - (int)(blockIdx.x / a.Hq);
-  const int row = (tile * nw + wave) * 32 + r;
-  Span own = {0, 0};
-  if (row < a.T) own = keys_of(sequence_of(a.cu, a.n_seqs, a.T, row), a.frame, row);
-  const WaveSpan ws = wave_span(own);
-  if (lane == 0) { s_span[2 * wave] = ws.any.hi > 0 ? ws.any.lo : 0x7fffffff; s_span[2 * wave + 1] = ws.any.hi; }
-  __syncthreads();
-  int lo = 0x7fffffff, hi = 0;
-  for (int w = 0; w < nw; ++w) { lo = min(lo, s_span[2 * w]); hi = max(hi, s_span[2 * w + 1]); }
-
   typename O::Frag qf[DP / 16];
-  {
+  f32x16_t o[DP / 32];
+  RowMax st;
+  Span own;
+  float c, thr;
+  int lane;
+  uint32_t rpart, cpart;
+  bool bad = false;        // a tile with masked places held a value that is not finite
+
+  __device__ __forceinline__ void start(const FwdArgs& a, int head, int row, int lane_) {
+    lane = lane_;
+    rpart = I::row_part(lane);
+    cpart = I::col_part(lane);
+    c = a.c;
+    thr = 8.f / a.c;
+    const int hh = lane >> 5;
     const char* src = a.q + (long)min(row, a.T - 1) * a.ldq + head * a.hsq;
 #pragma unroll
     for (int ks = 0; ks < DP / 16; ++ks) {
@@ -63,24 +53,19 @@ __global__ __launch_bounds__(256, 1) void packed_attn_fwd_kernel(FwdArgs a) {
       if (d < a.D && own.hi > 0) f = *reinterpret_cast<const typename O::Frag*>(src + d * O::SZ);
       qf[ks] = f;
     }
+#pragma unroll
+    for (int dt = 0; dt < DP / 32; ++dt) o[dt] = zero16();
   }
-  f32x16_t o[DP / 32];
-#pragma unroll
-  for (int dt = 0; dt < DP / 32; ++dt) o[dt] = zero16();
-  RowMax st;
-  const float thr = 8.f / a.c;
-  const char* kb = a.k + (head / (a.Hq / a.Hk)) * a.hsk;
-  const char* vb = a.v + (head / (a.Hq / a.Hk)) * a.hsv;
-
-  auto tile32 = [&](auto mask_tag, int t, int key0) __attribute__((always_inline)) {
-    constexpr bool MASK = decltype(mask_tag)::value;
+  template <bool MASK>
+  __device__ __forceinline__ void tile(uint32_t ik, uint32_t iv, int key0) {
     f32x16_t s = zero16();
+    const uint32_t rp = launder(rpart), cp = launder(cpart);
 #pragma unroll
-    for (int ks = 0; ks < DP / 16; ++ks) s = O::mma(I::rows(sk, t * 32, ks, lane), qf[ks], s);
+    for (int ks = 0; ks < DP / 16; ++ks) s = O::mma(I::rows(ik, rp, ks), qf[ks], s);
     if constexpr (MASK) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        const int key = key0 + 8 * (e >> 2) + 4 * hh + (e & 3);
+        const int key = key0 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
         s[e] = key >= own.lo && key < own.hi ? s[e] : NEG_INF;
       }
     }
@@ -89,7 +74,7 @@ __global__ __launch_bounds__(256, 1) void packed_attn_fwd_kernel(FwdArgs a) {
     for (int e = 1; e < 16; ++e) mx = fmaxf(mx, s[e]);
     mx = pair_max(mx);
     float alpha;
-    if (st.grow(mx, a.c, thr, alpha)) {
+    if (st.grow(mx, c, thr, alpha)) {
 #pragma unroll
       for (int dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
@@ -97,67 +82,193 @@ __global__ __launch_bounds__(256, 1) void packed_attn_fwd_kernel(FwdArgs a) {
     }
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
-      s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.c, st.nm));
+      s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], c, st.nm));
       st.l += s[e];
     }
+    accumulate<O, DP>(o, s, iv, cp);
+    if constexpr (MASK) bad |= tile_nonfinite<O, DP>(iv, lane);
+  }
+  // the same rows over 32-key tiles first, first + step, ..., one visible pair at a time
+  __device__ __forceinline__ void slow(const FwdArgs& a, const char* kb, const char* vb, int first, int step, int end) {
 #pragma unroll
-    for (int s2 = 0; s2 < 2; ++s2) {
-      const typename O::Frag p = O::pack(s, s2);
+    for (int dt = 0; dt < DP / 32; ++dt) o[dt] = zero16();
+    st = RowMax();
+#pragma unroll 1
+    for (int k0 = first; k0 < end; k0 += step)
+#pragma unroll 1
+      for (int key = k0; key < min(k0 + 32, end); ++key) {
+        const float s = slow_dot<O, DP>(qf, kb + (long)key * a.ldk, a.D, lane >> 5);
+        if (key < own.lo || key >= own.hi) continue;
+        const float to = fmaxf(st.m, s);
+        const float alpha = st.m == NEG_INF ? 0.f : __builtin_amdgcn_exp2f((st.m - to) * c);
+        st.m = to;
+        st.nm = to == NEG_INF ? 0.f : -to * c;
+        const float p = __builtin_amdgcn_exp2f(fmaf(s, c, st.nm));
+        st.l = fmaf(st.l, alpha, lane < 32 ? p : 0.f);                  // the pair's sum is taken at the end
 #pragma unroll
-      for (int dt = 0; dt < DP / 32; ++dt) o[dt] = mma_weighted<O, MASK, false>(I::cols(sv, t * 32 + 16 * s2, dt, lane), p, o[dt]);
-    }
-  };
+        for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[dt][e] *= alpha;
+        slow_add<O, DP>(o, p, vb + (long)key * a.ldv, a.D, lane >> 5);
+      }
+  }
+  __device__ __forceinline__ void any_tile(const WaveSpan& ws, uint32_t ik, uint32_t iv, int key0) {
+    if (key0 >= ws.any.hi || key0 + 32 <= ws.any.lo) return;
+    if (key0 >= ws.all.lo && key0 + 32 <= ws.all.hi) tile<false>(ik, iv, key0);
+    else tile<true>(ik, iv, key0);
+  }
+};
 
-  for (int b0 = lo; b0 < hi; b0 += KROWS) {
-    __syncthreads();
-    stage<O, DP, KROWS>(sk, kb, a.ldk, b0, hi, a.D, threadIdx.x, blockDim.x);
-    stage<O, DP, KROWS>(sv, vb, a.ldv, b0, hi, a.D, threadIdx.x, blockDim.x);
-    __syncthreads();
-    for (int t = 0; t < KROWS / 32; ++t) {
-      const int key0 = b0 + 32 * t;
-      if (key0 >= ws.any.hi || key0 + 32 <= ws.any.lo) continue;
-      if (key0 >= ws.all.lo && key0 + 32 <= ws.all.hi) tile32(std::false_type{}, t, key0);
-      else tile32(std::true_type{}, t, key0);
-    }
+// What the backward needs to have the same probabilities again.  fp32: the exponent's offset and 1 / l, applied as in the forward (one
+// log2-sum would round at the size of its integer part: 1e-6 of a probability); 16-bit: one offset that holds both.
+template <int DT>
+__device__ __forceinline__ void store_stat(const FwdArgs& a, int head, int row, float nm, float l, bool some) {
+  const size_t at = (size_t)head * a.T + row;
+  a.stat[at] = !some ? NEG_INF : DT == MVF_F32 ? nm : nm - __builtin_amdgcn_logf(l);
+  a.stat[(size_t)a.Hq * a.T + at] = some ? 1.0f / l : 0.f;
+}
+
+template <int DT, int DP, bool PAD>
+__global__ __launch_bounds__(256, DT == MVF_F32 && DP > 64 ? 1 : 2) void packed_attn_fwd_kernel(FwdArgs a) {
+  typedef Op<DT> O;
+  typedef Img<O, DP> I;
+  typedef Ring<O, DP> R;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  __shared__ int s_span[8];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int u = xcd_unit(a.ntiles * a.Hq);
+  if (u < 0) return;
+  const int head = u / a.ntiles, tile = a.ntiles - 1 - u % a.ntiles;       // the longest walks (causal: the last rows) first
+  const int row = (tile * 4 + wave) * 32 + (lane & 31);
+  Fwd<DT, DP> f;
+  f.own = {0, 0};
+  if (row < a.T) f.own = keys_of(sequence_of(a.cu, a.n_seqs, a.T, row), a.frame, row);
+  const WaveSpan ws = wave_span(f.own);
+  f.start(a, head, row, lane);
+  if constexpr (PAD) clear_lds(smem, R::NB * R::BUF);
+  const Span span = block_span(ws, s_span, lane, wave, 4);
+  const int g = a.Hq / a.Hk;
+#pragma unroll
+  for (int ks = 0; ks < DP / 16; ++ks) asm volatile("" : "+v"(f.qf[ks]));      // landed before any DMA is in flight
+  const char *kb = a.k + head / g * a.hsk, *vb = a.v + head / g * a.hsv;
+  R ring;
+  ring.start(kb, a.ldk, vb, a.ldv, span.lo, a.D, wave, lane, lds_addr(smem));
+  if (span.lo < span.hi) ring.template issue<PAD>(span.lo, span.hi, 0, wave, lane);
+  if (span.lo + R::KB < span.hi) ring.template issue<PAD>(span.lo + R::KB, span.hi, 1, wave, lane);
+  int buf = 0;
+  for (int b0 = span.lo; b0 < span.hi; b0 += R::KB) {
+    if (b0 + R::KB < span.hi) wait_dma<R::PP>();
+    else wait_dma<0>();
+    __builtin_amdgcn_s_barrier();
+    if (b0 + 2 * R::KB < span.hi) ring.template issue<PAD>(b0 + 2 * R::KB, span.hi, buf == 0 ? 2 : buf - 1, wave, lane);
+    const uint32_t ik = lds_addr(smem) + buf * R::BUF;
+#pragma unroll 1
+    for (int t = 0; t < R::KB / 32; ++t) f.any_tile(ws, ik + t * 32 * I::RB, ik + R::IMG + t * 32 * I::RB, b0 + 32 * t);
+    buf = buf == 2 ? 0 : buf + 1;
   }
+  if (f.bad) f.slow(a, kb, vb, ws.any.lo, 32, ws.any.hi);
   if (row >= a.T) return;
-  const float l = pair_sum(st.l);
-  const bool some = own.hi > own.lo && l != 0.f;          // (l is NaN where a score was)
+  const float l = pair_sum(f.st.l);
+  const bool some = f.own.hi > f.own.lo && l != 0.f;          // (l is NaN where a score was)
   const float inv = some ? 1.0f / l : 0.f;
-  // What the backward needs to have the same probabilities again.  fp32: the exponent's offset and 1 / l, applied as here (one log2-sum
-  // would round at the size of its integer part: 1e-6 of a probability); 16-bit: one offset that holds both.
-  if (a.stat != nullptr && hh == 0) {
-    const size_t at = (size_t)head * a.T + row;
-    a.stat[at] = !some ? NEG_INF : DT == MVF_F32 ? st.nm : st.nm - __builtin_amdgcn_logf(l);
-    a.stat[(size_t)a.Hq * a.T + at] = inv;
-  }
+  if (a.stat != nullptr && lane < 32) store_stat<DT>(a, head, row, f.st.nm, l, some);
   typename O::E* dst = reinterpret_cast<typename O::E*>(a.out) + ((size_t)row * a.Hq + head) * a.D;
 #pragma unroll
   for (int dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int d = 32 * dt + 8 * g + 4 * hh;
+    for (int e = 0; e < 4; ++e) {
+      const int d = 32 * dt + 8 * e + 4 * (lane >> 5);
       if (d < a.D) {
-        if (some) O::store4(dst + d, o[dt][4 * g] * inv, o[dt][4 * g + 1] * inv, o[dt][4 * g + 2] * inv, o[dt][4 * g + 3] * inv);
+        if (some) O::store4(dst + d, f.o[dt][4 * e] * inv, f.o[dt][4 * e + 1] * inv, f.o[dt][4 * e + 2] * inv, f.o[dt][4 * e + 3] * inv);
         else O::store4(dst + d, 0.f, 0.f, 0.f, 0.f);
       }
     }
 }
 
-template <int DT, int DP>
+template <int DT, int DP, bool PAD>
+__global__ __launch_bounds__(256, 1) void packed_attn_fwd_split_kernel(FwdArgs a) {
+  typedef Op<DT> O;
+  typedef Tiles<O, DP> S;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  __shared__ float s_m[4][32], s_l[4][32];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int u = xcd_unit(a.ntiles * a.Hq);
+  if (u < 0) return;
+  const int head = u / a.ntiles, tile = a.ntiles - 1 - u % a.ntiles;
+  const int row0 = tile * 32, row = row0 + (lane & 31);
+  Fwd<DT, DP> f;
+  f.own = {0, 0};
+  if (row < a.T) f.own = keys_of(sequence_of(a.cu, a.n_seqs, a.T, row), a.frame, row);
+  const WaveSpan ws = wave_span(f.own);
+  f.start(a, head, row, lane);
+  if constexpr (PAD) clear_lds(smem, 4 * S::NB * S::BUF);
+  const int g = a.Hq / a.Hk;
+#pragma unroll
+  for (int ks = 0; ks < DP / 16; ++ks) asm volatile("" : "+v"(f.qf[ks]));
+  const char *kb = a.k + head / g * a.hsk, *vb = a.v + head / g * a.hsv;
+  const uint32_t lds = lds_addr(smem) + wave * S::NB * S::BUF;
+  auto issue = [&](int key0, int buf) __attribute__((always_inline)) {
+    S::template issue<PAD>(kb, vb, [&](int i, long& oa, long& ob) {
+      const long r = min(key0 + i, ws.any.hi - 1);
+      oa = r * a.ldk;
+      ob = r * a.ldv;
+    }, a.D, lane, lds + buf * S::BUF);
+  };
+  int key0 = ws.any.lo + wave * 32, buf = 0;
+  if (key0 < ws.any.hi) issue(key0, 0);
+  for (; key0 < ws.any.hi; key0 += 128) {
+    const bool more = key0 + 128 < ws.any.hi;
+    if (S::NB == 2 && more) { issue(key0 + 128, buf ^ 1); wait_dma<S::NP>(); }
+    else wait_dma<0>();
+    f.any_tile(ws, lds + buf * S::BUF, lds + buf * S::BUF + S::IMG, key0);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (S::NB == 2) buf ^= 1;
+    else if (more) issue(key0 + 128, 0);
+  }
+  if (f.bad) f.slow(a, kb, vb, ws.any.lo + wave * 32, 128, ws.any.hi);
+  if (f.own.hi == 0) {           // rows of no sequence rode along in unmasked tiles
+    f.st = RowMax();
+#pragma unroll
+    for (int dt = 0; dt < DP / 32; ++dt) f.o[dt] = zero16();
+  }
+  __syncthreads();
+  const bool stat = a.stat != nullptr;
+  join_waves<DP>(reinterpret_cast<float*>(smem), s_m, s_l, f.o, f.st, min(32, a.T - row0), a.D, wave, lane,
+                 [&](int i, int d, const f32x4_t& acc, float mx, float l) {
+    const bool some = l != 0.f;
+    const float inv = some ? 1.0f / l : 0.f;
+    if (stat && d == 0) store_stat<DT>(a, head, row0 + i, -mx, l, some);
+    O::store4(reinterpret_cast<typename O::E*>(a.out) + ((size_t)(row0 + i) * a.Hq + head) * a.D + d, acc[0] * inv, acc[1] * inv,
+              acc[2] * inv, acc[3] * inv);
+  });
+}
+
+// The split form while the wide one's workgroups are fewer than two for each of the 256 compute units.
+template <int DT, int DP, bool PAD>
 int launch(FwdArgs a, hipStream_t st) {
-  const size_t lds = 2 * 64 * Img<Op<DT>, DP>::RB;
-  static uint64_t attr = 0;
-  if (int rc = mvf_ensure_lds(reinterpret_cast<const void*>(packed_attn_fwd_kernel<DT, DP>), lds, attr)) return rc;
-  const int nw = 4;
-  a.ntiles = ceil_div(a.T, 32 * nw);
-  hipLaunchKernelGGL((packed_attn_fwd_kernel<DT, DP>), dim3((unsigned)a.ntiles * a.Hq), dim3(64 * nw), lds, st, a);
+  typedef Ring<Op<DT>, DP> R;
+  typedef Tiles<Op<DT>, DP> S;
+  if ((long)ceil_div(a.T, 128) * a.Hq < 512) {
+    const size_t lds = std::max(4 * S::NB * S::BUF, JOIN_BYTES<DP>);
+    static uint64_t attr = 0;
+    if (int rc = mvf_ensure_lds(reinterpret_cast<const void*>(packed_attn_fwd_split_kernel<DT, DP, PAD>), lds, attr)) return rc;
+    a.ntiles = ceil_div(a.T, 32);
+    hipLaunchKernelGGL((packed_attn_fwd_split_kernel<DT, DP, PAD>), dim3(xcd_grid((long)a.ntiles * a.Hq)), dim3(256), lds, st, a);
+  } else {
+    const size_t lds = R::NB * R::BUF;
+    static uint64_t attr = 0;
+    if (int rc = mvf_ensure_lds(reinterpret_cast<const void*>(packed_attn_fwd_kernel<DT, DP, PAD>), lds, attr)) return rc;
+    a.ntiles = ceil_div(a.T, 128);
+    hipLaunchKernelGGL((packed_attn_fwd_kernel<DT, DP, PAD>), dim3(xcd_grid((long)a.ntiles * a.Hq)), dim3(256), lds, st, a);
+  }
   MVF_LAUNCH_CHECK();
   return MVF_OK;
 }
+template <int DT, int DP>
+int launch_p(const FwdArgs& a, hipStream_t st) { return a.D == DP ? launch<DT, DP, false>(a, st) : launch<DT, DP, true>(a, st); }
 template <int DT>
 int launch_d(const FwdArgs& a, hipStream_t st) {
-  return a.D <= 32 ? launch<DT, 32>(a, st) : a.D <= 64 ? launch<DT, 64>(a, st) : a.D <= 96 ? launch<DT, 96>(a, st) : launch<DT, 128>(a, st);
+  return a.D <= 32 ? launch_p<DT, 32>(a, st) : a.D <= 64 ? launch_p<DT, 64>(a, st) : a.D <= 96 ? launch_p<DT, 96>(a, st) : launch_p<DT, 128>(a, st);
 }
 
 }  // namespace
@@ -167,7 +278,7 @@ extern "C" int mvf_packed_attn_fwd(int dtype, const void* q, long ldq, long hsq,
                                    int D, int frame, float scale, hipStream_t st) {
   MVF_CHECK_ARG(dtype == MVF_F32 || dtype == MVF_BF16 || dtype == MVF_F16);
   MVF_CHECK_ARG(q && k && v && cu_seqlens && out && T > 0 && n_seqs > 0 && Hk > 0 && Hq > 0 && Hq % Hk == 0 && frame >= 0);
-  MVF_CHECK_ARG(scale > 0.f && scale < 1e30f && (long)T * Hq < (1l << 36) && (long)ceil_div(T, 32) * Hq < (1l << 31));
+  MVF_CHECK_ARG(scale > 0.f && scale < 1e30f && T < (1 << 30) && (long)ceil_div(T, 32) * Hq < (1l << 30));
   if (D <= 0 || D > 128 || D % 8 != 0) return MVF_ERR_UNSUPPORTED;
   const long sz = dtype == MVF_F32 ? 4 : 2;
   const long s[6] = {ldq * sz, hsq * sz, ldk * sz, hsk * sz, ldv * sz, hsv * sz};

@@ -3,6 +3,8 @@
 // dK and dV summed over the query heads of a group.  Two kernels, each owning what it writes, so no atomics and the same bits every time:
 //   dQ:     owns 32 queries per wave, streams K and V;       also writes delta, which the second kernel reads
 //   dK/dV:  owns 32 keys per wave, streams Q and dO of every head of the group (the sum over the group stays in registers)
+// Each in the two forms of the forward: wide (four waves of 32 rows share the streamed blocks) and split (one 32-row tile, every wave
+// walks its own quarter of the streamed tiles, the four sums are added at the end in a fixed order).
 #include "mvf_hip_internal.h"
 #include "seq_attn.h"
 
@@ -21,17 +23,6 @@ struct BwdArgs {
   int T, Hq, Hk, D, frame, ntiles;
   float c, scale;
 };
-
-template <class O, int DP, int ROWS>
-__device__ __forceinline__ void stage(char* img, const char* src, long ld, int row0, int end, int D, int tid, int nthreads) {
-  typedef Img<O, DP> I;
-  for (int i = tid; i < ROWS * I::C; i += nthreads) {
-    const int r = i / I::C, ch = i % I::C;
-    uint4 x = make_uint4(0, 0, 0, 0);
-    if (row0 + r < end && ch * 16 < D * O::SZ) x = *reinterpret_cast<const uint4*>(src + (long)(row0 + r) * ld + ch * 16);
-    *reinterpret_cast<uint4*>(img + I::off(r, ch)) = x;
-  }
-}
 
 // a row as the B operand's fragments (zeros where it is not wanted)
 template <class O, int DP>
@@ -60,139 +51,243 @@ __device__ __forceinline__ void store_rows(char* base, size_t row_elems, const f
     }
 }
 
-__device__ __forceinline__ Span block_span(const WaveSpan& ws, int* s_span, int lane, int wave, int nw) {
-  if (lane == 0) { s_span[2 * wave] = ws.any.hi > 0 ? ws.any.lo : 0x7fffffff; s_span[2 * wave + 1] = ws.any.hi; }
+// The four waves' sums of the same 32 rows, added in order: wave 0 + 1 + 2 + 3, out as [row][D].  All threads; barriers inside.
+template <class O, int DP>
+__device__ __forceinline__ void store_joined(float* so, const f32x16_t (&x)[DP / 32], char* base, int row0, int rows, long stride, float f,
+                                             int D, int wave, int lane) {
+  constexpr int ROWF = DP + 4;
+  const int r = lane & 31, hh = lane >> 5;
   __syncthreads();
-  Span s = {0x7fffffff, 0};
-  for (int w = 0; w < nw; ++w) { s.lo = min(s.lo, s_span[2 * w]); s.hi = max(s.hi, s_span[2 * w + 1]); }
-  return s;
+#pragma unroll
+  for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      *reinterpret_cast<f32x4_t*>(so + (wave * 32 + r) * ROWF + 32 * dt + 8 * g + 4 * hh) =
+          (f32x4_t){x[dt][4 * g], x[dt][4 * g + 1], x[dt][4 * g + 2], x[dt][4 * g + 3]};
+  __syncthreads();
+  for (int i = threadIdx.x; i < rows * (DP / 4); i += 256) {
+    const int row = i / (DP / 4), d = i % (DP / 4) * 4;
+    if (d >= D) continue;
+    f32x4_t acc = *reinterpret_cast<const f32x4_t*>(so + row * ROWF + d);
+#pragma unroll
+    for (int w = 1; w < 4; ++w) acc += *reinterpret_cast<const f32x4_t*>(so + (w * 32 + row) * ROWF + d);
+    O::store4(reinterpret_cast<typename O::E*>(base) + (long)(row0 + row) * stride + d, acc[0] * f, acc[1] * f, acc[2] * f, acc[3] * f);
+  }
 }
 
 // ------------------------------------------------------------------------------------------------ dQ
 template <int DT, int DP>
-__global__ __launch_bounds__(256, 1) void packed_attn_dq_kernel(BwdArgs a) {
+struct Dq {
   typedef Op<DT> O;
   typedef Img<O, DP> I;
-  constexpr int KROWS = 64;
-  extern __shared__ __attribute__((aligned(16))) char smem[];
-  __shared__ int s_span[8];
-  char* sk = smem;
-  char* sv = smem + KROWS * I::RB;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nw = blockDim.x >> 6;
-  const int r = lane & 31, hh = lane >> 5;
-  const int head = blockIdx.x % a.Hq, tile = a.ntiles - 1 - (int)(blockIdx.x / a.Hq);
-  const int row = (tile * nw + wave) * 32 + r, rr = min(row, a.T - 1);
-  Span own = {0, 0};
-  if (row < a.T) own = keys_of(sequence_of(a.cu, a.n_seqs, a.T, row), a.frame, row);
-  const WaveSpan ws = wave_span(own);
-  const Span span = block_span(ws, s_span, lane, wave, nw);
-  const bool want = own.hi > 0;
   typename O::Frag qf[DP / 16], dof[DP / 16];
-  load_row<O, DP>(qf, a.q + (long)rr * a.ldq + head * a.hsq, a.D, hh, want);
-  const size_t orow = ((size_t)rr * a.Hq + head) * a.D * O::SZ;
-  load_row<O, DP>(dof, a.d_out + orow, a.D, hh, want);
-  float dl = 0.f;
-  {
-    typename O::Frag of[DP / 16];
-    load_row<O, DP>(of, a.out + orow, a.D, hh, want);
-#pragma unroll
-    for (int ks = 0; ks < DP / 16; ++ks)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) dl = fmaf(O::get(dof[ks], j), O::get(of[ks], j), dl);
-    dl = pair_sum(dl);
-  }
-  const size_t at = (size_t)head * a.T + rr;
-  const float off = want ? a.stat[at] : NEG_INF, inv = DT == MVF_F32 && want ? a.stat[(size_t)a.Hq * a.T + at] : 1.f;
-  if (row < a.T && hh == 0) a.delta[at] = dl;
   f32x16_t dq[DP / 32];
-#pragma unroll
-  for (int dt = 0; dt < DP / 32; ++dt) dq[dt] = zero16();
-  const char* kb = a.k + (head / (a.Hq / a.Hk)) * a.hsk;
-  const char* vb = a.v + (head / (a.Hq / a.Hk)) * a.hsv;
+  Span own;
+  float c, off, inv, dl;
+  int lane;
+  uint32_t rpart, cpart;
+  bool bad = false;        // a tile with masked places held a value that is not finite
 
-  auto tile32 = [&](auto mask_tag, int t, int key0) __attribute__((always_inline)) {
-    constexpr bool MASK = decltype(mask_tag)::value;
-    f32x16_t s = zero16(), dp = zero16();
+  __device__ __forceinline__ void start(const BwdArgs& a, int head, int row, int lane_, bool write_delta) {
+    lane = lane_;
+    rpart = I::row_part(lane);
+    cpart = I::col_part(lane);
+    c = a.c;
+    const int hh = lane >> 5, rr = min(row, a.T - 1);
+    const bool want = own.hi > 0;
+    load_row<O, DP>(qf, a.q + (long)rr * a.ldq + head * a.hsq, a.D, hh, want);
+    const size_t orow = ((size_t)rr * a.Hq + head) * a.D * O::SZ;
+    load_row<O, DP>(dof, a.d_out + orow, a.D, hh, want);
+    dl = 0.f;
 #pragma unroll
     for (int ks = 0; ks < DP / 16; ++ks) {
-      s = O::mma(I::rows(sk, t * 32, ks, lane), qf[ks], s);
-      dp = O::mma(I::rows(sv, t * 32, ks, lane), dof[ks], dp);
+      const int d = 16 * ks + 8 * hh;
+      typename O::Frag x = {};
+      if (want && d < a.D) x = *reinterpret_cast<const typename O::Frag*>(a.out + orow + d * O::SZ);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) dl = fmaf(O::get(dof[ks], j), O::get(x, j), dl);
     }
+    dl = pair_sum(dl);
+    const size_t at = (size_t)head * a.T + rr;
+    off = want ? a.stat[at] : NEG_INF;
+    inv = DT == MVF_F32 && want ? a.stat[(size_t)a.Hq * a.T + at] : 1.f;
+    if (write_delta && row < a.T && hh == 0) a.delta[at] = dl;
+#pragma unroll
+    for (int dt = 0; dt < DP / 32; ++dt) dq[dt] = zero16();
+#pragma unroll
+    for (int ks = 0; ks < DP / 16; ++ks) asm volatile("" : "+v"(qf[ks]), "+v"(dof[ks]));      // landed before any DMA is in flight
+    asm volatile("" : "+v"(off), "+v"(inv), "+v"(dl));
+  }
+  template <bool MASK>
+  __device__ __forceinline__ void tile(uint32_t ik, uint32_t iv, int key0) {
+    const uint32_t rp = launder(rpart), cp = launder(cpart);
+    f32x16_t s = zero16(), dp = zero16();
+#pragma unroll
+    for (int ks = 0; ks < DP / 16; ++ks) s = O::mma(I::rows(ik, rp, ks), qf[ks], s);
+#pragma unroll
+    for (int ks = 0; ks < DP / 16; ++ks) dp = O::mma(I::rows(iv, rp, ks), dof[ks], dp);
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
-      const int key = key0 + 8 * (e >> 2) + 4 * hh + (e & 3);
-      float p = __builtin_amdgcn_exp2f(fmaf(s[e], a.c, off));
+      const int key = key0 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
+      float p = __builtin_amdgcn_exp2f(fmaf(s[e], c, off));
       if constexpr (DT == MVF_F32) p *= inv;
       const float ds = p * (dp[e] - dl);
       s[e] = !MASK || (key >= own.lo && key < own.hi) ? ds : 0.f;
     }
-#pragma unroll
-    for (int s2 = 0; s2 < 2; ++s2) {
-      const typename O::Frag ds = O::pack(s, s2);
-#pragma unroll
-      for (int dt = 0; dt < DP / 32; ++dt) dq[dt] = mma_weighted<O, MASK, true>(I::cols(sk, t * 32 + 16 * s2, dt, lane), ds, dq[dt]);
-    }
-  };
-  for (int b0 = span.lo; b0 < span.hi; b0 += KROWS) {
-    __syncthreads();
-    stage<O, DP, KROWS>(sk, kb, a.ldk, b0, span.hi, a.D, threadIdx.x, blockDim.x);
-    stage<O, DP, KROWS>(sv, vb, a.ldv, b0, span.hi, a.D, threadIdx.x, blockDim.x);
-    __syncthreads();
-    for (int t = 0; t < KROWS / 32; ++t) {
-      const int key0 = b0 + 32 * t;
-      if (key0 >= ws.any.hi || key0 + 32 <= ws.any.lo) continue;
-      if (key0 >= ws.all.lo && key0 + 32 <= ws.all.hi) tile32(std::false_type{}, t, key0);
-      else tile32(std::true_type{}, t, key0);
-    }
+    accumulate<O, DP>(dq, s, ik, cp);
+    if constexpr (MASK) bad |= tile_nonfinite<O, DP>(ik, lane);
   }
-  if (row < a.T) store_rows<O, DP>(a.dq, ((size_t)row * a.Hq + head) * a.D, dq, a.scale, want, a.D, hh);
+  __device__ __forceinline__ void slow(const BwdArgs& a, const char* kb, const char* vb, int first, int step, int end) {
+#pragma unroll
+    for (int dt = 0; dt < DP / 32; ++dt) dq[dt] = zero16();
+#pragma unroll 1
+    for (int k0 = first; k0 < end; k0 += step)
+#pragma unroll 1
+      for (int key = k0; key < min(k0 + 32, end); ++key) {
+        const float s = slow_dot<O, DP>(qf, kb + (long)key * a.ldk, a.D, lane >> 5);
+        const float dp = slow_dot<O, DP>(dof, vb + (long)key * a.ldv, a.D, lane >> 5);
+        if (key < own.lo || key >= own.hi) continue;
+        slow_add<O, DP>(dq, __builtin_amdgcn_exp2f(fmaf(s, c, off)) * inv * (dp - dl), kb + (long)key * a.ldk, a.D, lane >> 5);
+      }
+  }
+  __device__ __forceinline__ void any_tile(const WaveSpan& ws, uint32_t ik, uint32_t iv, int key0) {
+    if (key0 >= ws.any.hi || key0 + 32 <= ws.any.lo) return;
+    if (key0 >= ws.all.lo && key0 + 32 <= ws.all.hi) tile<false>(ik, iv, key0);
+    else tile<true>(ik, iv, key0);
+  }
+};
+
+template <int DT, int DP, bool PAD>
+__global__ __launch_bounds__(256, DT == MVF_F32 && DP > 32 ? 1 : 2) void packed_attn_dq_kernel(BwdArgs a) {
+  typedef Op<DT> O;
+  typedef Img<O, DP> I;
+  typedef Ring<O, DP> R;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  __shared__ int s_span[8];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int u = xcd_unit(a.ntiles * a.Hq);
+  if (u < 0) return;
+  const int head = u / a.ntiles, tile = a.ntiles - 1 - u % a.ntiles;
+  const int row = (tile * 4 + wave) * 32 + (lane & 31);
+  Dq<DT, DP> f;
+  f.own = {0, 0};
+  if (row < a.T) f.own = keys_of(sequence_of(a.cu, a.n_seqs, a.T, row), a.frame, row);
+  const WaveSpan ws = wave_span(f.own);
+  f.start(a, head, row, lane, true);
+  if constexpr (PAD) clear_lds(smem, R::NB * R::BUF);
+  const Span span = block_span(ws, s_span, lane, wave, 4);
+  const int g = a.Hq / a.Hk;
+  const char *kb = a.k + head / g * a.hsk, *vb = a.v + head / g * a.hsv;
+  R ring;
+  ring.start(kb, a.ldk, vb, a.ldv, span.lo, a.D, wave, lane, lds_addr(smem));
+  if (span.lo < span.hi) ring.template issue<PAD>(span.lo, span.hi, 0, wave, lane);
+  if (span.lo + R::KB < span.hi) ring.template issue<PAD>(span.lo + R::KB, span.hi, 1, wave, lane);
+  int buf = 0;
+  for (int b0 = span.lo; b0 < span.hi; b0 += R::KB) {
+    if (b0 + R::KB < span.hi) wait_dma<R::PP>();
+    else wait_dma<0>();
+    __builtin_amdgcn_s_barrier();
+    if (b0 + 2 * R::KB < span.hi) ring.template issue<PAD>(b0 + 2 * R::KB, span.hi, buf == 0 ? 2 : buf - 1, wave, lane);
+    const uint32_t ik = lds_addr(smem) + buf * R::BUF;
+#pragma unroll 1
+    for (int t = 0; t < R::KB / 32; ++t) f.any_tile(ws, ik + t * 32 * I::RB, ik + R::IMG + t * 32 * I::RB, b0 + 32 * t);
+    buf = buf == 2 ? 0 : buf + 1;
+  }
+  if (f.bad) f.slow(a, kb, vb, ws.any.lo, 32, ws.any.hi);
+  if (row < a.T) store_rows<O, DP>(a.dq, ((size_t)row * a.Hq + head) * a.D, f.dq, a.scale, f.own.hi > 0, a.D, lane >> 5);
+}
+
+template <int DT, int DP, bool PAD>
+__global__ __launch_bounds__(256, 1) void packed_attn_dq_split_kernel(BwdArgs a) {
+  typedef Op<DT> O;
+  typedef Tiles<O, DP> S;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int u = xcd_unit(a.ntiles * a.Hq);
+  if (u < 0) return;
+  const int head = u / a.ntiles, tile = a.ntiles - 1 - u % a.ntiles;
+  const int row0 = tile * 32, row = row0 + (lane & 31);
+  Dq<DT, DP> f;
+  f.own = {0, 0};
+  if (row < a.T) f.own = keys_of(sequence_of(a.cu, a.n_seqs, a.T, row), a.frame, row);
+  const WaveSpan ws = wave_span(f.own);
+  f.start(a, head, row, lane, wave == 0);
+  if constexpr (PAD) clear_lds(smem, 4 * S::NB * S::BUF);
+  const int g = a.Hq / a.Hk;
+  const char *kb = a.k + head / g * a.hsk, *vb = a.v + head / g * a.hsv;
+  const uint32_t lds = lds_addr(smem) + wave * S::NB * S::BUF;
+  auto issue = [&](int key0, int buf) __attribute__((always_inline)) {
+    S::template issue<PAD>(kb, vb, [&](int i, long& oa, long& ob) {
+      const long r = min(key0 + i, ws.any.hi - 1);
+      oa = r * a.ldk;
+      ob = r * a.ldv;
+    }, a.D, lane, lds + buf * S::BUF);
+  };
+  int key0 = ws.any.lo + wave * 32, buf = 0;
+  if (key0 < ws.any.hi) issue(key0, 0);
+  for (; key0 < ws.any.hi; key0 += 128) {
+    const bool more = key0 + 128 < ws.any.hi;
+    if (S::NB == 2 && more) { issue(key0 + 128, buf ^ 1); wait_dma<S::NP>(); }
+    else wait_dma<0>();
+    f.any_tile(ws, lds + buf * S::BUF, lds + buf * S::BUF + S::IMG, key0);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (S::NB == 2) buf ^= 1;
+    else if (more) issue(key0 + 128, 0);
+  }
+  if (f.bad) f.slow(a, kb, vb, ws.any.lo + wave * 32, 128, ws.any.hi);
+  if (f.own.hi == 0) {           // rows of no sequence rode along in unmasked tiles
+#pragma unroll
+    for (int dt = 0; dt < DP / 32; ++dt) f.dq[dt] = zero16();
+  }
+  store_joined<O, DP>(reinterpret_cast<float*>(smem), f.dq, a.dq + (size_t)head * a.D * O::SZ, row0, min(32, a.T - row0), (long)a.Hq * a.D,
+                      a.scale, a.D, wave, lane);
 }
 
 // ------------------------------------------------------------------------------------------------ dK, dV
 template <int DT, int DP>
-__global__ __launch_bounds__(256, 1) void packed_attn_dkv_kernel(BwdArgs a) {
+struct Dkv {
   typedef Op<DT> O;
   typedef Img<O, DP> I;
-  constexpr int QROWS = 64;
-  extern __shared__ __attribute__((aligned(16))) char smem[];
-  __shared__ int s_span[8];
-  __shared__ __attribute__((aligned(16))) float s_off[QROWS], s_inv[QROWS], s_dl[QROWS];
-  char* sq = smem;
-  char* sd = smem + QROWS * I::RB;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nw = blockDim.x >> 6;
-  const int r = lane & 31, hh = lane >> 5;
-  const int kh = blockIdx.x % a.Hk, tile = blockIdx.x / a.Hk;
-  const int row = (tile * nw + wave) * 32 + r, rr = min(row, a.T - 1);
-  Span own = {0, 0};
-  if (row < a.T) own = queries_of(sequence_of(a.cu, a.n_seqs, a.T, row), a.frame, row);
-  const WaveSpan ws = wave_span(own);
-  const Span span = block_span(ws, s_span, lane, wave, nw);
-  const bool want = own.hi > 0;
   typename O::Frag kf[DP / 16], vf[DP / 16];
-  load_row<O, DP>(kf, a.k + (long)rr * a.ldk + kh * a.hsk, a.D, hh, want);
-  load_row<O, DP>(vf, a.v + (long)rr * a.ldv + kh * a.hsv, a.D, hh, want);
   f32x16_t dk[DP / 32], dv[DP / 32];
-#pragma unroll
-  for (int dt = 0; dt < DP / 32; ++dt) { dk[dt] = zero16(); dv[dt] = zero16(); }
+  Span own;
+  float c;
+  int lane;
+  uint32_t rpart, cpart;
+  bool bad = false;        // a tile with masked places held a value that is not finite
 
-  auto tile32 = [&](auto mask_tag, int t, int q0) __attribute__((always_inline)) {
-    constexpr bool MASK = decltype(mask_tag)::value;
+  __device__ __forceinline__ void start(const BwdArgs& a, int kh, int row, int lane_) {
+    lane = lane_;
+    rpart = I::row_part(lane);
+    cpart = I::col_part(lane);
+    c = a.c;
+    const int rr = min(row, a.T - 1);
+    load_row<O, DP>(kf, a.k + (long)rr * a.ldk + kh * a.hsk, a.D, lane >> 5, own.hi > 0);
+    load_row<O, DP>(vf, a.v + (long)rr * a.ldv + kh * a.hsv, a.D, lane >> 5, own.hi > 0);
+#pragma unroll
+    for (int dt = 0; dt < DP / 32; ++dt) { dk[dt] = zero16(); dv[dt] = zero16(); }
+#pragma unroll
+    for (int ks = 0; ks < DP / 16; ++ks) asm volatile("" : "+v"(kf[ks]), "+v"(vf[ks]));
+  }
+  // soff: the tile's row statistics in LDS, planes of `plane` bytes: exponent offset, delta, (fp32: 1 / l)
+  template <bool MASK>
+  __device__ __forceinline__ void tile(uint32_t iq, uint32_t id, uint32_t soff, int plane, int q0) {
+    const uint32_t rp = launder(rpart), cp = launder(cpart);
     f32x16_t s = zero16(), dp = zero16();
 #pragma unroll
-    for (int ks = 0; ks < DP / 16; ++ks) {
-      s = O::mma(I::rows(sq, t * 32, ks, lane), kf[ks], s);
-      dp = O::mma(I::rows(sd, t * 32, ks, lane), vf[ks], dp);
-    }
+    for (int ks = 0; ks < DP / 16; ++ks) s = O::mma(I::rows(iq, rp, ks), kf[ks], s);
+#pragma unroll
+    for (int ks = 0; ks < DP / 16; ++ks) dp = O::mma(I::rows(id, rp, ks), vf[ks], dp);
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-      const int i = t * 32 + 8 * g + 4 * hh;
-      const f32x4_t off = *reinterpret_cast<const f32x4_t*>(s_off + i), dl = *reinterpret_cast<const f32x4_t*>(s_dl + i);
+      const uint32_t at = soff + 16 * (lane >> 5) + 32 * g;
+      const f32x4_t off = lds_read<f32x4_t>(at), dl = lds_read<f32x4_t>(at + plane);
       f32x4_t inv = {1.f, 1.f, 1.f, 1.f};
-      if constexpr (DT == MVF_F32) inv = *reinterpret_cast<const f32x4_t*>(s_inv + i);
+      if constexpr (DT == MVF_F32) inv = lds_read<f32x4_t>(at + 2 * plane);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int e = 4 * g + j, q = q0 + 8 * g + 4 * hh + j;
-        float p = __builtin_amdgcn_exp2f(fmaf(s[e], a.c, off[j]));
+        const int e = 4 * g + j, q = q0 + 8 * g + 4 * (lane >> 5) + j;
+        float p = __builtin_amdgcn_exp2f(fmaf(s[e], c, off[j]));
         if constexpr (DT == MVF_F32) p *= inv[j];
         const float ds = p * (dp[e] - dl[j]);
         const bool sees = !MASK || (q >= own.lo && q < own.hi);
@@ -200,63 +295,192 @@ __global__ __launch_bounds__(256, 1) void packed_attn_dkv_kernel(BwdArgs a) {
         dp[e] = sees ? ds : 0.f;
       }
     }
+    accumulate<O, DP>(dv, s, id, cp);
+    accumulate<O, DP>(dk, dp, iq, cp);
+    if constexpr (MASK) bad |= tile_nonfinite<O, DP>(id, lane) | tile_nonfinite<O, DP>(iq, lane);
+  }
+  // over tiles it = first, first + step, ... of (head of the group, 32-query tile)
+  __device__ __forceinline__ void slow(const BwdArgs& a, int kh, Span any, int first, int step) {
 #pragma unroll
-    for (int s2 = 0; s2 < 2; ++s2) {
-      const typename O::Frag p = O::pack(s, s2), ds = O::pack(dp, s2);
-#pragma unroll
-      for (int dt = 0; dt < DP / 32; ++dt) {
-        dv[dt] = mma_weighted<O, MASK, false>(I::cols(sd, t * 32 + 16 * s2, dt, lane), p, dv[dt]);
-        dk[dt] = mma_weighted<O, MASK, true>(I::cols(sq, t * 32 + 16 * s2, dt, lane), ds, dk[dt]);
-      }
-    }
-  };
-  const int g = a.Hq / a.Hk;
-  for (int h = kh * g; h < (kh + 1) * g; ++h) {
-    const char* qb = a.q + h * a.hsq;
-    const char* db = a.d_out + (size_t)h * a.D * O::SZ;
-    for (int b0 = span.lo; b0 < span.hi; b0 += QROWS) {
-      __syncthreads();
-      stage<O, DP, QROWS>(sq, qb, a.ldq, b0, span.hi, a.D, threadIdx.x, blockDim.x);
-      stage<O, DP, QROWS>(sd, db, (long)a.Hq * a.D * O::SZ, b0, span.hi, a.D, threadIdx.x, blockDim.x);
-      if (threadIdx.x < QROWS) {
-        const int i = b0 + threadIdx.x;
-        const size_t at = (size_t)h * a.T + min(i, a.T - 1);
-        s_off[threadIdx.x] = i < span.hi ? a.stat[at] : NEG_INF;
-        s_inv[threadIdx.x] = i < span.hi ? a.stat[(size_t)a.Hq * a.T + at] : 0.f;
-        s_dl[threadIdx.x] = i < span.hi ? a.delta[at] : 0.f;
-      }
-      __syncthreads();
-      for (int t = 0; t < QROWS / 32; ++t) {
-        const int q0 = b0 + 32 * t;
-        if (q0 >= ws.any.hi || q0 + 32 <= ws.any.lo) continue;
-        if (q0 >= ws.all.lo && q0 + 32 <= ws.all.hi) tile32(std::false_type{}, t, q0);
-        else tile32(std::true_type{}, t, q0);
+    for (int dt = 0; dt < DP / 32; ++dt) { dk[dt] = zero16(); dv[dt] = zero16(); }
+    const int g = a.Hq / a.Hk, nt = (any.hi - any.lo + 31) >> 5;
+#pragma unroll 1
+    for (int it = first; it < nt * g; it += step) {
+      const int h = kh * g + it / nt, q0 = any.lo + it % nt * 32;
+#pragma unroll 1
+      for (int q = q0; q < min(q0 + 32, any.hi); ++q) {
+        const char *qr = a.q + (long)q * a.ldq + h * a.hsq, *dr = a.d_out + ((size_t)q * a.Hq + h) * a.D * O::SZ;
+        const float s = slow_dot<O, DP>(kf, qr, a.D, lane >> 5), dp = slow_dot<O, DP>(vf, dr, a.D, lane >> 5);
+        if (q < own.lo || q >= own.hi) continue;
+        const size_t at = (size_t)h * a.T + q;
+        const float p = __builtin_amdgcn_exp2f(fmaf(s, c, a.stat[at])) * (DT == MVF_F32 ? a.stat[(size_t)a.Hq * a.T + at] : 1.f);
+        slow_add<O, DP>(dv, p, dr, a.D, lane >> 5);
+        slow_add<O, DP>(dk, p * (dp - a.delta[at]), qr, a.D, lane >> 5);
       }
     }
   }
+  __device__ __forceinline__ void any_tile(const WaveSpan& ws, uint32_t iq, uint32_t id, uint32_t soff, int plane, int q0) {
+    if (q0 >= ws.any.hi || q0 + 32 <= ws.any.lo) return;
+    if (q0 >= ws.all.lo && q0 + 32 <= ws.all.hi) tile<false>(iq, id, soff, plane, q0);
+    else tile<true>(iq, id, soff, plane, q0);
+  }
+};
+
+constexpr int planes(int dt) { return dt == MVF_F32 ? 3 : 2; }
+// float f of the statistics of rows row .. row + n of head h: plane f / n (offset, delta, 1 / l), row f % n
+__device__ __forceinline__ const float* stat_at(const BwdArgs& a, int h, int row, int f, int n) {
+  const int plane = f / n;
+  const float* base = plane == 1 ? a.delta : plane == 0 ? a.stat : a.stat + (size_t)a.Hq * a.T;
+  return base + (size_t)h * a.T + min(row + f % n, a.T - 1);
+}
+
+template <int DT, int DP, bool PAD>
+__global__ __launch_bounds__(256, DP > (DT == MVF_F32 ? 32 : 64) ? 1 : 2) void packed_attn_dkv_kernel(BwdArgs a) {
+  typedef Op<DT> O;
+  typedef Img<O, DP> I;
+  typedef Ring<O, DP> R;
+  constexpr int NF = planes(DT) * R::KB, SB = (NF + 63) / 64 * 256;     // floats of a block's statistics, bytes of their buffer
+  static_assert(NF <= 256, "one piece per wave");
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  __shared__ int s_span[8];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int u = xcd_unit(a.ntiles * a.Hk);
+  if (u < 0) return;
+  const int kh = u / a.ntiles, tile = u % a.ntiles;                       // causal: the first keys have the longest walks
+  const int row = (tile * 4 + wave) * 32 + (lane & 31);
+  Dkv<DT, DP> f;
+  f.own = {0, 0};
+  if (row < a.T) f.own = queries_of(sequence_of(a.cu, a.n_seqs, a.T, row), a.frame, row);
+  const WaveSpan ws = wave_span(f.own);
+  f.start(a, kh, row, lane);
+  if constexpr (PAD) clear_lds(smem, R::NB * R::BUF);
+  const Span span = block_span(ws, s_span, lane, wave, 4);
+  const int g = a.Hq / a.Hk, nblk = span.hi > span.lo ? (span.hi - span.lo + R::KB - 1) / R::KB : 0, total = nblk * g;
+  const uint32_t lds0 = lds_addr(smem), stat0 = lds0 + R::NB * R::BUF;
+  const int sp = min(wave, SB / 256 - 1);                                 // (a wave without a piece of its own repeats the last one)
+  R ring;
+  int ih = kh * g, ib = 0;                                                // head and block that are asked for next
+  auto issue = [&](int buf) __attribute__((always_inline)) {
+    if (ib == 0)
+      ring.start(a.q + ih * a.hsq, a.ldq, a.d_out + (size_t)ih * a.D * O::SZ, (long)a.Hq * a.D * O::SZ, span.lo, a.D, wave, lane, lds0);
+    const int b0 = span.lo + ib * R::KB;
+    ring.template issue<PAD>(b0, span.hi, buf, wave, lane);
+    dma4(stat_at(a, ih, b0, min(sp * 64 + lane, NF - 1), R::KB), stat0 + buf * SB + sp * 256);
+    if (++ib == nblk) { ib = 0; ++ih; }
+  };
+  if (total > 0) issue(0);
+  if (total > 1) issue(1);
+  int buf = 0, b0 = span.lo;
+  for (int it = 0; it < total; ++it) {
+    if (it + 1 < total) wait_dma<R::PP + 1>();
+    else wait_dma<0>();
+    __builtin_amdgcn_s_barrier();
+    if (it + 2 < total) issue(buf == 0 ? 2 : buf - 1);
+    const uint32_t iq = lds0 + buf * R::BUF, so = stat0 + buf * SB;
+#pragma unroll 1
+    for (int t = 0; t < R::KB / 32; ++t)
+      f.any_tile(ws, iq + t * 32 * I::RB, iq + R::IMG + t * 32 * I::RB, so + t * 128, R::KB * 4, b0 + 32 * t);
+    buf = buf == 2 ? 0 : buf + 1;
+    b0 += R::KB;
+    if (b0 >= span.hi) b0 = span.lo;
+  }
+  if (f.bad) f.slow(a, kh, ws.any, 0, 1);
   if (row < a.T) {
-    store_rows<O, DP>(a.dk, ((size_t)row * a.Hk + kh) * a.D, dk, a.scale, want, a.D, hh);
-    store_rows<O, DP>(a.dv, ((size_t)row * a.Hk + kh) * a.D, dv, 1.f, want, a.D, hh);
+    store_rows<O, DP>(a.dk, ((size_t)row * a.Hk + kh) * a.D, f.dk, a.scale, f.own.hi > 0, a.D, lane >> 5);
+    store_rows<O, DP>(a.dv, ((size_t)row * a.Hk + kh) * a.D, f.dv, 1.f, f.own.hi > 0, a.D, lane >> 5);
   }
 }
 
-template <int DT, int DP>
+template <int DT, int DP, bool PAD>
+__global__ __launch_bounds__(256, 1) void packed_attn_dkv_split_kernel(BwdArgs a) {
+  typedef Op<DT> O;
+  typedef Tiles<O, DP> S;
+  constexpr int NF = planes(DT) * 32, NSP = (NF + 63) / 64, SB = NSP * 256;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int u = xcd_unit(a.ntiles * a.Hk);
+  if (u < 0) return;
+  const int kh = u / a.ntiles, tile = u % a.ntiles;
+  const int row0 = tile * 32, row = row0 + (lane & 31);
+  Dkv<DT, DP> f;
+  f.own = {0, 0};
+  if (row < a.T) f.own = queries_of(sequence_of(a.cu, a.n_seqs, a.T, row), a.frame, row);
+  const WaveSpan ws = wave_span(f.own);
+  f.start(a, kh, row, lane);
+  if constexpr (PAD) clear_lds(smem, 4 * S::NB * S::BUF);
+  const int g = a.Hq / a.Hk, nt = (ws.any.hi - ws.any.lo + 31) >> 5, total = nt * g;
+  const uint32_t lds = lds_addr(smem) + wave * S::NB * S::BUF, stat0 = lds_addr(smem) + 4 * S::NB * S::BUF + wave * S::NB * SB;
+  auto issue = [&](int it, int buf) __attribute__((always_inline)) {
+    const int h = kh * g + it / nt, q0 = ws.any.lo + it % nt * 32;
+    const long ldo = (long)a.Hq * a.D * O::SZ;
+    S::template issue<PAD>(a.q + h * a.hsq, a.d_out + (size_t)h * a.D * O::SZ, [&](int i, long& oa, long& ob) {
+      const long r = min(q0 + i, ws.any.hi - 1);
+      oa = r * a.ldq;
+      ob = r * ldo;
+    }, a.D, lane, lds + buf * S::BUF);
+#pragma unroll
+    for (int j = 0; j < NSP; ++j) dma4(stat_at(a, h, q0, min(j * 64 + lane, NF - 1), 32), stat0 + buf * SB + j * 256);
+  };
+  int buf = 0;
+  if (wave < total) issue(wave, 0);
+  for (int it = wave; it < total; it += 4) {
+    const bool more = it + 4 < total;
+    if (S::NB == 2 && more) { issue(it + 4, buf ^ 1); wait_dma<S::NP + NSP>(); }
+    else wait_dma<0>();
+    f.any_tile(ws, lds + buf * S::BUF, lds + buf * S::BUF + S::IMG, stat0 + buf * SB, 128, ws.any.lo + it % nt * 32);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (S::NB == 2) buf ^= 1;
+    else if (more) issue(it + 4, 0);
+  }
+  if (f.bad) f.slow(a, kh, ws.any, wave, 4);
+  if (f.own.hi == 0) {
+#pragma unroll
+    for (int dt = 0; dt < DP / 32; ++dt) { f.dk[dt] = zero16(); f.dv[dt] = zero16(); }
+  }
+  const int rows = min(32, a.T - row0);
+  float* so = reinterpret_cast<float*>(smem);
+  store_joined<O, DP>(so, f.dk, a.dk + (size_t)kh * a.D * O::SZ, row0, rows, (long)a.Hk * a.D, a.scale, a.D, wave, lane);
+  store_joined<O, DP>(so, f.dv, a.dv + (size_t)kh * a.D * O::SZ, row0, rows, (long)a.Hk * a.D, 1.f, a.D, wave, lane);
+}
+
+// The split forms while the wide ones' workgroups are fewer than two for each of the 256 compute units.
+template <int DT, int DP, bool PAD>
 int launch(BwdArgs a, hipStream_t st) {
-  const size_t lds = 2 * 64 * Img<Op<DT>, DP>::RB;
-  static uint64_t attr1 = 0, attr2 = 0;
-  if (int rc = mvf_ensure_lds(reinterpret_cast<const void*>(packed_attn_dq_kernel<DT, DP>), lds, attr1)) return rc;
-  if (int rc = mvf_ensure_lds(reinterpret_cast<const void*>(packed_attn_dkv_kernel<DT, DP>), lds, attr2)) return rc;
-  const int nw = 4;
-  a.ntiles = ceil_div(a.T, 32 * nw);
-  hipLaunchKernelGGL((packed_attn_dq_kernel<DT, DP>), dim3((unsigned)a.ntiles * a.Hq), dim3(64 * nw), lds, st, a);
+  typedef Ring<Op<DT>, DP> R;
+  typedef Tiles<Op<DT>, DP> S;
+  static uint64_t attr[4] = {0, 0, 0, 0};
+  const int wide = ceil_div(a.T, 128), narrow = ceil_div(a.T, 32);
+  if ((long)wide * a.Hq < 512) {
+    const size_t lds = std::max(4 * S::NB * S::BUF, JOIN_BYTES<DP>);
+    if (int rc = mvf_ensure_lds(reinterpret_cast<const void*>(packed_attn_dq_split_kernel<DT, DP, PAD>), lds, attr[0])) return rc;
+    a.ntiles = narrow;
+    hipLaunchKernelGGL((packed_attn_dq_split_kernel<DT, DP, PAD>), dim3(xcd_grid((long)narrow * a.Hq)), dim3(256), lds, st, a);
+  } else {
+    const size_t lds = R::NB * R::BUF;
+    if (int rc = mvf_ensure_lds(reinterpret_cast<const void*>(packed_attn_dq_kernel<DT, DP, PAD>), lds, attr[1])) return rc;
+    a.ntiles = wide;
+    hipLaunchKernelGGL((packed_attn_dq_kernel<DT, DP, PAD>), dim3(xcd_grid((long)wide * a.Hq)), dim3(256), lds, st, a);
+  }
   MVF_LAUNCH_CHECK();
-  hipLaunchKernelGGL((packed_attn_dkv_kernel<DT, DP>), dim3((unsigned)a.ntiles * a.Hk), dim3(64 * nw), lds, st, a);
+  if ((long)wide * a.Hk < 512) {
+    const size_t lds = std::max(4 * S::NB * (S::BUF + (planes(DT) * 32 + 63) / 64 * 256), JOIN_BYTES<DP>);
+    if (int rc = mvf_ensure_lds(reinterpret_cast<const void*>(packed_attn_dkv_split_kernel<DT, DP, PAD>), lds, attr[2])) return rc;
+    a.ntiles = narrow;
+    hipLaunchKernelGGL((packed_attn_dkv_split_kernel<DT, DP, PAD>), dim3(xcd_grid((long)narrow * a.Hk)), dim3(256), lds, st, a);
+  } else {
+    const size_t lds = R::NB * (R::BUF + (planes(DT) * R::KB + 63) / 64 * 256);
+    if (int rc = mvf_ensure_lds(reinterpret_cast<const void*>(packed_attn_dkv_kernel<DT, DP, PAD>), lds, attr[3])) return rc;
+    a.ntiles = wide;
+    hipLaunchKernelGGL((packed_attn_dkv_kernel<DT, DP, PAD>), dim3(xcd_grid((long)wide * a.Hk)), dim3(256), lds, st, a);
+  }
   MVF_LAUNCH_CHECK();
   return MVF_OK;
 }
+template <int DT, int DP>
+int launch_p(const BwdArgs& a, hipStream_t st) { return a.D == DP ? launch<DT, DP, false>(a, st) : launch<DT, DP, true>(a, st); }
 template <int DT>
 int launch_d(const BwdArgs& a, hipStream_t st) {
-  return a.D <= 32 ? launch<DT, 32>(a, st) : a.D <= 64 ? launch<DT, 64>(a, st) : a.D <= 96 ? launch<DT, 96>(a, st) : launch<DT, 128>(a, st);
+  return a.D <= 32 ? launch_p<DT, 32>(a, st) : a.D <= 64 ? launch_p<DT, 64>(a, st) : a.D <= 96 ? launch_p<DT, 96>(a, st) : launch_p<DT, 128>(a, st);
 }
 
 }  // namespace
@@ -268,7 +492,7 @@ extern "C" int mvf_packed_attn_bwd(int dtype, const void* q, long ldq, long hsq,
   MVF_CHECK_ARG(dtype == MVF_F32 || dtype == MVF_BF16 || dtype == MVF_F16);
   MVF_CHECK_ARG(q && k && v && cu_seqlens && out && d_out && stat && delta && dq && dk && dv);
   MVF_CHECK_ARG(T > 0 && n_seqs > 0 && Hk > 0 && Hq > 0 && Hq % Hk == 0 && frame >= 0);
-  MVF_CHECK_ARG(scale > 0.f && scale < 1e30f && (long)T * Hq < (1l << 36) && (long)ceil_div(T, 32) * Hq < (1l << 31));
+  MVF_CHECK_ARG(scale > 0.f && scale < 1e30f && T < (1 << 30) && (long)ceil_div(T, 32) * Hq < (1l << 30));
   if (D <= 0 || D > 128 || D % 8 != 0) return MVF_ERR_UNSUPPORTED;
   const long sz = dtype == MVF_F32 ? 4 : 2;
   const long s[6] = {ldq * sz, hsq * sz, ldk * sz, hsk * sz, ldv * sz, hsv * sz};
