@@ -2211,13 +2211,17 @@ def _index_operand(t, like, shape, what):
         raise ValueError('%s must be int32 (or int64), got %s' % (what, t.dtype))
     if t.dim() != len(shape) or any(n >= 0 and n != m for n, m in zip(shape, t.shape)):
         raise ValueError('%s: expected shape %s, got %s' % (what, shape, tuple(t.shape)))
-    return t.to(torch.int32).contiguous()
+    return t if t.dtype is torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
 
 
 def _aligned(t):
     """The tensor itself if its channels are contiguous and every other stride and the start are multiples of 16 bytes, else a copy."""
-    a = 16 // t.element_size()
-    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s > 0 and s % a == 0 for s in t.stride()[:-1]):
+    *outer, inner = t.stride()
+    a = 3 if t.element_size() == 4 else 7
+    bad = inner != 1 or t.data_ptr() & 15
+    for s in outer:
+        bad = bad or s <= 0 or s & a
+    if not bad:
         return t
     t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
@@ -2244,9 +2248,14 @@ def _scale_arg(scale, d):
     return scale
 
 
-def _here(t):
-    """Launches go to the operands' device, whichever is current."""
-    return torch.cuda.device(t.device)
+def _launch(name, like, *args):
+    """call() on the current stream of the operands' device, whichever device is current."""
+    dev = like.get_device()
+    if dev == torch.cuda.current_device():
+        call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        with torch.cuda.device(dev):
+            call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
 
 
 def rotary_freqs(sections, base=10000.0, device='cuda'):
@@ -2264,7 +2273,7 @@ def _rotary_args(pos, freqs, sections, tokens, size, like):
         raise ValueError('pos: expected [%d, %d] of int32, int64 or float32, got %s %s' % (tokens, len(sections), tuple(pos.shape), pos.dtype))
     if freqs.dtype != torch.float64 or tuple(freqs.shape) != (sum(sections),):
         raise ValueError('freqs: expected [%d] float64, got %s %s' % (sum(sections), tuple(freqs.shape), freqs.dtype))
-    return pos.contiguous(), freqs.contiguous(), sections + (0,) * (3 - len(sections))
+    return pos.contiguous(), freqs.contiguous(), sections + (0, 0, 0)[len(sections):]
 
 
 def _rotary_call(q, k, pos, freqs, sections, interleaved, inverse):
@@ -2275,10 +2284,9 @@ def _rotary_call(q, k, pos, freqs, sections, interleaved, inverse):
     ko = torch.empty(T, k.shape[1], D, device=q.device, dtype=q.dtype) if k is not None else None
     if T == 0:
         return qo, ko
-    with _here(q):
-        call('mvf_rotary', _SEQ_DT[q.dtype], q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr() if k is not None else None,
-             k.stride(0) if k is not None else 0, k.stride(1) if k is not None else 0, pos.data_ptr(), _POS_DT[pos.dtype], freqs.data_ptr(),
-             *sections, int(interleaved), int(inverse), qo.data_ptr(), ptr(ko), T, Hq, k.shape[1] if k is not None else 0, D, stream())
+    kp, ldk, hsk, kop, Hk = (k.data_ptr(), *k.stride()[:2], ko.data_ptr(), k.shape[1]) if k is not None else (None, 0, 0, None, 0)
+    _launch('mvf_rotary', q, _SEQ_DT[q.dtype], q.data_ptr(), *q.stride()[:2], kp, ldk, hsk, pos.data_ptr(), _POS_DT[pos.dtype],
+            freqs.data_ptr(), *sections, interleaved, inverse, qo.data_ptr(), kop, T, Hq, Hk, D)
     return qo, ko
 
 
@@ -2349,11 +2357,10 @@ def rotary_append(q, k, v, pos, freqs, sections, k_cache, v_cache, block_table, 
         return qo
     if 0 in table.shape:
         raise ValueError('block_table is empty: %s' % (tuple(table.shape),))
-    with _here(q):
-        call('mvf_rotary_append', code, q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
-             v.stride(0), v.stride(1), pos.data_ptr(), _POS_DT[pos.dtype], freqs.data_ptr(), *sections, int(interleaved), qo.data_ptr(),
-             k_cache.data_ptr(), v_cache.data_ptr(), table.data_ptr(), table.shape[1], table.shape[0], seq.data_ptr(), index.data_ptr(),
-             k_cache.shape[0], k_cache.shape[1], T, Hq, k.shape[1], D, stream())
+    _launch('mvf_rotary_append', q, code, q.data_ptr(), *q.stride()[:2], k.data_ptr(), *k.stride()[:2], v.data_ptr(), *v.stride()[:2],
+            pos.data_ptr(), _POS_DT[pos.dtype], freqs.data_ptr(), *sections, bool(interleaved), qo.data_ptr(), k_cache.data_ptr(),
+            v_cache.data_ptr(), table.data_ptr(), table.shape[1], table.shape[0], seq.data_ptr(), index.data_ptr(), k_cache.shape[0],
+            k_cache.shape[1], T, Hq, k.shape[1], D)
     return qo
 
 
@@ -2362,10 +2369,9 @@ def _packed_fwd(q, k, v, cu, frame, scale, need_stat):
     out = torch.empty(T, Hq, D, device=q.device, dtype=q.dtype)
     stat = torch.empty(2, Hq, T, device=q.device, dtype=torch.float32) if need_stat else None
     if T:
-        with _here(q):
-            call('mvf_packed_attn_fwd', _SEQ_DT[q.dtype], q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
-                 v.data_ptr(), v.stride(0), v.stride(1), cu.data_ptr(), cu.shape[0] - 1, out.data_ptr(), ptr(stat), T, Hq, k.shape[1], D,
-                 frame, scale, stream())
+        _launch('mvf_packed_attn_fwd', q, _SEQ_DT[q.dtype], q.data_ptr(), *q.stride()[:2], k.data_ptr(), *k.stride()[:2], v.data_ptr(),
+                *v.stride()[:2], cu.data_ptr(), cu.shape[0] - 1, out.data_ptr(), stat.data_ptr() if need_stat else None, T, Hq, k.shape[1], D,
+                frame, scale)
     return out, stat
 
 
@@ -2388,12 +2394,10 @@ class _PackedAttention(torch.autograd.Function):
             d_out = d_out.clone()
         dq, dk, dv = (torch.empty(x.shape, device=x.device, dtype=x.dtype) for x in (q, k, v))
         if T:
-            with _here(q):
-                delta = torch.empty(Hq, T, device=q.device, dtype=torch.float32)
-                call('mvf_packed_attn_bwd', _SEQ_DT[q.dtype], q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
-                     v.data_ptr(), v.stride(0), v.stride(1), cu.data_ptr(), cu.shape[0] - 1, out.data_ptr(), d_out.data_ptr(),
-                     stat.data_ptr(), delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), T, Hq, k.shape[1], D, frame, scale,
-                     stream())
+            delta = torch.empty(Hq, T, device=q.device, dtype=torch.float32)
+            _launch('mvf_packed_attn_bwd', q, _SEQ_DT[q.dtype], q.data_ptr(), *q.stride()[:2], k.data_ptr(), *k.stride()[:2], v.data_ptr(),
+                    *v.stride()[:2], cu.data_ptr(), cu.shape[0] - 1, out.data_ptr(), d_out.data_ptr(), stat.data_ptr(), delta.data_ptr(),
+                    dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), T, Hq, k.shape[1], D, frame, scale)
         return dq, dk, dv, None, None, None
 
 
@@ -2441,9 +2445,8 @@ def paged_attention(q, k_cache, v_cache, block_table, lengths, frame=1, scale=No
     if width == 0:
         raise ValueError('block_table has no columns')
     q = _aligned(q)
-    with _here(q):
-        need = _lib.load().mvf_paged_attn_workspace_bytes(B, n, Hq, Hk, D, width, page)
-        ws = torch.empty(need, device=q.device, dtype=torch.uint8) if need else None
-        call('mvf_paged_attn', code, q.data_ptr(), q.stride(0), q.stride(1), q.stride(2), k_cache.data_ptr(), v_cache.data_ptr(),
-             table.data_ptr(), lens.data_ptr(), out.data_ptr(), ptr(ws), need, B, n, Hq, Hk, D, n_pages, page, width, frame, scale, stream())
+    need = _lib.load().mvf_paged_attn_workspace_bytes(B, n, Hq, Hk, D, width, page)
+    ws = torch.empty(need, device=q.device, dtype=torch.uint8) if need else None
+    _launch('mvf_paged_attn', q, code, q.data_ptr(), *q.stride()[:3], k_cache.data_ptr(), v_cache.data_ptr(), table.data_ptr(),
+            lens.data_ptr(), out.data_ptr(), ws.data_ptr() if need else None, need, B, n, Hq, Hk, D, n_pages, page, width, frame, scale)
     return out
