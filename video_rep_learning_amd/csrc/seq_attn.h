@@ -322,10 +322,50 @@ __device__ __forceinline__ int xcd_unit(int units) {
   const int per = (units + 7) >> 3, slot = blockIdx.x >> 3, u = (blockIdx.x & 7) * per + slot;
   return slot < per && u < units ? u : -1;
 }
+#ifndef MVF_SPLIT_RULE
+#define MVF_SPLIT_RULE(x) ((x) < 512)
+#endif
 static inline unsigned xcd_grid(long units) { return (unsigned)((units + 7) / 8 * 8); }
 
 // ---------------------------------------------------------------------------------------------- which rows meet
 struct Span { int lo, hi; };
+// Which rows a workgroup owns.  Up to SEQ_TILES sequences every sequence is cut into tiles of its own (a tile across two sequences would walk
+// both: twice the longest path), and so are the rows before the first and behind the last one; beyond that, the packed rows are, and
+// every row looks its sequence up.
+constexpr int SEQ_TILES = 510;
+struct OwnTile { int row0, end; Span seq; };      // rows [row0, end); seq: their sequence ({0, 0}: none)
+template <int ROWS>
+static inline long tile_bound(long T, long n) {   // no fewer than the tiles there are
+  return n > SEQ_TILES ? (T + ROWS - 1) / ROWS : (T + (ROWS - 1) * (n + 2 < T ? n + 2 : T)) / ROWS;
+}
+// the t-th tile, found by every wave for itself: lane i sizes segment i, one prefix sum per 64 of them
+template <int ROWS>
+__device__ __forceinline__ OwnTile find_tile(const int* __restrict__ cu, int n, int T, int t) {
+  if (n > SEQ_TILES) return {t * ROWS, min(T, t * ROWS + ROWS), {0, 0}};
+  const int lane = threadIdx.x & 63;
+  int before = 0;
+  for (int s0 = 0; s0 < n + 2; s0 += 64) {
+    const int i = s0 + lane;                        // segment 0: rows before cu[0]; i: sequence i - 1; n + 1: rows behind cu[n]
+    const int lo = i == 0 ? 0 : min(max(cu[min(i - 1, n)], 0), T), hi = i > n ? T : min(max(cu[i], 0), T);
+    const int tiles = i < n + 2 && hi > lo ? (hi - lo + ROWS - 1) / ROWS : 0;
+    int sum = tiles;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int up = __shfl_up(sum, o, 64);
+      if (lane >= o) sum += up;
+    }
+    const uint64_t in = __builtin_amdgcn_ballot_w64(t >= before + sum - tiles && t < before + sum);
+    if (in != 0) {
+      const int j = __builtin_ctzll(in);
+      const int l = __builtin_amdgcn_readlane(lo, j), h = __builtin_amdgcn_readlane(hi, j);
+      const int first = before + __builtin_amdgcn_readlane(sum - tiles, j), r0 = l + (t - first) * ROWS;
+      const int seg = s0 + j;
+      return {r0, min(h, r0 + ROWS), seg == 0 || seg == n + 1 ? Span{0, 0} : Span{l, h}};
+    }
+    before += __builtin_amdgcn_readlane(sum, 63);
+  }
+  return {0, 0, {0, 0}};
+}
 // largest b < n with cu[b] <= row < cu[b + 1], as [start, end) cut to [0, T); {0, 0} for a row of no sequence
 __device__ __forceinline__ Span sequence_of(const int* __restrict__ cu, int n, int T, int row) {
   int lo = 0, hi = n;                      // the first index with cu > row lies in [lo, hi]
@@ -334,9 +374,12 @@ __device__ __forceinline__ Span sequence_of(const int* __restrict__ cu, int n, i
     if (cu[mid] <= row) lo = mid + 1;
     else hi = mid;
   }
-  if (lo == 0) return {0, 0};
-  const int s = max(cu[lo - 1], 0), e = min(cu[lo], T);
-  return row < e ? Span{s, e} : Span{0, 0};
+  const int s = max(cu[max(lo - 1, 0)], 0), e = min(cu[lo], T);
+  return lo > 0 && row < e ? Span{s, e} : Span{0, 0};
+}
+__device__ __forceinline__ Span sequence_of(const OwnTile& t, const int* __restrict__ cu, int n, int T, int row) {
+  if (row >= t.end) return {0, 0};
+  return n > SEQ_TILES ? sequence_of(cu, n, T, row) : t.seq;
 }
 // keys that query `row` sees: its sequence's, up to the end of its own group of `frame` tokens (frame = 0: all)
 __device__ __forceinline__ Span keys_of(Span s, int frame, int row) {

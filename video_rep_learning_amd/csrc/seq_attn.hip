@@ -50,7 +50,7 @@ struct Fwd {
     for (int ks = 0; ks < DP / 16; ++ks) {
       const int d = 16 * ks + 8 * hh;
       typename O::Frag f = {};
-      if (d < a.D && own.hi > 0) f = *reinterpret_cast<const typename O::Frag*>(src + d * O::SZ);
+      if (d < a.D) f = *reinterpret_cast<const typename O::Frag*>(src + d * O::SZ);
       qf[ks] = f;
     }
 #pragma unroll
@@ -139,12 +139,13 @@ __global__ __launch_bounds__(256, DT == MVF_F32 && DP > 64 ? 1 : 2) void packed_
   const int u = xcd_unit(a.ntiles * a.Hq);
   if (u < 0) return;
   const int head = u / a.ntiles, tile = a.ntiles - 1 - u % a.ntiles;       // the longest walks (causal: the last rows) first
-  const int row = (tile * 4 + wave) * 32 + (lane & 31);
+  const OwnTile own = find_tile<128>(a.cu, a.n_seqs, a.T, tile);
+  if (own.row0 >= own.end) return;
+  const int row = own.row0 + wave * 32 + (lane & 31);
   Fwd<DT, DP> f;
-  f.own = {0, 0};
-  if (row < a.T) f.own = keys_of(sequence_of(a.cu, a.n_seqs, a.T, row), a.frame, row);
+  f.start(a, head, row, lane);                 // (a row of no sequence may hold anything: it stays in its own lanes and is not stored)
+  f.own = keys_of(sequence_of(own, a.cu, a.n_seqs, a.T, row), a.frame, row);
   const WaveSpan ws = wave_span(f.own);
-  f.start(a, head, row, lane);
   if constexpr (PAD) clear_lds(smem, R::NB * R::BUF);
   const Span span = block_span(ws, s_span, lane, wave, 4);
   const int g = a.Hq / a.Hk;
@@ -167,7 +168,7 @@ __global__ __launch_bounds__(256, DT == MVF_F32 && DP > 64 ? 1 : 2) void packed_
     buf = buf == 2 ? 0 : buf + 1;
   }
   if (f.bad) f.slow(a, kb, vb, ws.any.lo, 32, ws.any.hi);
-  if (row >= a.T) return;
+  if (row >= own.end) return;
   const float l = pair_sum(f.st.l);
   const bool some = f.own.hi > f.own.lo && l != 0.f;          // (l is NaN where a score was)
   const float inv = some ? 1.0f / l : 0.f;
@@ -195,12 +196,13 @@ __global__ __launch_bounds__(256, 1) void packed_attn_fwd_split_kernel(FwdArgs a
   const int u = xcd_unit(a.ntiles * a.Hq);
   if (u < 0) return;
   const int head = u / a.ntiles, tile = a.ntiles - 1 - u % a.ntiles;
-  const int row0 = tile * 32, row = row0 + (lane & 31);
+  const OwnTile own = find_tile<32>(a.cu, a.n_seqs, a.T, tile);
+  if (own.row0 >= own.end) return;
+  const int row0 = own.row0, row = row0 + (lane & 31);
   Fwd<DT, DP> f;
-  f.own = {0, 0};
-  if (row < a.T) f.own = keys_of(sequence_of(a.cu, a.n_seqs, a.T, row), a.frame, row);
+  f.start(a, head, row, lane);                 // (a row of no sequence may hold anything: it stays in its own lanes and is not stored)
+  f.own = keys_of(sequence_of(own, a.cu, a.n_seqs, a.T, row), a.frame, row);
   const WaveSpan ws = wave_span(f.own);
-  f.start(a, head, row, lane);
   if constexpr (PAD) clear_lds(smem, 4 * S::NB * S::BUF);
   const int g = a.Hq / a.Hk;
 #pragma unroll
@@ -233,7 +235,7 @@ __global__ __launch_bounds__(256, 1) void packed_attn_fwd_split_kernel(FwdArgs a
   }
   __syncthreads();
   const bool stat = a.stat != nullptr;
-  join_waves<DP>(reinterpret_cast<float*>(smem), s_m, s_l, f.o, f.st, min(32, a.T - row0), a.D, wave, lane,
+  join_waves<DP>(reinterpret_cast<float*>(smem), s_m, s_l, f.o, f.st, own.end - row0, a.D, wave, lane,
                  [&](int i, int d, const f32x4_t& acc, float mx, float l) {
     const bool some = l != 0.f;
     const float inv = some ? 1.0f / l : 0.f;
@@ -248,17 +250,17 @@ template <int DT, int DP, bool PAD>
 int launch(FwdArgs a, hipStream_t st) {
   typedef Ring<Op<DT>, DP> R;
   typedef Tiles<Op<DT>, DP> S;
-  if ((long)ceil_div(a.T, 128) * a.Hq < 512) {
+  if (MVF_SPLIT_RULE(tile_bound<128>(a.T, a.n_seqs) * a.Hq)) {
     const size_t lds = std::max(4 * S::NB * S::BUF, JOIN_BYTES<DP>);
     static uint64_t attr = 0;
     if (int rc = mvf_ensure_lds(reinterpret_cast<const void*>(packed_attn_fwd_split_kernel<DT, DP, PAD>), lds, attr)) return rc;
-    a.ntiles = ceil_div(a.T, 32);
+    a.ntiles = (int)tile_bound<32>(a.T, a.n_seqs);
     hipLaunchKernelGGL((packed_attn_fwd_split_kernel<DT, DP, PAD>), dim3(xcd_grid((long)a.ntiles * a.Hq)), dim3(256), lds, st, a);
   } else {
     const size_t lds = R::NB * R::BUF;
     static uint64_t attr = 0;
     if (int rc = mvf_ensure_lds(reinterpret_cast<const void*>(packed_attn_fwd_kernel<DT, DP, PAD>), lds, attr)) return rc;
-    a.ntiles = ceil_div(a.T, 128);
+    a.ntiles = (int)tile_bound<128>(a.T, a.n_seqs);
     hipLaunchKernelGGL((packed_attn_fwd_kernel<DT, DP, PAD>), dim3(xcd_grid((long)a.ntiles * a.Hq)), dim3(256), lds, st, a);
   }
   MVF_LAUNCH_CHECK();
@@ -278,7 +280,7 @@ extern "C" int mvf_packed_attn_fwd(int dtype, const void* q, long ldq, long hsq,
                                    int D, int frame, float scale, hipStream_t st) {
   MVF_CHECK_ARG(dtype == MVF_F32 || dtype == MVF_BF16 || dtype == MVF_F16);
   MVF_CHECK_ARG(q && k && v && cu_seqlens && out && T > 0 && n_seqs > 0 && Hk > 0 && Hq > 0 && Hq % Hk == 0 && frame >= 0);
-  MVF_CHECK_ARG(scale > 0.f && scale < 1e30f && T < (1 << 30) && (long)ceil_div(T, 32) * Hq < (1l << 30));
+  MVF_CHECK_ARG(scale > 0.f && scale < 1e30f && T < (1 << 30) && tile_bound<32>(T, n_seqs) * Hq < (1l << 30));
   if (D <= 0 || D > 128 || D % 8 != 0) return MVF_ERR_UNSUPPORTED;
   const long sz = dtype == MVF_F32 ? 4 : 2;
   const long s[6] = {ldq * sz, hsq * sz, ldk * sz, hsk * sz, ldv * sz, hsv * sz};

@@ -24,14 +24,14 @@ struct BwdArgs {
   float c, scale;
 };
 
-// a row as the B operand's fragments (zeros where it is not wanted)
+// a row as the B operand's fragments.  (A row of no sequence may hold anything: it stays in its own lanes and is not stored.)
 template <class O, int DP>
-__device__ __forceinline__ void load_row(typename O::Frag (&f)[DP / 16], const char* src, int D, int hh, bool want) {
+__device__ __forceinline__ void load_row(typename O::Frag (&f)[DP / 16], const char* src, int D, int hh) {
 #pragma unroll
   for (int ks = 0; ks < DP / 16; ++ks) {
     const int d = 16 * ks + 8 * hh;
     typename O::Frag x = {};
-    if (want && d < D) x = *reinterpret_cast<const typename O::Frag*>(src + d * O::SZ);
+    if (d < D) x = *reinterpret_cast<const typename O::Frag*>(src + d * O::SZ);
     f[ks] = x;
   }
 }
@@ -94,24 +94,23 @@ struct Dq {
     cpart = I::col_part(lane);
     c = a.c;
     const int hh = lane >> 5, rr = min(row, a.T - 1);
-    const bool want = own.hi > 0;
-    load_row<O, DP>(qf, a.q + (long)rr * a.ldq + head * a.hsq, a.D, hh, want);
+    load_row<O, DP>(qf, a.q + (long)rr * a.ldq + head * a.hsq, a.D, hh);
     const size_t orow = ((size_t)rr * a.Hq + head) * a.D * O::SZ;
-    load_row<O, DP>(dof, a.d_out + orow, a.D, hh, want);
+    load_row<O, DP>(dof, a.d_out + orow, a.D, hh);
     dl = 0.f;
 #pragma unroll
     for (int ks = 0; ks < DP / 16; ++ks) {
       const int d = 16 * ks + 8 * hh;
       typename O::Frag x = {};
-      if (want && d < a.D) x = *reinterpret_cast<const typename O::Frag*>(a.out + orow + d * O::SZ);
+      if (d < a.D) x = *reinterpret_cast<const typename O::Frag*>(a.out + orow + d * O::SZ);
 #pragma unroll
       for (int j = 0; j < 8; ++j) dl = fmaf(O::get(dof[ks], j), O::get(x, j), dl);
     }
     dl = pair_sum(dl);
     const size_t at = (size_t)head * a.T + rr;
-    off = want ? a.stat[at] : NEG_INF;
-    inv = DT == MVF_F32 && want ? a.stat[(size_t)a.Hq * a.T + at] : 1.f;
-    if (write_delta && row < a.T && hh == 0) a.delta[at] = dl;
+    off = a.stat[at];
+    inv = DT == MVF_F32 ? a.stat[(size_t)a.Hq * a.T + at] : 1.f;
+    if (write_delta && hh == 0) a.delta[at] = dl;
 #pragma unroll
     for (int dt = 0; dt < DP / 32; ++dt) dq[dt] = zero16();
 #pragma unroll
@@ -168,12 +167,13 @@ __global__ __launch_bounds__(256, DT == MVF_F32 && DP > 32 ? 1 : 2) void packed_
   const int u = xcd_unit(a.ntiles * a.Hq);
   if (u < 0) return;
   const int head = u / a.ntiles, tile = a.ntiles - 1 - u % a.ntiles;
-  const int row = (tile * 4 + wave) * 32 + (lane & 31);
+  const OwnTile own = find_tile<128>(a.cu, a.n_seqs, a.T, tile);
+  if (own.row0 >= own.end) return;
+  const int row = own.row0 + wave * 32 + (lane & 31);
   Dq<DT, DP> f;
-  f.own = {0, 0};
-  if (row < a.T) f.own = keys_of(sequence_of(a.cu, a.n_seqs, a.T, row), a.frame, row);
+  f.start(a, head, row, lane, row < own.end);
+  f.own = keys_of(sequence_of(own, a.cu, a.n_seqs, a.T, row), a.frame, row);
   const WaveSpan ws = wave_span(f.own);
-  f.start(a, head, row, lane, true);
   if constexpr (PAD) clear_lds(smem, R::NB * R::BUF);
   const Span span = block_span(ws, s_span, lane, wave, 4);
   const int g = a.Hq / a.Hk;
@@ -194,7 +194,7 @@ __global__ __launch_bounds__(256, DT == MVF_F32 && DP > 32 ? 1 : 2) void packed_
     buf = buf == 2 ? 0 : buf + 1;
   }
   if (f.bad) f.slow(a, kb, vb, ws.any.lo, 32, ws.any.hi);
-  if (row < a.T) store_rows<O, DP>(a.dq, ((size_t)row * a.Hq + head) * a.D, f.dq, a.scale, f.own.hi > 0, a.D, lane >> 5);
+  if (row < own.end) store_rows<O, DP>(a.dq, ((size_t)row * a.Hq + head) * a.D, f.dq, a.scale, f.own.hi > 0, a.D, lane >> 5);
 }
 
 template <int DT, int DP, bool PAD>
@@ -206,12 +206,13 @@ __global__ __launch_bounds__(256, 1) void packed_attn_dq_split_kernel(BwdArgs a)
   const int u = xcd_unit(a.ntiles * a.Hq);
   if (u < 0) return;
   const int head = u / a.ntiles, tile = a.ntiles - 1 - u % a.ntiles;
-  const int row0 = tile * 32, row = row0 + (lane & 31);
+  const OwnTile own = find_tile<32>(a.cu, a.n_seqs, a.T, tile);
+  if (own.row0 >= own.end) return;
+  const int row0 = own.row0, row = row0 + (lane & 31);
   Dq<DT, DP> f;
-  f.own = {0, 0};
-  if (row < a.T) f.own = keys_of(sequence_of(a.cu, a.n_seqs, a.T, row), a.frame, row);
+  f.start(a, head, row, lane, wave == 0 && row < own.end);
+  f.own = keys_of(sequence_of(own, a.cu, a.n_seqs, a.T, row), a.frame, row);
   const WaveSpan ws = wave_span(f.own);
-  f.start(a, head, row, lane, wave == 0);
   if constexpr (PAD) clear_lds(smem, 4 * S::NB * S::BUF);
   const int g = a.Hq / a.Hk;
   const char *kb = a.k + head / g * a.hsk, *vb = a.v + head / g * a.hsv;
@@ -239,7 +240,7 @@ __global__ __launch_bounds__(256, 1) void packed_attn_dq_split_kernel(BwdArgs a)
 #pragma unroll
     for (int dt = 0; dt < DP / 32; ++dt) f.dq[dt] = zero16();
   }
-  store_joined<O, DP>(reinterpret_cast<float*>(smem), f.dq, a.dq + (size_t)head * a.D * O::SZ, row0, min(32, a.T - row0), (long)a.Hq * a.D,
+  store_joined<O, DP>(reinterpret_cast<float*>(smem), f.dq, a.dq + (size_t)head * a.D * O::SZ, row0, own.end - row0, (long)a.Hq * a.D,
                       a.scale, a.D, wave, lane);
 }
 
@@ -262,8 +263,8 @@ struct Dkv {
     cpart = I::col_part(lane);
     c = a.c;
     const int rr = min(row, a.T - 1);
-    load_row<O, DP>(kf, a.k + (long)rr * a.ldk + kh * a.hsk, a.D, lane >> 5, own.hi > 0);
-    load_row<O, DP>(vf, a.v + (long)rr * a.ldv + kh * a.hsv, a.D, lane >> 5, own.hi > 0);
+    load_row<O, DP>(kf, a.k + (long)rr * a.ldk + kh * a.hsk, a.D, lane >> 5);
+    load_row<O, DP>(vf, a.v + (long)rr * a.ldv + kh * a.hsv, a.D, lane >> 5);
 #pragma unroll
     for (int dt = 0; dt < DP / 32; ++dt) { dk[dt] = zero16(); dv[dt] = zero16(); }
 #pragma unroll
@@ -347,12 +348,13 @@ __global__ __launch_bounds__(256, DP > (DT == MVF_F32 ? 32 : 64) ? 1 : 2) void p
   const int u = xcd_unit(a.ntiles * a.Hk);
   if (u < 0) return;
   const int kh = u / a.ntiles, tile = u % a.ntiles;                       // causal: the first keys have the longest walks
-  const int row = (tile * 4 + wave) * 32 + (lane & 31);
+  const OwnTile own = find_tile<128>(a.cu, a.n_seqs, a.T, tile);
+  if (own.row0 >= own.end) return;
+  const int row = own.row0 + wave * 32 + (lane & 31);
   Dkv<DT, DP> f;
-  f.own = {0, 0};
-  if (row < a.T) f.own = queries_of(sequence_of(a.cu, a.n_seqs, a.T, row), a.frame, row);
-  const WaveSpan ws = wave_span(f.own);
   f.start(a, kh, row, lane);
+  f.own = queries_of(sequence_of(own, a.cu, a.n_seqs, a.T, row), a.frame, row);
+  const WaveSpan ws = wave_span(f.own);
   if constexpr (PAD) clear_lds(smem, R::NB * R::BUF);
   const Span span = block_span(ws, s_span, lane, wave, 4);
   const int g = a.Hq / a.Hk, nblk = span.hi > span.lo ? (span.hi - span.lo + R::KB - 1) / R::KB : 0, total = nblk * g;
@@ -385,7 +387,7 @@ __global__ __launch_bounds__(256, DP > (DT == MVF_F32 ? 32 : 64) ? 1 : 2) void p
     if (b0 >= span.hi) b0 = span.lo;
   }
   if (f.bad) f.slow(a, kh, ws.any, 0, 1);
-  if (row < a.T) {
+  if (row < own.end) {
     store_rows<O, DP>(a.dk, ((size_t)row * a.Hk + kh) * a.D, f.dk, a.scale, f.own.hi > 0, a.D, lane >> 5);
     store_rows<O, DP>(a.dv, ((size_t)row * a.Hk + kh) * a.D, f.dv, 1.f, f.own.hi > 0, a.D, lane >> 5);
   }
@@ -401,12 +403,13 @@ __global__ __launch_bounds__(256, 1) void packed_attn_dkv_split_kernel(BwdArgs a
   const int u = xcd_unit(a.ntiles * a.Hk);
   if (u < 0) return;
   const int kh = u / a.ntiles, tile = u % a.ntiles;
-  const int row0 = tile * 32, row = row0 + (lane & 31);
+  const OwnTile own = find_tile<32>(a.cu, a.n_seqs, a.T, tile);
+  if (own.row0 >= own.end) return;
+  const int row0 = own.row0, row = row0 + (lane & 31);
   Dkv<DT, DP> f;
-  f.own = {0, 0};
-  if (row < a.T) f.own = queries_of(sequence_of(a.cu, a.n_seqs, a.T, row), a.frame, row);
-  const WaveSpan ws = wave_span(f.own);
   f.start(a, kh, row, lane);
+  f.own = queries_of(sequence_of(own, a.cu, a.n_seqs, a.T, row), a.frame, row);
+  const WaveSpan ws = wave_span(f.own);
   if constexpr (PAD) clear_lds(smem, 4 * S::NB * S::BUF);
   const int g = a.Hq / a.Hk, nt = (ws.any.hi - ws.any.lo + 31) >> 5, total = nt * g;
   const uint32_t lds = lds_addr(smem) + wave * S::NB * S::BUF, stat0 = lds_addr(smem) + 4 * S::NB * S::BUF + wave * S::NB * SB;
@@ -437,7 +440,7 @@ __global__ __launch_bounds__(256, 1) void packed_attn_dkv_split_kernel(BwdArgs a
 #pragma unroll
     for (int dt = 0; dt < DP / 32; ++dt) { f.dk[dt] = zero16(); f.dv[dt] = zero16(); }
   }
-  const int rows = min(32, a.T - row0);
+  const int rows = own.end - row0;
   float* so = reinterpret_cast<float*>(smem);
   store_joined<O, DP>(so, f.dk, a.dk + (size_t)kh * a.D * O::SZ, row0, rows, (long)a.Hk * a.D, a.scale, a.D, wave, lane);
   store_joined<O, DP>(so, f.dv, a.dv + (size_t)kh * a.D * O::SZ, row0, rows, (long)a.Hk * a.D, 1.f, a.D, wave, lane);
@@ -449,8 +452,8 @@ int launch(BwdArgs a, hipStream_t st) {
   typedef Ring<Op<DT>, DP> R;
   typedef Tiles<Op<DT>, DP> S;
   static uint64_t attr[4] = {0, 0, 0, 0};
-  const int wide = ceil_div(a.T, 128), narrow = ceil_div(a.T, 32);
-  if ((long)wide * a.Hq < 512) {
+  const int wide = (int)tile_bound<128>(a.T, a.n_seqs), narrow = (int)tile_bound<32>(a.T, a.n_seqs);
+  if (MVF_SPLIT_RULE((long)wide * a.Hq)) {
     const size_t lds = std::max(4 * S::NB * S::BUF, JOIN_BYTES<DP>);
     if (int rc = mvf_ensure_lds(reinterpret_cast<const void*>(packed_attn_dq_split_kernel<DT, DP, PAD>), lds, attr[0])) return rc;
     a.ntiles = narrow;
@@ -462,7 +465,7 @@ int launch(BwdArgs a, hipStream_t st) {
     hipLaunchKernelGGL((packed_attn_dq_kernel<DT, DP, PAD>), dim3(xcd_grid((long)wide * a.Hq)), dim3(256), lds, st, a);
   }
   MVF_LAUNCH_CHECK();
-  if ((long)wide * a.Hk < 512) {
+  if (MVF_SPLIT_RULE((long)wide * a.Hk)) {
     const size_t lds = std::max(4 * S::NB * (S::BUF + (planes(DT) * 32 + 63) / 64 * 256), JOIN_BYTES<DP>);
     if (int rc = mvf_ensure_lds(reinterpret_cast<const void*>(packed_attn_dkv_split_kernel<DT, DP, PAD>), lds, attr[2])) return rc;
     a.ntiles = narrow;
@@ -492,7 +495,7 @@ extern "C" int mvf_packed_attn_bwd(int dtype, const void* q, long ldq, long hsq,
   MVF_CHECK_ARG(dtype == MVF_F32 || dtype == MVF_BF16 || dtype == MVF_F16);
   MVF_CHECK_ARG(q && k && v && cu_seqlens && out && d_out && stat && delta && dq && dk && dv);
   MVF_CHECK_ARG(T > 0 && n_seqs > 0 && Hk > 0 && Hq > 0 && Hq % Hk == 0 && frame >= 0);
-  MVF_CHECK_ARG(scale > 0.f && scale < 1e30f && T < (1 << 30) && (long)ceil_div(T, 32) * Hq < (1l << 30));
+  MVF_CHECK_ARG(scale > 0.f && scale < 1e30f && T < (1 << 30) && tile_bound<32>(T, n_seqs) * Hq < (1l << 30));
   if (D <= 0 || D > 128 || D % 8 != 0) return MVF_ERR_UNSUPPORTED;
   const long sz = dtype == MVF_F32 ? 4 : 2;
   const long s[6] = {ldq * sz, hsq * sz, ldk * sz, hsk * sz, ldv * sz, hsv * sz};
