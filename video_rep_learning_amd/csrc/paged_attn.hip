@@ -29,7 +29,7 @@ __global__ __launch_bounds__(64 * NW, 1) void paged_attn_kernel(PagedArgs a) {
   typedef Op<DT> O;
   typedef Img<O, DP> I;
   typedef Tiles<O, DP> S;
-  extern __shared__ __attribute__((aligned(16))) char smem[];
+  extern __shared__ __attribute__((aligned(256))) char smem[];
   __shared__ float s_m[NW][32], s_l[NW][32];
   __shared__ int s_tab[NW][2][64];                    // page ids of a tile's 32 keys (twice)
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -95,13 +95,13 @@ __global__ __launch_bounds__(64 * NW, 1) void paged_attn_kernel(PagedArgs a) {
     }, a.D, lane, lds + buf * S::BUF);
   };
   bool bad = false;
-  auto tile = [&](auto mask_tag, int t, uint32_t there, uint32_t ik) __attribute__((always_inline)) {
-    constexpr bool MASK = decltype(mask_tag)::value;
-    const uint32_t rp = launder(rpart), cp = launder(cpart);
+  auto tile = [&](int t, uint32_t there, uint32_t ik, bool mask) __attribute__((always_inline)) {
+    const uint32_t rl = launder(rpart + ik), cl = launder(cpart + ik + S::IMG);
     f32x16_t s = zero16();
 #pragma unroll
-    for (int ks = 0; ks < DP / 16; ++ks) s = O::mma(I::rows(ik, rp, ks), qf[ks], s);
-    if constexpr (MASK) {
+    for (int ks = 0; ks < DP / 16; ++ks) s = O::mma(I::rows(rl, ks), qf[ks], s);
+    if (mask) {
+      bad |= tile_nonfinite<O, DP>(ik + S::IMG, lane);
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         const int i = 8 * (e >> 2) + 4 * hh + (e & 3);
@@ -124,8 +124,7 @@ __global__ __launch_bounds__(64 * NW, 1) void paged_attn_kernel(PagedArgs a) {
       s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.c, st.nm));
       st.l += s[e];
     }
-    accumulate<O, DP>(o, s, ik + S::IMG, cp);
-    if constexpr (MASK) bad |= tile_nonfinite<O, DP>(ik + S::IMG, lane);
+    accumulate<O, DP>(o, s, cl);
   };
 
   // Per tile: its page ids are asked for two tiles ahead, its rows one tile ahead (where the buffers allow two tiles).
@@ -153,8 +152,7 @@ __global__ __launch_bounds__(64 * NW, 1) void paged_attn_kernel(PagedArgs a) {
     } else {
       wait_dma<0>();
     }
-    if (there == 0xffffffffu && t * 32 + 32 <= hi_all) tile(std::false_type{}, t, there, ik);
-    else if (there != 0) tile(std::true_type{}, t, there, ik);
+    if (there != 0) tile(t, there, ik, there != 0xffffffffu || t * 32 + 32 > hi_all);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     if (S::NB == 2) {
       buf ^= 1;

@@ -144,17 +144,17 @@ struct Img {
     else return ((i & 3) << 2) | ((i >> 2) & 3);
   }
   static __device__ __forceinline__ int off(int i, int c) { return i * RB + ((c ^ swz(i)) << 4); }
-  // chunk c of a row whose lane part is `lane_part`: the low bits meet swz, the others are added
-  static __device__ __forceinline__ uint32_t at(uint32_t lane_part, int c, int x, uint32_t base) {
-    return (lane_part ^ (uint32_t)(((c & M) ^ x) << 4)) + base + (uint32_t)((c & ~M) << 4);
+  // chunk c of a row at `lane` (image base, a multiple of 256, + lane part): the low bits meet swz, the others are added
+  static __device__ __forceinline__ uint32_t at(uint32_t lane, int c, int x) {
+    return (lane ^ (uint32_t)(((c & M) ^ x) << 4)) + (uint32_t)((c & ~M) << 4);
   }
   // A operand = 32 rows of the image from `img` on: lane (r, h) <- X[r][16 ks + 8h .. + 8]
   static __device__ __forceinline__ uint32_t row_part(int lane) { return off(lane & 31, (lane >> 5) * (O::SZ / 2)); }
-  static __device__ __forceinline__ typename O::Frag rows(uint32_t img, uint32_t part, int ks) {
+  static __device__ __forceinline__ typename O::Frag rows(uint32_t lane, int ks) {
     if constexpr (O::SZ == 2) {
-      return lds_read<bf16x8_t>(at(part, 2 * ks, 0, img));
+      return lds_read<bf16x8_t>(at(lane, 2 * ks, 0));
     } else {
-      const f32x4_t a = lds_read<f32x4_t>(at(part, 4 * ks, 0, img)), b = lds_read<f32x4_t>(at(part, 4 * ks + 1, 0, img));
+      const f32x4_t a = lds_read<f32x4_t>(at(lane, 4 * ks, 0)), b = lds_read<f32x4_t>(at(lane, 4 * ks + 1, 0));
       return (f32x8_t){a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
     }
   }
@@ -164,20 +164,20 @@ struct Img {
     if constexpr (O::SZ == 2) return off(4 * h + (li >> 2), 2 * ((lane >> 4) & 1) + ((li & 3) >> 1)) + 8 * (li & 1);
     else return off(4 * h, (lane & 31) >> 2) + 4 * (lane & 3);
   }
-  static __device__ __forceinline__ typename O::Frag cols(uint32_t img, uint32_t part, int s, int dt) {
+  static __device__ __forceinline__ typename O::Frag cols(uint32_t lane, int s, int dt) {
     if constexpr (O::SZ == 2) {
       union { bf16x8_t v; bf16x4_t q[2]; } f;
 #pragma unroll
       for (int j = 0; j < 2; ++j)
         f.q[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) bf16x4_t*)lds_at(
-            at(part, 4 * dt, 2 * j, img) + (16 * s + 8 * j) * RB));
+            at(lane, 4 * dt, 2 * j) + (16 * s + 8 * j) * RB));
       return f.v;
     } else {
       f32x8_t f;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {     // row 16 s + 8 (j >> 2) + 4 h + (j & 3)
         const int x = (M == 7 ? ((j >> 1) & 1) << 2 : (j & 3) << 2) ^ (2 * (j >> 2));
-        f[j] = lds_read<float>(at(part, 8 * dt, x, img) + (16 * s + 8 * (j >> 2) + (j & 3)) * RB);
+        f[j] = lds_read<float>(at(lane, 8 * dt, x) + (16 * s + 8 * (j >> 2) + (j & 3)) * RB);
       }
       return f;
     }
@@ -189,12 +189,12 @@ struct Img {
 // tiles with masked places the kernels look for non-finite values, and a wave that met one goes over its rows again, element by
 // element and visible pairs only (their slow()), after the loop.
 template <class O, int DP>
-__device__ __forceinline__ void accumulate(f32x16_t (&acc)[DP / 32], const f32x16_t& w, uint32_t img, uint32_t part) {
+__device__ __forceinline__ void accumulate(f32x16_t (&acc)[DP / 32], const f32x16_t& w, uint32_t lane) {
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
     const typename O::Frag b = O::pack(w, s);
 #pragma unroll
-    for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = O::mma(Img<O, DP>::cols(img, part, s, dt), b, acc[dt]);
+    for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = O::mma(Img<O, DP>::cols(lane, s, dt), b, acc[dt]);
   }
 }
 template <class O, int DP>

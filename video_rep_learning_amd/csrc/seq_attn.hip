@@ -56,13 +56,14 @@ struct Fwd {
 #pragma unroll
     for (int dt = 0; dt < DP / 32; ++dt) o[dt] = zero16();
   }
-  template <bool MASK>
-  __device__ __forceinline__ void tile(uint32_t ik, uint32_t iv, int key0) {
+  // one 32-key tile; mask (wave-uniform): some row does not see all of it
+  __device__ __forceinline__ void tile(uint32_t ik, uint32_t iv, int key0, bool mask) {
+    const uint32_t rl = launder(rpart + ik), cl = launder(cpart + iv);
     f32x16_t s = zero16();
-    const uint32_t rp = launder(rpart), cp = launder(cpart);
 #pragma unroll
-    for (int ks = 0; ks < DP / 16; ++ks) s = O::mma(I::rows(ik, rp, ks), qf[ks], s);
-    if constexpr (MASK) {
+    for (int ks = 0; ks < DP / 16; ++ks) s = O::mma(I::rows(rl, ks), qf[ks], s);
+    if (mask) {
+      bad |= tile_nonfinite<O, DP>(iv, lane);
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         const int key = key0 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
@@ -85,8 +86,7 @@ struct Fwd {
       s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], c, st.nm));
       st.l += s[e];
     }
-    accumulate<O, DP>(o, s, iv, cp);
-    if constexpr (MASK) bad |= tile_nonfinite<O, DP>(iv, lane);
+    accumulate<O, DP>(o, s, cl);
   }
   // the same rows over 32-key tiles first, first + step, ..., one visible pair at a time
   __device__ __forceinline__ void slow(const FwdArgs& a, const char* kb, const char* vb, int first, int step, int end) {
@@ -114,8 +114,7 @@ struct Fwd {
   }
   __device__ __forceinline__ void any_tile(const WaveSpan& ws, uint32_t ik, uint32_t iv, int key0) {
     if (key0 >= ws.any.hi || key0 + 32 <= ws.any.lo) return;
-    if (key0 >= ws.all.lo && key0 + 32 <= ws.all.hi) tile<false>(ik, iv, key0);
-    else tile<true>(ik, iv, key0);
+    tile(ik, iv, key0, key0 < ws.all.lo || key0 + 32 > ws.all.hi);
   }
 };
 
@@ -133,7 +132,7 @@ __global__ __launch_bounds__(256, DT == MVF_F32 && DP > 64 ? 1 : 2) void packed_
   typedef Op<DT> O;
   typedef Img<O, DP> I;
   typedef Ring<O, DP> R;
-  extern __shared__ __attribute__((aligned(16))) char smem[];
+  extern __shared__ __attribute__((aligned(256))) char smem[];
   __shared__ int s_span[8];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int u = xcd_unit(a.ntiles * a.Hq);
@@ -190,7 +189,7 @@ template <int DT, int DP, bool PAD>
 __global__ __launch_bounds__(256, 1) void packed_attn_fwd_split_kernel(FwdArgs a) {
   typedef Op<DT> O;
   typedef Tiles<O, DP> S;
-  extern __shared__ __attribute__((aligned(16))) char smem[];
+  extern __shared__ __attribute__((aligned(256))) char smem[];
   __shared__ float s_m[4][32], s_l[4][32];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int u = xcd_unit(a.ntiles * a.Hq);

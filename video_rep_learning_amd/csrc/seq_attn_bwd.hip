@@ -117,24 +117,28 @@ struct Dq {
     for (int ks = 0; ks < DP / 16; ++ks) asm volatile("" : "+v"(qf[ks]), "+v"(dof[ks]));      // landed before any DMA is in flight
     asm volatile("" : "+v"(off), "+v"(inv), "+v"(dl));
   }
-  template <bool MASK>
-  __device__ __forceinline__ void tile(uint32_t ik, uint32_t iv, int key0) {
-    const uint32_t rp = launder(rpart), cp = launder(cpart);
+  __device__ __forceinline__ void tile(uint32_t ik, uint32_t iv, int key0, bool mask) {
+    const uint32_t rk = launder(rpart + ik), rv = launder(rpart + iv), ck = launder(cpart + ik);
     f32x16_t s = zero16(), dp = zero16();
 #pragma unroll
-    for (int ks = 0; ks < DP / 16; ++ks) s = O::mma(I::rows(ik, rp, ks), qf[ks], s);
+    for (int ks = 0; ks < DP / 16; ++ks) s = O::mma(I::rows(rk, ks), qf[ks], s);
 #pragma unroll
-    for (int ks = 0; ks < DP / 16; ++ks) dp = O::mma(I::rows(iv, rp, ks), dof[ks], dp);
+    for (int ks = 0; ks < DP / 16; ++ks) dp = O::mma(I::rows(rv, ks), dof[ks], dp);
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
-      const int key = key0 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
       float p = __builtin_amdgcn_exp2f(fmaf(s[e], c, off));
       if constexpr (DT == MVF_F32) p *= inv;
-      const float ds = p * (dp[e] - dl);
-      s[e] = !MASK || (key >= own.lo && key < own.hi) ? ds : 0.f;
+      s[e] = p * (dp[e] - dl);
     }
-    accumulate<O, DP>(dq, s, ik, cp);
-    if constexpr (MASK) bad |= tile_nonfinite<O, DP>(ik, lane);
+    if (mask) {
+      bad |= tile_nonfinite<O, DP>(ik, lane);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int key = key0 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
+        s[e] = key >= own.lo && key < own.hi ? s[e] : 0.f;
+      }
+    }
+    accumulate<O, DP>(dq, s, ck);
   }
   __device__ __forceinline__ void slow(const BwdArgs& a, const char* kb, const char* vb, int first, int step, int end) {
 #pragma unroll
@@ -151,8 +155,7 @@ struct Dq {
   }
   __device__ __forceinline__ void any_tile(const WaveSpan& ws, uint32_t ik, uint32_t iv, int key0) {
     if (key0 >= ws.any.hi || key0 + 32 <= ws.any.lo) return;
-    if (key0 >= ws.all.lo && key0 + 32 <= ws.all.hi) tile<false>(ik, iv, key0);
-    else tile<true>(ik, iv, key0);
+    tile(ik, iv, key0, key0 < ws.all.lo || key0 + 32 > ws.all.hi);
   }
 };
 
@@ -161,7 +164,7 @@ __global__ __launch_bounds__(256, DT == MVF_F32 && DP > 32 ? 1 : 2) void packed_
   typedef Op<DT> O;
   typedef Img<O, DP> I;
   typedef Ring<O, DP> R;
-  extern __shared__ __attribute__((aligned(16))) char smem[];
+  extern __shared__ __attribute__((aligned(256))) char smem[];
   __shared__ int s_span[8];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int u = xcd_unit(a.ntiles * a.Hq);
@@ -201,7 +204,7 @@ template <int DT, int DP, bool PAD>
 __global__ __launch_bounds__(256, 1) void packed_attn_dq_split_kernel(BwdArgs a) {
   typedef Op<DT> O;
   typedef Tiles<O, DP> S;
-  extern __shared__ __attribute__((aligned(16))) char smem[];
+  extern __shared__ __attribute__((aligned(256))) char smem[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int u = xcd_unit(a.ntiles * a.Hq);
   if (u < 0) return;
@@ -271,34 +274,40 @@ struct Dkv {
     for (int ks = 0; ks < DP / 16; ++ks) asm volatile("" : "+v"(kf[ks]), "+v"(vf[ks]));
   }
   // soff: the tile's row statistics in LDS, planes of `plane` bytes: exponent offset, delta, (fp32: 1 / l)
-  template <bool MASK>
-  __device__ __forceinline__ void tile(uint32_t iq, uint32_t id, uint32_t soff, int plane, int q0) {
-    const uint32_t rp = launder(rpart), cp = launder(cpart);
+  __device__ __forceinline__ void tile(uint32_t iq, uint32_t id, uint32_t soff, int plane, int q0, bool mask) {
+    const uint32_t rq = launder(rpart + iq), rd = launder(rpart + id), cq = launder(cpart + iq), cd = launder(cpart + id);
     f32x16_t s = zero16(), dp = zero16();
 #pragma unroll
-    for (int ks = 0; ks < DP / 16; ++ks) s = O::mma(I::rows(iq, rp, ks), kf[ks], s);
+    for (int ks = 0; ks < DP / 16; ++ks) s = O::mma(I::rows(rq, ks), kf[ks], s);
 #pragma unroll
-    for (int ks = 0; ks < DP / 16; ++ks) dp = O::mma(I::rows(id, rp, ks), vf[ks], dp);
+    for (int ks = 0; ks < DP / 16; ++ks) dp = O::mma(I::rows(rd, ks), vf[ks], dp);
+    const uint32_t at = launder(soff + 16 * (lane >> 5));
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-      const uint32_t at = soff + 16 * (lane >> 5) + 32 * g;
-      const f32x4_t off = lds_read<f32x4_t>(at), dl = lds_read<f32x4_t>(at + plane);
+      const f32x4_t off = lds_read<f32x4_t>(at + 32 * g), dl = lds_read<f32x4_t>(at + plane + 32 * g);
       f32x4_t inv = {1.f, 1.f, 1.f, 1.f};
-      if constexpr (DT == MVF_F32) inv = lds_read<f32x4_t>(at + 2 * plane);
+      if constexpr (DT == MVF_F32) inv = lds_read<f32x4_t>(at + 2 * plane + 32 * g);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int e = 4 * g + j, q = q0 + 8 * g + 4 * (lane >> 5) + j;
+        const int e = 4 * g + j;
         float p = __builtin_amdgcn_exp2f(fmaf(s[e], c, off[j]));
         if constexpr (DT == MVF_F32) p *= inv[j];
-        const float ds = p * (dp[e] - dl[j]);
-        const bool sees = !MASK || (q >= own.lo && q < own.hi);
-        s[e] = sees ? p : 0.f;
-        dp[e] = sees ? ds : 0.f;
+        s[e] = p;
+        dp[e] = p * (dp[e] - dl[j]);
       }
     }
-    accumulate<O, DP>(dv, s, id, cp);
-    accumulate<O, DP>(dk, dp, iq, cp);
-    if constexpr (MASK) bad |= tile_nonfinite<O, DP>(id, lane) | tile_nonfinite<O, DP>(iq, lane);
+    if (mask) {
+      bad |= tile_nonfinite<O, DP>(id, lane) | tile_nonfinite<O, DP>(iq, lane);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int q = q0 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
+        const bool sees = q >= own.lo && q < own.hi;
+        s[e] = sees ? s[e] : 0.f;
+        dp[e] = sees ? dp[e] : 0.f;
+      }
+    }
+    accumulate<O, DP>(dv, s, cd);
+    accumulate<O, DP>(dk, dp, cq);
   }
   // over tiles it = first, first + step, ... of (head of the group, 32-query tile)
   __device__ __forceinline__ void slow(const BwdArgs& a, int kh, Span any, int first, int step) {
@@ -322,8 +331,7 @@ struct Dkv {
   }
   __device__ __forceinline__ void any_tile(const WaveSpan& ws, uint32_t iq, uint32_t id, uint32_t soff, int plane, int q0) {
     if (q0 >= ws.any.hi || q0 + 32 <= ws.any.lo) return;
-    if (q0 >= ws.all.lo && q0 + 32 <= ws.all.hi) tile<false>(iq, id, soff, plane, q0);
-    else tile<true>(iq, id, soff, plane, q0);
+    tile(iq, id, soff, plane, q0, q0 < ws.all.lo || q0 + 32 > ws.all.hi);
   }
 };
 
@@ -342,7 +350,7 @@ __global__ __launch_bounds__(256, DP > (DT == MVF_F32 ? 32 : 64) ? 1 : 2) void p
   typedef Ring<O, DP> R;
   constexpr int NF = planes(DT) * R::KB, SB = (NF + 63) / 64 * 256;     // floats of a block's statistics, bytes of their buffer
   static_assert(NF <= 256, "one piece per wave");
-  extern __shared__ __attribute__((aligned(16))) char smem[];
+  extern __shared__ __attribute__((aligned(256))) char smem[];
   __shared__ int s_span[8];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int u = xcd_unit(a.ntiles * a.Hk);
@@ -398,7 +406,7 @@ __global__ __launch_bounds__(256, 1) void packed_attn_dkv_split_kernel(BwdArgs a
   typedef Op<DT> O;
   typedef Tiles<O, DP> S;
   constexpr int NF = planes(DT) * 32, NSP = (NF + 63) / 64, SB = NSP * 256;
-  extern __shared__ __attribute__((aligned(16))) char smem[];
+  extern __shared__ __attribute__((aligned(256))) char smem[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int u = xcd_unit(a.ntiles * a.Hk);
   if (u < 0) return;
