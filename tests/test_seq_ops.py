@@ -111,7 +111,7 @@ def test_packed_entry_points_refuse(lib, name, value):
     assert lib.mvf_packed_attn_fwd(*a.values(), None) == 10001
     head = [a[n] for n in ('dtype', 'q', 'ldq', 'hsq', 'k', 'ldk', 'hsk', 'v', 'ldv', 'hsv', 'cu', 'n', 'out')]
     tail = [a[n] for n in ('T', 'Hq', 'Hk', 'D', 'frame', 'scale')]
-    assert lib.mvf_packed_attn_bwd(*head, P, P, P, P, P, P, *tail, None) == 10001
+    assert lib.mvf_packed_attn_bwd(*head, P, P, P, 1 << 40, P, P, P, *tail, None) == 10001
 
 
 @pytest.mark.parametrize('d', [0, 12, 136, -8])
@@ -125,7 +125,18 @@ def test_packed_backward_refuses_missing_buffers(lib, missing):
     bufs = [P] * 6
     bufs[missing] = None
     head = [FWD[n] for n in ('dtype', 'q', 'ldq', 'hsq', 'k', 'ldk', 'hsk', 'v', 'ldv', 'hsv', 'cu', 'n', 'out')]
-    assert lib.mvf_packed_attn_bwd(*head, *bufs, 4, 2, 2, 32, 1, 1.0, None) == 10001
+    assert lib.mvf_packed_attn_bwd(*head, *bufs[:3], 1 << 40, *bufs[3:], 4, 2, 2, 32, 1, 1.0, None) == 10001
+
+
+def test_packed_backward_workspace_is_asked_for_and_checked(lib):
+    head = [FWD[n] for n in ('dtype', 'q', 'ldq', 'hsq', 'k', 'ldk', 'hsk', 'v', 'ldv', 'hsv', 'cu', 'n', 'out')]
+    size = lib.mvf_packed_attn_bwd_workspace_bytes(_lib.BF16, 4, 1, 2, 2, 32)
+    assert size >= 4 * 2 * 4                                                         # delta
+    assert lib.mvf_packed_attn_bwd(*head, P, P, P, size - 1, P, P, P, 4, 2, 2, 32, 1, 1.0, None) == 10001
+    # few key heads: the group's heads are shared out and their sums kept in fp32; many: they are not
+    assert lib.mvf_packed_attn_bwd_workspace_bytes(_lib.BF16, 512, 1, 16, 4, 128) == 4 * (16 * 512 + 2 * 4 * 512 * 4 * 128)
+    assert lib.mvf_packed_attn_bwd_workspace_bytes(_lib.BF16, 1 << 17, 1, 16, 4, 128) == 4 * 16 * (1 << 17)
+    assert lib.mvf_packed_attn_bwd_workspace_bytes(_lib.BF16, 512, 1, 3, 2, 128) == 0
 
 
 ROT = dict(dtype=_lib.F32, q=P, ldq=64, hsq=32, k=P, ldk=64, hsk=32, pos=P, pos_type=0, freqs=P, s0=8, s1=4, s2=0, il=0, inv=0, qo=P, ko=P, T=4,

@@ -123,7 +123,8 @@ SIGNATURES = {
     'mvf_rotary': 'ipllpll' + 'pip' + 'iiiii' + 'pp' + 'iiiip',
     'mvf_rotary_append': 'ipllpllpll' + 'pip' + 'iiii' + 'ppp' + 'pii' + 'pp' + 'ii' + 'iiiip',
     'mvf_packed_attn_fwd': 'ipllpllpll' + 'pi' + 'pp' + 'iiiiifp',
-    'mvf_packed_attn_bwd': 'ipllpllpll' + 'pi' + 'ppppppp' + 'iiiiifp',
+    'mvf_packed_attn_bwd_workspace_bytes': 'iiiiii',
+    'mvf_packed_attn_bwd': 'ipllpllpll' + 'pi' + 'ppppz' + 'ppp' + 'iiiiifp',
     'mvf_paged_attn_workspace_bytes': 'iiiiiii',
     'mvf_paged_attn': 'iplllppppppz' + 'iiiiiiiiifp',
     'mvf_augment_workspace_bytes': 'iii',
@@ -227,7 +228,7 @@ def load():
         fn = getattr(lib, name)  # AttributeError if a declared symbol is not exported
         fn.argtypes = [_KIND[k] for k in sig]
         fn.restype = _Z if name in ('mvf_vit_workspace_bytes', 'mvf_bn_workspace_floats', 'mvf_augment_workspace_bytes',
-                                    'mvf_head_pack_elems', 'mvf_paged_attn_workspace_bytes') else _I
+                                    'mvf_head_pack_elems', 'mvf_packed_attn_bwd_workspace_bytes', 'mvf_paged_attn_workspace_bytes') else _I
     _lib = lib
     return lib
 

@@ -24,6 +24,9 @@ struct PagedArgs {
   float c;
 };
 
+// every stream cuts its own length evenly
+__device__ __forceinline__ int tiles_per_split(int ntile, int splits) { return max((ntile + splits - 1) / splits, 1); }
+
 template <int DT, int DP, bool PAD>
 __global__ __launch_bounds__(64 * NW, 1) void paged_attn_kernel(PagedArgs a) {
   typedef Op<DT> O;
@@ -37,7 +40,8 @@ __global__ __launch_bounds__(64 * NW, 1) void paged_attn_kernel(PagedArgs a) {
   const int split = blockIdx.x % a.splits, unit = blockIdx.x / a.splits;
   const int rt = unit % a.rt, kh = unit / a.rt % a.Hk, b = unit / a.rt / a.Hk;
   const int len = (int)max(0l, min((long)a.len[b], (long)a.width * a.page));
-  const int ntile = (len + 31) >> 5, per = (ntile + a.splits - 1) / a.splits;
+  const int ntile = (len + 31) >> 5, per = tiles_per_split(ntile, a.splits);
+  if (split > 0 && split * per >= ntile) return;
   const int t_end = min(ntile, (split + 1) * per);
   const int m0 = rt * 32, m = m0 + r, mi = m / a.g, rows = min(32, a.R - m0);
   int hi = 0;                                        // keys this row sees
@@ -191,7 +195,7 @@ __global__ __launch_bounds__(64 * NW, 1) void paged_attn_kernel(PagedArgs a) {
       }
   }
   __syncthreads();
-  join_waves<DP>(reinterpret_cast<float*>(smem), s_m, s_l, o, st, rows, a.D, wave, lane,
+  join_waves<DP, NW>(reinterpret_cast<float*>(smem), s_m, s_l, o, st, rows, a.D, wave, lane,
                  [&](int row, int d, const f32x4_t& acc, float mx, float l) {
     const int mm = m0 + row;
     if (a.splits == 1) {
@@ -220,8 +224,10 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
   const float* ml = a.part + (size_t)a.B * a.Hk * a.R * a.splits * a.D + (size_t)prow * a.splits * 2;
   const float* po = a.part + (size_t)prow * a.splits * a.D;
   const int tid = threadIdx.x;
+  const int len = (int)max(0l, min((long)a.len[prow / a.R / a.Hk], (long)a.width * a.page)), ntile = (len + 31) >> 5;
+  const int per = tiles_per_split(ntile, a.splits), n = max(1, (ntile + per - 1) / per);      // the splits that were written
   float m = NEG_INF, l = 0.f;
-  if (tid < a.splits) { m = ml[2 * tid]; l = ml[2 * tid + 1]; }
+  if (tid < n) { m = ml[2 * tid]; l = ml[2 * tid + 1]; }
   const float mw = wave_max(m);
   if ((tid & 63) == 0) s_red[tid >> 6] = mw;
   __syncthreads();
@@ -236,7 +242,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
   const int d = (tid & 31) * 4;
   f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
   if (d < a.D)
-    for (int s = tid >> 5; s < a.splits; s += 8)
+    for (int s = tid >> 5; s < n; s += 8)
       if (s_w[s] != 0.f) {
         const f32x4_t x = *reinterpret_cast<const f32x4_t*>(po + (size_t)s * a.D + d);
 #pragma unroll
@@ -255,15 +261,15 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
 
 // How many workgroups share a stream's keys.  The lengths are on the device; the host knows the longest possible one.
 int split_count(long units, long max_keys) {
-  const long fill = (512 + units - 1) / units;          // two workgroups per compute unit
-  const long most = (max_keys + 255) / 256;             // two tiles per wave
-  return (int)std::max(1l, std::min({std::max(fill, (max_keys + 1023) / 1024), most, 256l}));
+  const long fill = (2048 / NW + units - 1) / units;          // two workgroups per compute unit
+  const long most = (max_keys + 64 * NW - 1) / (64 * NW);             // two tiles per wave
+  return (int)std::max(1l, std::min({std::max(fill, (max_keys + 1024 - 1) / 1024), most, 256l}));
 }
 
 template <int DT, int DP, bool PAD>
 int launch(const PagedArgs& a, hipStream_t st) {
   typedef Tiles<Op<DT>, DP> S;
-  const size_t lds = std::max(NW * S::NB * S::BUF, JOIN_BYTES<DP>);
+  const size_t lds = std::max(NW * S::NB * S::BUF, (JOIN_BYTES<DP, NW>));
   static uint64_t attr = 0;
   if (int rc = mvf_ensure_lds(reinterpret_cast<const void*>(paged_attn_kernel<DT, DP, PAD>), lds, attr)) return rc;
   hipLaunchKernelGGL((paged_attn_kernel<DT, DP, PAD>), dim3((unsigned)a.B * a.Hk * a.rt * a.splits), dim3(64 * NW), lds, st, a);

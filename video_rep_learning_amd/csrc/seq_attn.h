@@ -252,13 +252,13 @@ __device__ __forceinline__ void wait_dma() {           // all but the wave's las
 }
 
 // A workgroup of four waves streams blocks of KB rows of two matrices (a and b) through a ring of three buffers: waves 0 and 1 fetch a's
-// pieces, waves 2 and 3 b's, block n + 2 is asked for right behind the one barrier of block n.  A row behind the last one repeats it;
+// pieces, waves 2 and 3 b's, block n + 2 is asked for right behind the one barrier of block n (with two buffers: block n + 1).  A row behind the last one repeats it;
 // chunks behind the row's D elements are not fetched (the caller cleared the buffers once).
-template <class O, int DP>
+template <class O, int DP, int NBUF = 3>
 struct Ring {
   typedef Img<O, DP> I;
   static constexpr int KB = I::RB <= 64 ? 128 : I::RB <= 128 ? 64 : 32;
-  static constexpr int IMG = KB * I::RB, BUF = 2 * IMG, NB = 3, PP = IMG / 2048;     // PP: pieces per wave and block
+  static constexpr int IMG = KB * I::RB, BUF = 2 * IMG, NB = NBUF, PP = IMG / 2048;     // PP: pieces per wave and block
   const char* p[PP];
   long ld;
   uint32_t on, lds;
@@ -293,10 +293,10 @@ struct Ring {
 };
 
 // A wave streams 32-row tiles of two matrices through buffers of its own (one or two): no barrier, nothing shared.
-template <class O, int DP>
+template <class O, int DP, int NBUF = (DP * O::SZ <= 256 ? 2 : 1)>
 struct Tiles {
   typedef Img<O, DP> I;
-  static constexpr int IMG = 32 * I::RB, BUF = 2 * IMG, NB = I::RB <= 256 ? 2 : 1, NP = I::C;    // NP: pieces per tile
+  static constexpr int IMG = 32 * I::RB, BUF = 2 * IMG, NB = NBUF, NP = I::C;    // NP: pieces per tile
   template <bool PAD, class RowAt>      // RowAt(i): byte offsets of the tile's row i in a and in b
   static __device__ __forceinline__ void issue(const char* a, const char* b, RowAt&& at, int D, int lane, uint32_t lds) {
 #pragma unroll
@@ -317,14 +317,37 @@ __device__ __forceinline__ void clear_lds(char* p, int bytes) {
   __syncthreads();
 }
 
-// blockIdx -> unit such that every XCD (workgroups go round them) gets a contiguous run of units: neighbours share keys and values
-__device__ __forceinline__ int xcd_unit(int units) {
-  const int per = (units + 7) >> 3, slot = blockIdx.x >> 3, u = (blockIdx.x & 7) * per + slot;
-  return slot < per && u < units ? u : -1;
+// blockIdx -> (head, tile).  Workgroups go round the 8 XCDs; a head's keys and values should stay in one XCD's cache, every XCD should get the
+// same share of long and short tiles, and the tiles should start in their order.  Heads a multiple of 8: an eighth of them on each XCD; of
+// 4: a quarter on each pair of XCDs, which take the tiles in turn; else: runs of (head, tile) units.
+struct Unit { int head, tile; };
+__device__ __forceinline__ Unit xcd_unit(int heads, int tiles) {
+  const int x = blockIdx.x & 7, s = blockIdx.x >> 3;
+  if ((heads & 7) == 0) {
+    const int h = heads >> 3;
+    return {x * h + s % h, s / h};
+  }
+  if ((heads & 3) == 0) {
+    const int h = heads >> 2, t = 2 * (s / h) + (x >> 2);
+    return {t < tiles ? (x & 3) * h + s % h : -1, t};
+  }
+  const int units = heads * tiles, per = (units + 7) >> 3, u = x * per + s;
+  return {s < per && u < units ? u / tiles : -1, u % tiles};
 }
-#ifndef MVF_SPLIT_RULE
-#define MVF_SPLIT_RULE(x) ((x) < 512)
+static inline unsigned xcd_grid(long heads, long tiles) {
+  return (unsigned)((heads & 7) == 0 ? heads * tiles : (heads & 3) == 0 ? heads * ((tiles + 1) / 2 * 2) : (heads * tiles + 7) / 8 * 8);
+}
+
+// Which form: `wide` = the wide one's workgroups.  Below one for each of the 256 compute units the split form is faster (measured, us: 1 x 512
+// bf16 D 128 16 heads, 80 workgroups: wide 20, split 13; 4 x 197 D 64, 96: 10.5, 9.5), above it the wide one (16 x 197 D 64, 384: 13, 23;
+// 4 x 1024 D 128, 544: 43, 96) unless few workgroups walk far: up to two for each unit and 4096 tokens a sequence (1 x 4096 D 64, 408: 99,
+// 82; 1 x 2048 D 128, 304: 62, 69), in fp32, whose walks are 8 times as long, 1024 (4 x 1024 D 128, 280: 157, 131; 8 x 400 D 64, 384: 65, 83).
+static inline bool use_split(long wide, int dtype, long T, long n_seqs) {
+#ifdef MVF_SPLIT_FORCE     // build flag, A/B measurements only
+  return MVF_SPLIT_FORCE;
 #endif
+  return wide < 256 || (wide < 512 && T >= (dtype == MVF_F32 ? 1024 : 4096) * n_seqs);
+}
 static inline unsigned xcd_grid(long units) { return (unsigned)((units + 7) / 8 * 8); }
 
 // ---------------------------------------------------------------------------------------------- which rows meet
@@ -338,14 +361,78 @@ template <int ROWS>
 static inline long tile_bound(long T, long n) {   // no fewer than the tiles there are
   return n > SEQ_TILES ? (T + ROWS - 1) / ROWS : (T + (ROWS - 1) * (n + 2 < T ? n + 2 : T)) / ROWS;
 }
-// the t-th tile, found by every wave for itself: lane i sizes segment i, one prefix sum per 64 of them
+// The t-th tile, found by every wave for itself.  Up to 62 sequences the tiles come in the order of their walks, longest first (causal: the
+// tile's place in its sequence, counted from the end that sees most; else the sequence's length), so that the last workgroups to
+// finish are short ones: lane i holds segment i, and the walk w of the t-th tile is found by 64 candidates at a time, F(w) = tiles
+// that walk at least w.  Beyond that sequence by sequence, with a prefix sum per 64 of them.
+enum class Walk { ALL, LATE, EARLY };             // non-causal; causal: late rows walk far (queries), early rows do (keys)
+__device__ __forceinline__ int nth_bit(uint64_t m, int k) {
+  for (; k > 0; --k) m &= m - 1;
+  return __builtin_ctzll(m);
+}
 template <int ROWS>
-__device__ __forceinline__ OwnTile find_tile(const int* __restrict__ cu, int n, int T, int t) {
-  if (n > SEQ_TILES) return {t * ROWS, min(T, t * ROWS + ROWS), {0, 0}};
+__device__ __forceinline__ OwnTile find_tile(const int* __restrict__ cu, int n, int T, int t, int bound, Walk walk) {
   const int lane = threadIdx.x & 63;
+  if (n > SEQ_TILES) {
+    if (walk == Walk::LATE) t = bound - 1 - t;
+    return {t * ROWS, min(T, t * ROWS + ROWS), {0, 0}};
+  }
+  if (n <= 62) {
+    const int i = lane;                             // segment 0: rows before cu[0]; i: sequence i - 1; n + 1: rows behind cu[n]
+    const int lo = i == 0 ? 0 : min(max(cu[min(i - 1, n)], 0), T), hi = i > n ? T : min(max(cu[min(i, n)], 0), T);
+    const int tiles = i < n + 2 && hi > lo ? (hi - lo + ROWS - 1) / ROWS : 0;
+    const int c = i > 0 && i <= n ? tiles : 0;      // of sequences
+    int most = 0, total = 0;
+    for (int k0 = 0; k0 <= n; k0 += 8)              // (lanes behind n hold 0)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int x = __builtin_amdgcn_readlane(c, k0 + k);
+        most = max(most, x);
+        total += x;
+      }
+    if (t >= total) {                               // rows of no sequence
+      const int g0 = __builtin_amdgcn_readlane(tiles, 0), j = t - total, seg = j < g0 ? 0 : n + 1, k = j < g0 ? j : j - g0;
+      if (seg != 0 && k >= __builtin_amdgcn_readlane(tiles, n + 1)) return {0, 0, {0, 0}};
+      const int l = __builtin_amdgcn_readlane(lo, seg), h = __builtin_amdgcn_readlane(hi, seg);
+      return {l + k * ROWS, min(h, l + k * ROWS + ROWS), {0, 0}};
+    }
+    int w0 = 1, w1 = most + 1, above = 0;           // the smallest w with F(w) <= t; above = F(w)
+    while (true) {
+      const int step = (w1 - w0 + 62) / 63, w = min(w0 + lane * max(step, 1), w1);
+      int f = 0;
+      for (int k0 = 0; k0 <= n; k0 += 8) {
+        if (walk == Walk::ALL) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const int x = __builtin_amdgcn_readlane(c, k0 + k);
+            f += x >= w ? x : 0;
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) f += max(__builtin_amdgcn_readlane(c, k0 + k) - w + 1, 0);
+        }
+      }
+      const uint64_t ok = __builtin_amdgcn_ballot_w64(f <= t);       // never 0: lane 63 stands at w1
+      const int j = __builtin_ctzll(ok);
+      const int at = __builtin_amdgcn_readlane(w, j);
+      if (j == 0 || step <= 1) {
+        w1 = at;
+        above = __builtin_amdgcn_readlane(f, j);
+        break;
+      }
+      w0 = __builtin_amdgcn_readlane(w, j - 1) + 1;
+      w1 = at;
+    }
+    const int w = w1 - 1, r = t - above;            // the tile's walk, its place among those
+    const int seg = walk == Walk::ALL ? nth_bit(__builtin_amdgcn_ballot_w64(c == w), r / w) : nth_bit(__builtin_amdgcn_ballot_w64(c >= w), r);
+    const int j = walk == Walk::ALL ? r % w : walk == Walk::LATE ? w - 1 : __builtin_amdgcn_readlane(c, seg) - w;
+    const int l = __builtin_amdgcn_readlane(lo, seg), h = __builtin_amdgcn_readlane(hi, seg);
+    return {l + j * ROWS, min(h, l + j * ROWS + ROWS), {l, h}};
+  }
+  if (walk == Walk::LATE) t = bound - 1 - t;
   int before = 0;
   for (int s0 = 0; s0 < n + 2; s0 += 64) {
-    const int i = s0 + lane;                        // segment 0: rows before cu[0]; i: sequence i - 1; n + 1: rows behind cu[n]
+    const int i = s0 + lane;
     const int lo = i == 0 ? 0 : min(max(cu[min(i - 1, n)], 0), T), hi = i > n ? T : min(max(cu[i], 0), T);
     const int tiles = i < n + 2 && hi > lo ? (hi - lo + ROWS - 1) / ROWS : 0;
     int sum = tiles;
@@ -438,12 +525,12 @@ __device__ __forceinline__ Span block_span(const WaveSpan& ws, int* s_span, int 
   return {__builtin_amdgcn_readfirstlane(s.hi == 0 ? 0 : s.lo), __builtin_amdgcn_readfirstlane(s.hi)};
 }
 
-// Four waves hold partial softmaxes of the same 32 rows: sums o^T against their own maxima.  Joins them in LDS (fixed order) and hands
+// NW waves hold partial softmaxes of the same 32 rows: sums o^T against their own maxima.  Joins them in LDS (fixed order) and hands
 // use(row, first channel of four, unnormalised sums, maximum in the exponent's units, sum of weights) for every row and channel.  All
 // threads; the caller's earlier LDS reads are behind a barrier.
-template <int DP>
-constexpr int JOIN_BYTES = 4 * 32 * (DP + 4) * 4;
-template <int DP, class Use>
+template <int DP, int NW = 4>
+constexpr int JOIN_BYTES = NW * 32 * (DP + 4) * 4;
+template <int DP, int NW = 4, class Use>
 __device__ __forceinline__ void join_waves(float* so, float (*s_m)[32], float (*s_l)[32], const f32x16_t (&o)[DP / 32], const RowMax& st,
                                            int rows, int D, int wave, int lane, Use&& use) {
   constexpr int ROWF = DP + 4;
@@ -459,16 +546,16 @@ __device__ __forceinline__ void join_waves(float* so, float (*s_m)[32], float (*
             (f32x4_t){o[dt][4 * g], o[dt][4 * g + 1], o[dt][4 * g + 2], o[dt][4 * g + 3]};
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < rows * (DP / 4); i += 256) {
+  for (int i = threadIdx.x; i < rows * (DP / 4); i += 64 * NW) {
     const int row = i / (DP / 4), d = i % (DP / 4) * 4;
     if (d >= D) continue;
     float mx = NEG_INF;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) mx = fmaxf(mx, s_m[w][row]);
+    for (int w = 0; w < NW; ++w) mx = fmaxf(mx, s_m[w][row]);
     float sum = 0.f;
     f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < NW; ++w) {
       const float m = s_m[w][row], lw = s_l[w][row];
       if (m == NEG_INF && lw == lw) continue;                 // saw nothing (a NaN sum with no maximum saw a NaN)
       const float f = m == NEG_INF ? lw : __builtin_amdgcn_exp2f(m - mx);

@@ -135,10 +135,10 @@ __global__ __launch_bounds__(256, DT == MVF_F32 && DP > 64 ? 1 : 2) void packed_
   extern __shared__ __attribute__((aligned(256))) char smem[];
   __shared__ int s_span[8];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int u = xcd_unit(a.ntiles * a.Hq);
-  if (u < 0) return;
-  const int head = u / a.ntiles, tile = a.ntiles - 1 - u % a.ntiles;       // the longest walks (causal: the last rows) first
-  const OwnTile own = find_tile<128>(a.cu, a.n_seqs, a.T, tile);
+  const Unit u = xcd_unit(a.Hq, a.ntiles);
+  if (u.head < 0) return;
+  const int head = u.head;
+  const OwnTile own = find_tile<128>(a.cu, a.n_seqs, a.T, u.tile, a.ntiles, a.frame == 0 ? Walk::ALL : Walk::LATE);
   if (own.row0 >= own.end) return;
   const int row = own.row0 + wave * 32 + (lane & 31);
   Fwd<DT, DP> f;
@@ -192,10 +192,10 @@ __global__ __launch_bounds__(256, 1) void packed_attn_fwd_split_kernel(FwdArgs a
   extern __shared__ __attribute__((aligned(256))) char smem[];
   __shared__ float s_m[4][32], s_l[4][32];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int u = xcd_unit(a.ntiles * a.Hq);
-  if (u < 0) return;
-  const int head = u / a.ntiles, tile = a.ntiles - 1 - u % a.ntiles;
-  const OwnTile own = find_tile<32>(a.cu, a.n_seqs, a.T, tile);
+  const Unit u = xcd_unit(a.Hq, a.ntiles);
+  if (u.head < 0) return;
+  const int head = u.head;
+  const OwnTile own = find_tile<32>(a.cu, a.n_seqs, a.T, u.tile, a.ntiles, a.frame == 0 ? Walk::ALL : Walk::LATE);
   if (own.row0 >= own.end) return;
   const int row0 = own.row0, row = row0 + (lane & 31);
   Fwd<DT, DP> f;
@@ -244,23 +244,22 @@ __global__ __launch_bounds__(256, 1) void packed_attn_fwd_split_kernel(FwdArgs a
   });
 }
 
-// The split form while the wide one's workgroups are fewer than two for each of the 256 compute units.
 template <int DT, int DP, bool PAD>
 int launch(FwdArgs a, hipStream_t st) {
   typedef Ring<Op<DT>, DP> R;
   typedef Tiles<Op<DT>, DP> S;
-  if (MVF_SPLIT_RULE(tile_bound<128>(a.T, a.n_seqs) * a.Hq)) {
+  if (use_split(tile_bound<128>(a.T, a.n_seqs) * a.Hq, DT, a.T, a.n_seqs)) {
     const size_t lds = std::max(4 * S::NB * S::BUF, JOIN_BYTES<DP>);
     static uint64_t attr = 0;
     if (int rc = mvf_ensure_lds(reinterpret_cast<const void*>(packed_attn_fwd_split_kernel<DT, DP, PAD>), lds, attr)) return rc;
     a.ntiles = (int)tile_bound<32>(a.T, a.n_seqs);
-    hipLaunchKernelGGL((packed_attn_fwd_split_kernel<DT, DP, PAD>), dim3(xcd_grid((long)a.ntiles * a.Hq)), dim3(256), lds, st, a);
+    hipLaunchKernelGGL((packed_attn_fwd_split_kernel<DT, DP, PAD>), dim3(xcd_grid(a.Hq, a.ntiles)), dim3(256), lds, st, a);
   } else {
     const size_t lds = R::NB * R::BUF;
     static uint64_t attr = 0;
     if (int rc = mvf_ensure_lds(reinterpret_cast<const void*>(packed_attn_fwd_kernel<DT, DP, PAD>), lds, attr)) return rc;
     a.ntiles = (int)tile_bound<128>(a.T, a.n_seqs);
-    hipLaunchKernelGGL((packed_attn_fwd_kernel<DT, DP, PAD>), dim3(xcd_grid((long)a.ntiles * a.Hq)), dim3(256), lds, st, a);
+    hipLaunchKernelGGL((packed_attn_fwd_kernel<DT, DP, PAD>), dim3(xcd_grid(a.Hq, a.ntiles)), dim3(256), lds, st, a);
   }
   MVF_LAUNCH_CHECK();
   return MVF_OK;

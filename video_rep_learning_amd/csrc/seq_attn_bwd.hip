@@ -19,6 +19,8 @@ struct BwdArgs {
   const char *out, *d_out;             // [T, Hq, D]
   const float* stat;                   // [2][Hq][T] of the forward
   float* delta;                        // [Hq][T]
+  float* part;                         // parts > 1: [parts][2 (dk, dv)][T][Hk][D]
+  int parts;                           // workgroups that share a group's heads
   char *dq, *dk, *dv;                  // [T, Hq, D], [T, Hk, D] x 2
   int T, Hq, Hk, D, frame, ntiles;
   float c, scale;
@@ -50,6 +52,9 @@ __device__ __forceinline__ void store_rows(char* base, size_t row_elems, const f
       }
     }
 }
+
+// the fp32 format of the partial sums
+typedef Op<MVF_F32> Part;
 
 // The four waves' sums of the same 32 rows, added in order: wave 0 + 1 + 2 + 3, out as [row][D].  All threads; barriers inside.
 template <class O, int DP>
@@ -167,10 +172,10 @@ __global__ __launch_bounds__(256, DT == MVF_F32 && DP > 32 ? 1 : 2) void packed_
   extern __shared__ __attribute__((aligned(256))) char smem[];
   __shared__ int s_span[8];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int u = xcd_unit(a.ntiles * a.Hq);
-  if (u < 0) return;
-  const int head = u / a.ntiles, tile = a.ntiles - 1 - u % a.ntiles;
-  const OwnTile own = find_tile<128>(a.cu, a.n_seqs, a.T, tile);
+  const Unit u = xcd_unit(a.Hq, a.ntiles);
+  if (u.head < 0) return;
+  const int head = u.head;
+  const OwnTile own = find_tile<128>(a.cu, a.n_seqs, a.T, u.tile, a.ntiles, a.frame == 0 ? Walk::ALL : Walk::LATE);
   if (own.row0 >= own.end) return;
   const int row = own.row0 + wave * 32 + (lane & 31);
   Dq<DT, DP> f;
@@ -206,10 +211,10 @@ __global__ __launch_bounds__(256, 1) void packed_attn_dq_split_kernel(BwdArgs a)
   typedef Tiles<O, DP> S;
   extern __shared__ __attribute__((aligned(256))) char smem[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int u = xcd_unit(a.ntiles * a.Hq);
-  if (u < 0) return;
-  const int head = u / a.ntiles, tile = a.ntiles - 1 - u % a.ntiles;
-  const OwnTile own = find_tile<32>(a.cu, a.n_seqs, a.T, tile);
+  const Unit u = xcd_unit(a.Hq, a.ntiles);
+  if (u.head < 0) return;
+  const int head = u.head;
+  const OwnTile own = find_tile<32>(a.cu, a.n_seqs, a.T, u.tile, a.ntiles, a.frame == 0 ? Walk::ALL : Walk::LATE);
   if (own.row0 >= own.end) return;
   const int row0 = own.row0, row = row0 + (lane & 31);
   Dq<DT, DP> f;
@@ -248,11 +253,14 @@ __global__ __launch_bounds__(256, 1) void packed_attn_dq_split_kernel(BwdArgs a)
 }
 
 // ------------------------------------------------------------------------------------------------ dK, dV
-template <int DT, int DP>
+// VL: the wave's own V rows as an image in LDS instead of registers: 16-bit D = 128 then fits two waves on a SIMD, whose products and
+// exponentials overlap (one wave with everything in registers: 2.2 ms for 2 x 8192 causal 16/4 heads, this: see the launcher).
+template <int DT, int DP, bool VL>
 struct Dkv {
   typedef Op<DT> O;
   typedef Img<O, DP> I;
-  typename O::Frag kf[DP / 16], vf[DP / 16];
+  typename O::Frag kf[DP / 16], vf[VL ? 1 : DP / 16];
+  uint32_t vimg;
   f32x16_t dk[DP / 32], dv[DP / 32];
   Span own;
   float c;
@@ -260,18 +268,28 @@ struct Dkv {
   uint32_t rpart, cpart;
   bool bad = false;        // a tile with masked places held a value that is not finite
 
-  __device__ __forceinline__ void start(const BwdArgs& a, int kh, int row, int lane_) {
+  __device__ __forceinline__ void start(const BwdArgs& a, int kh, int row, int lane_, char* own_v) {
     lane = lane_;
     rpart = I::row_part(lane);
     cpart = I::col_part(lane);
     c = a.c;
     const int rr = min(row, a.T - 1);
     load_row<O, DP>(kf, a.k + (long)rr * a.ldk + kh * a.hsk, a.D, lane >> 5);
-    load_row<O, DP>(vf, a.v + (long)rr * a.ldv + kh * a.hsv, a.D, lane >> 5);
+    if constexpr (VL) {
+      typename O::Frag x[DP / 16];
+      load_row<O, DP>(x, a.v + (long)rr * a.ldv + kh * a.hsv, a.D, lane >> 5);
+#pragma unroll
+      for (int ks = 0; ks < DP / 16; ++ks) *reinterpret_cast<typename O::Frag*>(own_v + I::off(lane & 31, 2 * ks + (lane >> 5))) = x[ks];
+      vimg = lds_addr(own_v);
+    } else {
+      load_row<O, DP>(vf, a.v + (long)rr * a.ldv + kh * a.hsv, a.D, lane >> 5);
+#pragma unroll
+      for (int ks = 0; ks < DP / 16; ++ks) asm volatile("" : "+v"(vf[ks]));
+    }
 #pragma unroll
     for (int dt = 0; dt < DP / 32; ++dt) { dk[dt] = zero16(); dv[dt] = zero16(); }
 #pragma unroll
-    for (int ks = 0; ks < DP / 16; ++ks) asm volatile("" : "+v"(kf[ks]), "+v"(vf[ks]));
+    for (int ks = 0; ks < DP / 16; ++ks) asm volatile("" : "+v"(kf[ks]));
   }
   // soff: the tile's row statistics in LDS, planes of `plane` bytes: exponent offset, delta, (fp32: 1 / l)
   __device__ __forceinline__ void tile(uint32_t iq, uint32_t id, uint32_t soff, int plane, int q0, bool mask) {
@@ -279,8 +297,9 @@ struct Dkv {
     f32x16_t s = zero16(), dp = zero16();
 #pragma unroll
     for (int ks = 0; ks < DP / 16; ++ks) s = O::mma(I::rows(rq, ks), kf[ks], s);
+    const uint32_t ro = VL ? launder(rpart + vimg) : 0;
 #pragma unroll
-    for (int ks = 0; ks < DP / 16; ++ks) dp = O::mma(I::rows(rd, ks), vf[ks], dp);
+    for (int ks = 0; ks < DP / 16; ++ks) dp = O::mma(I::rows(rd, ks), VL ? I::rows(ro, ks) : vf[VL ? 0 : ks], dp);
     const uint32_t at = launder(soff + 16 * (lane >> 5));
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
@@ -309,14 +328,16 @@ struct Dkv {
     accumulate<O, DP>(dv, s, cd);
     accumulate<O, DP>(dk, dp, cq);
   }
-  // over tiles it = first, first + step, ... of (head of the group, 32-query tile)
-  __device__ __forceinline__ void slow(const BwdArgs& a, int kh, Span any, int first, int step) {
+  // over tiles it = first, first + step, ... of (head h0 + .. of g, 32-query tile)
+  __device__ __forceinline__ void slow(const BwdArgs& a, int kh, int row, int h0, int g, Span any, int first, int step) {
+    typename O::Frag vf[DP / 16];
+    load_row<O, DP>(vf, a.v + (long)min(row, a.T - 1) * a.ldv + kh * a.hsv, a.D, lane >> 5);
 #pragma unroll
     for (int dt = 0; dt < DP / 32; ++dt) { dk[dt] = zero16(); dv[dt] = zero16(); }
-    const int g = a.Hq / a.Hk, nt = (any.hi - any.lo + 31) >> 5;
+    const int nt = (any.hi - any.lo + 31) >> 5;
 #pragma unroll 1
     for (int it = first; it < nt * g; it += step) {
-      const int h = kh * g + it / nt, q0 = any.lo + it % nt * 32;
+      const int h = h0 + it / nt, q0 = any.lo + it % nt * 32;
 #pragma unroll 1
       for (int q = q0; q < min(q0 + 32, any.hi); ++q) {
         const char *qr = a.q + (long)q * a.ldq + h * a.hsq, *dr = a.d_out + ((size_t)q * a.Hq + h) * a.D * O::SZ;
@@ -343,33 +364,40 @@ __device__ __forceinline__ const float* stat_at(const BwdArgs& a, int h, int row
   return base + (size_t)h * a.T + min(row + f % n, a.T - 1);
 }
 
+template <int DT, int DP>
+constexpr bool V_IN_LDS = DT != MVF_F32 && DP == 128;
+template <int DT, int DP>
+using DkvRing = Ring<Op<DT>, DP, V_IN_LDS<DT, DP> ? 2 : 3>;
+
 template <int DT, int DP, bool PAD>
-__global__ __launch_bounds__(256, DP > (DT == MVF_F32 ? 32 : 64) ? 1 : 2) void packed_attn_dkv_kernel(BwdArgs a) {
+__global__ __launch_bounds__(256, DT == MVF_F32 && DP > 32 ? 1 : 2) void packed_attn_dkv_kernel(BwdArgs a) {
   typedef Op<DT> O;
   typedef Img<O, DP> I;
-  typedef Ring<O, DP> R;
+  typedef DkvRing<DT, DP> R;
+  constexpr bool VL = V_IN_LDS<DT, DP>;
   constexpr int NF = planes(DT) * R::KB, SB = (NF + 63) / 64 * 256;     // floats of a block's statistics, bytes of their buffer
   static_assert(NF <= 256, "one piece per wave");
   extern __shared__ __attribute__((aligned(256))) char smem[];
   __shared__ int s_span[8];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int u = xcd_unit(a.ntiles * a.Hk);
-  if (u < 0) return;
-  const int kh = u / a.ntiles, tile = u % a.ntiles;                       // causal: the first keys have the longest walks
-  const OwnTile own = find_tile<128>(a.cu, a.n_seqs, a.T, tile);
+  const Unit u = xcd_unit(a.Hk * a.parts, a.ntiles);
+  if (u.head < 0) return;
+  const int kh = u.head / a.parts, part = u.head % a.parts;
+  const OwnTile own = find_tile<128>(a.cu, a.n_seqs, a.T, u.tile, a.ntiles, a.frame == 0 ? Walk::ALL : Walk::EARLY);
   if (own.row0 >= own.end) return;
   const int row = own.row0 + wave * 32 + (lane & 31);
-  Dkv<DT, DP> f;
-  f.start(a, kh, row, lane);
+  Dkv<DT, DP, VL> f;
+  f.start(a, kh, row, lane, smem + R::NB * (R::BUF + SB) + wave * 32 * I::RB);
   f.own = queries_of(sequence_of(own, a.cu, a.n_seqs, a.T, row), a.frame, row);
   const WaveSpan ws = wave_span(f.own);
   if constexpr (PAD) clear_lds(smem, R::NB * R::BUF);
   const Span span = block_span(ws, s_span, lane, wave, 4);
-  const int g = a.Hq / a.Hk, nblk = span.hi > span.lo ? (span.hi - span.lo + R::KB - 1) / R::KB : 0, total = nblk * g;
+  const int g = a.Hq / a.Hk / a.parts, h0 = kh * (a.Hq / a.Hk) + part * g;
+  const int nblk = span.hi > span.lo ? (span.hi - span.lo + R::KB - 1) / R::KB : 0, total = nblk * g;
   const uint32_t lds0 = lds_addr(smem), stat0 = lds0 + R::NB * R::BUF;
   const int sp = min(wave, SB / 256 - 1);                                 // (a wave without a piece of its own repeats the last one)
   R ring;
-  int ih = kh * g, ib = 0;                                                // head and block that are asked for next
+  int ih = h0, ib = 0;                                                    // head and block that are asked for next
   auto issue = [&](int buf) __attribute__((always_inline)) {
     if (ib == 0)
       ring.start(a.q + ih * a.hsq, a.ldq, a.d_out + (size_t)ih * a.D * O::SZ, (long)a.Hq * a.D * O::SZ, span.lo, a.D, wave, lane, lds0);
@@ -379,25 +407,32 @@ __global__ __launch_bounds__(256, DP > (DT == MVF_F32 ? 32 : 64) ? 1 : 2) void p
     if (++ib == nblk) { ib = 0; ++ih; }
   };
   if (total > 0) issue(0);
-  if (total > 1) issue(1);
+  if (R::NB == 3 && total > 1) issue(1);
   int buf = 0, b0 = span.lo;
   for (int it = 0; it < total; ++it) {
-    if (it + 1 < total) wait_dma<R::PP + 1>();
+    if (R::NB == 3 && it + 1 < total) wait_dma<R::PP + 1>();
     else wait_dma<0>();
     __builtin_amdgcn_s_barrier();
-    if (it + 2 < total) issue(buf == 0 ? 2 : buf - 1);
+    if (it + R::NB - 1 < total) issue(buf == 0 ? R::NB - 1 : buf - 1);
     const uint32_t iq = lds0 + buf * R::BUF, so = stat0 + buf * SB;
 #pragma unroll 1
     for (int t = 0; t < R::KB / 32; ++t)
       f.any_tile(ws, iq + t * 32 * I::RB, iq + R::IMG + t * 32 * I::RB, so + t * 128, R::KB * 4, b0 + 32 * t);
-    buf = buf == 2 ? 0 : buf + 1;
+    buf = buf == R::NB - 1 ? 0 : buf + 1;
     b0 += R::KB;
     if (b0 >= span.hi) b0 = span.lo;
   }
-  if (f.bad) f.slow(a, kh, ws.any, 0, 1);
-  if (row < own.end) {
-    store_rows<O, DP>(a.dk, ((size_t)row * a.Hk + kh) * a.D, f.dk, a.scale, f.own.hi > 0, a.D, lane >> 5);
-    store_rows<O, DP>(a.dv, ((size_t)row * a.Hk + kh) * a.D, f.dv, 1.f, f.own.hi > 0, a.D, lane >> 5);
+  if (f.bad) f.slow(a, kh, row, h0, g, ws.any, 0, 1);
+  if (row >= own.end) return;
+  const size_t at = ((size_t)row * a.Hk + kh) * a.D;
+  if (a.parts > 1) {
+    const size_t plane = (size_t)a.T * a.Hk * a.D;
+    char* base = reinterpret_cast<char*>(a.part + 2 * part * plane);
+    store_rows<Part, DP>(base, at, f.dk, a.scale, f.own.hi > 0, a.D, lane >> 5);
+    store_rows<Part, DP>(base, plane + at, f.dv, 1.f, f.own.hi > 0, a.D, lane >> 5);
+  } else {
+    store_rows<O, DP>(a.dk, at, f.dk, a.scale, f.own.hi > 0, a.D, lane >> 5);
+    store_rows<O, DP>(a.dv, at, f.dv, 1.f, f.own.hi > 0, a.D, lane >> 5);
   }
 }
 
@@ -408,21 +443,21 @@ __global__ __launch_bounds__(256, 1) void packed_attn_dkv_split_kernel(BwdArgs a
   constexpr int NF = planes(DT) * 32, NSP = (NF + 63) / 64, SB = NSP * 256;
   extern __shared__ __attribute__((aligned(256))) char smem[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int u = xcd_unit(a.ntiles * a.Hk);
-  if (u < 0) return;
-  const int kh = u / a.ntiles, tile = u % a.ntiles;
-  const OwnTile own = find_tile<32>(a.cu, a.n_seqs, a.T, tile);
+  const Unit u = xcd_unit(a.Hk * a.parts, a.ntiles);
+  if (u.head < 0) return;
+  const int kh = u.head / a.parts, part = u.head % a.parts;
+  const OwnTile own = find_tile<32>(a.cu, a.n_seqs, a.T, u.tile, a.ntiles, a.frame == 0 ? Walk::ALL : Walk::EARLY);
   if (own.row0 >= own.end) return;
   const int row0 = own.row0, row = row0 + (lane & 31);
-  Dkv<DT, DP> f;
-  f.start(a, kh, row, lane);
+  Dkv<DT, DP, false> f;
+  f.start(a, kh, row, lane, nullptr);
   f.own = queries_of(sequence_of(own, a.cu, a.n_seqs, a.T, row), a.frame, row);
   const WaveSpan ws = wave_span(f.own);
   if constexpr (PAD) clear_lds(smem, 4 * S::NB * S::BUF);
-  const int g = a.Hq / a.Hk, nt = (ws.any.hi - ws.any.lo + 31) >> 5, total = nt * g;
+  const int g = a.Hq / a.Hk / a.parts, h0 = kh * (a.Hq / a.Hk) + part * g, nt = (ws.any.hi - ws.any.lo + 31) >> 5, total = nt * g;
   const uint32_t lds = lds_addr(smem) + wave * S::NB * S::BUF, stat0 = lds_addr(smem) + 4 * S::NB * S::BUF + wave * S::NB * SB;
   auto issue = [&](int it, int buf) __attribute__((always_inline)) {
-    const int h = kh * g + it / nt, q0 = ws.any.lo + it % nt * 32;
+    const int h = h0 + it / nt, q0 = ws.any.lo + it % nt * 32;
     const long ldo = (long)a.Hq * a.D * O::SZ;
     S::template issue<PAD>(a.q + h * a.hsq, a.d_out + (size_t)h * a.D * O::SZ, [&](int i, long& oa, long& ob) {
       const long r = min(q0 + i, ws.any.hi - 1);
@@ -443,48 +478,84 @@ __global__ __launch_bounds__(256, 1) void packed_attn_dkv_split_kernel(BwdArgs a
     if (S::NB == 2) buf ^= 1;
     else if (more) issue(it + 4, 0);
   }
-  if (f.bad) f.slow(a, kh, ws.any, wave, 4);
+  if (f.bad) f.slow(a, kh, row, h0, g, ws.any, wave, 4);
   if (f.own.hi == 0) {
 #pragma unroll
     for (int dt = 0; dt < DP / 32; ++dt) { f.dk[dt] = zero16(); f.dv[dt] = zero16(); }
   }
   const int rows = own.end - row0;
   float* so = reinterpret_cast<float*>(smem);
-  store_joined<O, DP>(so, f.dk, a.dk + (size_t)kh * a.D * O::SZ, row0, rows, (long)a.Hk * a.D, a.scale, a.D, wave, lane);
-  store_joined<O, DP>(so, f.dv, a.dv + (size_t)kh * a.D * O::SZ, row0, rows, (long)a.Hk * a.D, 1.f, a.D, wave, lane);
+  if (a.parts > 1) {
+    const size_t plane = (size_t)a.T * a.Hk * a.D;
+    float* base = a.part + 2 * part * plane + (size_t)kh * a.D;
+    store_joined<Part, DP>(so, f.dk, reinterpret_cast<char*>(base), row0, rows, (long)a.Hk * a.D, a.scale, a.D, wave, lane);
+    store_joined<Part, DP>(so, f.dv, reinterpret_cast<char*>(base + plane), row0, rows, (long)a.Hk * a.D, 1.f, a.D, wave, lane);
+  } else {
+    store_joined<O, DP>(so, f.dk, a.dk + (size_t)kh * a.D * O::SZ, row0, rows, (long)a.Hk * a.D, a.scale, a.D, wave, lane);
+    store_joined<O, DP>(so, f.dv, a.dv + (size_t)kh * a.D * O::SZ, row0, rows, (long)a.Hk * a.D, 1.f, a.D, wave, lane);
+  }
 }
 
-// The split forms while the wide ones' workgroups are fewer than two for each of the 256 compute units.
+// dk and dv from the parts, added in order: n elements each (a multiple of 4)
+template <int DT>
+__global__ __launch_bounds__(256) void packed_attn_sum_kernel(const float* part, int parts, size_t n, char* dk, char* dv) {
+  typedef Op<DT> O;
+  const size_t i = ((size_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= 2 * n) return;
+  f32x4_t acc = *reinterpret_cast<const f32x4_t*>(part + i);
+  for (int p = 1; p < parts; ++p) acc += *reinterpret_cast<const f32x4_t*>(part + 2 * n * p + i);
+  O::store4(reinterpret_cast<typename O::E*>(i < n ? dk : dv) + (i < n ? i : i - n), acc[0], acc[1], acc[2], acc[3]);
+}
+
+// Into how many parts a group's heads are cut in the dK / dV kernel: the smallest divisor that gives it four workgroups for each of the 256
+// compute units (causal walks are of all lengths), or all of them.  2 x 8192 bf16 D 128 16/4 heads: 1 part 3.19 ms, 4 parts 1.32 + 0.03;
+// 1 x 2048: 436 us (dQ included), 175.  The parts' fp32 sums cost 16 bytes an element and part, so short walks only fill the units once
+// (16 x 64 D 128 32/8: 4 parts 65 us, 1 part 44).
+int head_parts(long T, long n_seqs, int Hq, int Hk, int dtype) {
+  const int g = Hq / Hk;
+  const bool split = use_split(tile_bound<128>(T, n_seqs) * Hq, dtype, T, n_seqs);
+  const long units = (split ? tile_bound<32>(T, n_seqs) : tile_bound<128>(T, n_seqs)) * Hk, want = T >= 512 * n_seqs ? 1024 : 256;
+  for (int p = 1; p < g; ++p)
+    if (g % p == 0 && units * p >= want) return p;
+  return g;
+}
+
 template <int DT, int DP, bool PAD>
 int launch(BwdArgs a, hipStream_t st) {
   typedef Ring<Op<DT>, DP> R;
+  typedef DkvRing<DT, DP> R2;
   typedef Tiles<Op<DT>, DP> S;
   static uint64_t attr[4] = {0, 0, 0, 0};
   const int wide = (int)tile_bound<128>(a.T, a.n_seqs), narrow = (int)tile_bound<32>(a.T, a.n_seqs);
-  if (MVF_SPLIT_RULE((long)wide * a.Hq)) {
+  if (use_split((long)wide * a.Hq, DT, a.T, a.n_seqs)) {
     const size_t lds = std::max(4 * S::NB * S::BUF, JOIN_BYTES<DP>);
     if (int rc = mvf_ensure_lds(reinterpret_cast<const void*>(packed_attn_dq_split_kernel<DT, DP, PAD>), lds, attr[0])) return rc;
     a.ntiles = narrow;
-    hipLaunchKernelGGL((packed_attn_dq_split_kernel<DT, DP, PAD>), dim3(xcd_grid((long)narrow * a.Hq)), dim3(256), lds, st, a);
+    hipLaunchKernelGGL((packed_attn_dq_split_kernel<DT, DP, PAD>), dim3(xcd_grid(a.Hq, narrow)), dim3(256), lds, st, a);
   } else {
     const size_t lds = R::NB * R::BUF;
     if (int rc = mvf_ensure_lds(reinterpret_cast<const void*>(packed_attn_dq_kernel<DT, DP, PAD>), lds, attr[1])) return rc;
     a.ntiles = wide;
-    hipLaunchKernelGGL((packed_attn_dq_kernel<DT, DP, PAD>), dim3(xcd_grid((long)wide * a.Hq)), dim3(256), lds, st, a);
+    hipLaunchKernelGGL((packed_attn_dq_kernel<DT, DP, PAD>), dim3(xcd_grid(a.Hq, wide)), dim3(256), lds, st, a);
   }
   MVF_LAUNCH_CHECK();
-  if (MVF_SPLIT_RULE((long)wide * a.Hk)) {
+  if (use_split((long)wide * a.Hq, DT, a.T, a.n_seqs)) {
     const size_t lds = std::max(4 * S::NB * (S::BUF + (planes(DT) * 32 + 63) / 64 * 256), JOIN_BYTES<DP>);
     if (int rc = mvf_ensure_lds(reinterpret_cast<const void*>(packed_attn_dkv_split_kernel<DT, DP, PAD>), lds, attr[2])) return rc;
     a.ntiles = narrow;
-    hipLaunchKernelGGL((packed_attn_dkv_split_kernel<DT, DP, PAD>), dim3(xcd_grid((long)narrow * a.Hk)), dim3(256), lds, st, a);
+    hipLaunchKernelGGL((packed_attn_dkv_split_kernel<DT, DP, PAD>), dim3(xcd_grid((long)a.Hk * a.parts, narrow)), dim3(256), lds, st, a);
   } else {
-    const size_t lds = R::NB * (R::BUF + (planes(DT) * R::KB + 63) / 64 * 256);
+    const size_t lds = R2::NB * (R2::BUF + (planes(DT) * R2::KB + 63) / 64 * 256) + (V_IN_LDS<DT, DP> ? 128 * Img<Op<DT>, DP>::RB : 0);
     if (int rc = mvf_ensure_lds(reinterpret_cast<const void*>(packed_attn_dkv_kernel<DT, DP, PAD>), lds, attr[3])) return rc;
     a.ntiles = wide;
-    hipLaunchKernelGGL((packed_attn_dkv_kernel<DT, DP, PAD>), dim3(xcd_grid((long)wide * a.Hk)), dim3(256), lds, st, a);
+    hipLaunchKernelGGL((packed_attn_dkv_kernel<DT, DP, PAD>), dim3(xcd_grid((long)a.Hk * a.parts, wide)), dim3(256), lds, st, a);
   }
   MVF_LAUNCH_CHECK();
+  if (a.parts > 1) {
+    const size_t n = (size_t)a.T * a.Hk * a.D;
+    hipLaunchKernelGGL((packed_attn_sum_kernel<DT>), dim3((unsigned)((2 * n / 4 + 255) / 256)), dim3(256), 0, st, a.part, a.parts, n, a.dk, a.dv);
+    MVF_LAUNCH_CHECK();
+  }
   return MVF_OK;
 }
 template <int DT, int DP>
@@ -496,12 +567,19 @@ int launch_d(const BwdArgs& a, hipStream_t st) {
 
 }  // namespace
 
+extern "C" size_t mvf_packed_attn_bwd_workspace_bytes(int dtype, int T, int n_seqs, int Hq, int Hk, int D) {
+  if (T <= 0 || n_seqs <= 0 || Hk <= 0 || Hq <= 0 || Hq % Hk != 0 || D <= 0) return 0;
+  const size_t delta = ((size_t)Hq * T + 3) / 4 * 4;
+  const int parts = head_parts(T, n_seqs, Hq, Hk, dtype);
+  return (delta + (parts > 1 ? 2 * parts * (size_t)T * Hk * D : 0)) * sizeof(float);
+}
+
 extern "C" int mvf_packed_attn_bwd(int dtype, const void* q, long ldq, long hsq, const void* k, long ldk, long hsk, const void* v,
                                    long ldv, long hsv, const int* cu_seqlens, int n_seqs, const void* out, const void* d_out,
-                                   const float* stat, float* delta, void* dq, void* dk, void* dv, int T, int Hq, int Hk, int D, int frame,
-                                   float scale, hipStream_t st) {
+                                   const float* stat, void* workspace, size_t ws_bytes, void* dq, void* dk, void* dv, int T, int Hq, int Hk,
+                                   int D, int frame, float scale, hipStream_t st) {
   MVF_CHECK_ARG(dtype == MVF_F32 || dtype == MVF_BF16 || dtype == MVF_F16);
-  MVF_CHECK_ARG(q && k && v && cu_seqlens && out && d_out && stat && delta && dq && dk && dv);
+  MVF_CHECK_ARG(q && k && v && cu_seqlens && out && d_out && stat && workspace && dq && dk && dv);
   MVF_CHECK_ARG(T > 0 && n_seqs > 0 && Hk > 0 && Hq > 0 && Hq % Hk == 0 && frame >= 0);
   MVF_CHECK_ARG(scale > 0.f && scale < 1e30f && T < (1 << 30) && tile_bound<32>(T, n_seqs) * Hq < (1l << 30));
   if (D <= 0 || D > 128 || D % 8 != 0) return MVF_ERR_UNSUPPORTED;
@@ -509,8 +587,12 @@ extern "C" int mvf_packed_attn_bwd(int dtype, const void* q, long ldq, long hsq,
   const long s[6] = {ldq * sz, hsq * sz, ldk * sz, hsk * sz, ldv * sz, hsv * sz};
   for (long x : s) MVF_CHECK_ARG(x > 0 && x % 16 == 0);
   MVF_CHECK_ARG((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out | (uintptr_t)d_out | (uintptr_t)dq | (uintptr_t)dk |
-                  (uintptr_t)dv) & 15) == 0);
+                  (uintptr_t)dv | (uintptr_t)workspace) & 15) == 0);
+  MVF_CHECK_ARG(ws_bytes >= mvf_packed_attn_bwd_workspace_bytes(dtype, T, n_seqs, Hq, Hk, D));
+  float* delta = (float*)workspace;
+  const int parts = head_parts(T, n_seqs, Hq, Hk, dtype);
+  MVF_CHECK_ARG(tile_bound<32>(T, n_seqs) * Hk * parts < (1l << 30) && (size_t)T * Hk * D / 512 < (1ul << 31));
   BwdArgs a = {(const char*)q, (const char*)k, (const char*)v, s[0], s[1], s[2], s[3], s[4], s[5], cu_seqlens, n_seqs, (const char*)out,
-               (const char*)d_out, stat, delta, (char*)dq, (char*)dk, (char*)dv, T, Hq, Hk, D, frame, 0, scale * LOG2E, scale};
+               (const char*)d_out, stat, delta, delta + ((size_t)Hq * T + 3) / 4 * 4, parts, (char*)dq, (char*)dk, (char*)dv, T, Hq, Hk, D, frame, 0, scale * LOG2E, scale};
   return dtype == MVF_F32 ? launch_d<MVF_F32>(a, st) : dtype == MVF_BF16 ? launch_d<MVF_BF16>(a, st) : launch_d<MVF_F16>(a, st);
 }

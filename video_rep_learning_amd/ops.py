@@ -2394,9 +2394,11 @@ class _PackedAttention(torch.autograd.Function):
             d_out = d_out.clone()
         dq, dk, dv = (torch.empty(x.shape, device=x.device, dtype=x.dtype) for x in (q, k, v))
         if T:
-            delta = torch.empty(Hq, T, device=q.device, dtype=torch.float32)
-            _launch('mvf_packed_attn_bwd', q, _SEQ_DT[q.dtype], q.data_ptr(), *q.stride()[:2], k.data_ptr(), *k.stride()[:2], v.data_ptr(),
-                    *v.stride()[:2], cu.data_ptr(), cu.shape[0] - 1, out.data_ptr(), d_out.data_ptr(), stat.data_ptr(), delta.data_ptr(),
+            code, n = _SEQ_DT[q.dtype], cu.shape[0] - 1
+            need = _lib.load().mvf_packed_attn_bwd_workspace_bytes(code, T, n, Hq, k.shape[1], D)
+            ws = torch.empty(need, device=q.device, dtype=torch.uint8)
+            _launch('mvf_packed_attn_bwd', q, code, q.data_ptr(), *q.stride()[:2], k.data_ptr(), *k.stride()[:2], v.data_ptr(),
+                    *v.stride()[:2], cu.data_ptr(), n, out.data_ptr(), d_out.data_ptr(), stat.data_ptr(), ws.data_ptr(), need,
                     dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), T, Hq, k.shape[1], D, frame, scale)
         return dq, dk, dv, None, None, None
 
