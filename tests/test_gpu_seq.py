@@ -136,6 +136,8 @@ LENGTHS = {
     'edges': [63, 64, 65, 127, 129],
     'long': [300, 1, 517],
     'many': [3] * 70,
+    'swarm': [2, 0, 1, 3] * 150,                        # more than the sequences that get tiles of their own
+    'far': [1100, 3],                                   # few rows that walk far: eight waves share a tile's keys
     'wide': [300, 1, 0, 33, 129, 64, 517, 31] * 4,      # with 16 heads: enough rows for the form whose workgroups own 128
 }
 PACKED = [  # lengths, hq, hk, d, frame
@@ -144,6 +146,8 @@ PACKED = [  # lengths, hq, hk, d, frame
     ('edges', 2, 2, 64, 1), ('edges', 6, 2, 128, 1), ('edges', 2, 1, 80, 7),
     ('long', 2, 2, 32, 6), ('long', 3, 1, 64, 0), ('long', 2, 2, 128, 100000),
     ('many', 2, 2, 16, 1), ('many', 5, 5, 48, 2),
+    ('swarm', 2, 1, 32, 1), ('swarm', 2, 2, 64, 0),
+    ('far', 2, 1, 64, 1), ('far', 1, 1, 32, 0), ('far', 2, 2, 24, 5), ('far', 4, 1, 128, 1),
     ('wide', 16, 16, 32, 1), ('wide', 16, 16, 64, 0), ('wide', 32, 16, 80, 3), ('wide', 16, 16, 128, 1), ('wide', 18, 9, 24, 0),
 ]
 
@@ -221,7 +225,8 @@ def test_packed_attention_hides_what_a_row_does_not_see(dtype, bad):
 
 
 @pytest.mark.parametrize('dtype', DTYPES, ids=IDS)
-@pytest.mark.parametrize('lengths,hq,hk', [([45, 30, 90], 4, 2), ([450, 35] + [100] * 37, 16, 16)], ids=['split', 'wide'])
+@pytest.mark.parametrize('lengths,hq,hk', [([45, 30, 90], 4, 2), ([450, 35] + [100] * 37, 16, 16), ([1600, 35], 2, 1)],
+                         ids=['split', 'wide', 'far'])
 def test_packed_attention_gradients_hide_other_sequences(dtype, lengths, hq, hk):
     """A sequence whose inputs or output gradients are not finite leaves its neighbours' gradients as they are."""
     c, d = cum(lengths), 64

@@ -312,6 +312,50 @@ struct Tiles {
   }
 };
 
+// ... of consecutive rows: the pieces' addresses walk along, 32 * NW rows a step
+template <class O, int DP, int NW, class S>
+struct TileWalk {
+  typedef Img<O, DP> I;
+  static constexpr int H = S::NP / 2;
+  const char *pa[H], *pb[H];
+  long lda, ldb;
+  __device__ __forceinline__ void start(const char* a, long lda_, const char* b, long ldb_, int row, int lane) {
+    lda = lda_;
+    ldb = ldb_;
+#pragma unroll
+    for (int j = 0; j < H; ++j) {
+      const int idx = j * 64 + lane, r = idx / I::C, ch = (idx % I::C) ^ I::swz(r);
+      pa[j] = a + (row + r) * lda + ch * 16;
+      pb[j] = b + (row + r) * ldb + ch * 16;
+    }
+  }
+  // the tile of rows [row, row + 32) of the rows before `end` (a row behind repeats the last), and on to the wave's next tile
+  template <bool PAD>
+  __device__ __forceinline__ void issue(int row, int end, int D, int lane, uint32_t lds) {
+    const bool last = row + 32 > end;
+    lane = launder(lane);
+#pragma unroll
+    for (int j = 0; j < H; ++j) {
+      const char *qa = pa[j], *qb = pb[j];
+      if (last) {
+        const int over = row + (j * 64 + lane) / I::C - (end - 1);
+        if (over > 0) { qa -= over * lda; qb -= over * ldb; }
+      }
+      bool on = true;
+      if constexpr (PAD) {
+        const int idx = j * 64 + lane;
+        on = ((idx % I::C) ^ I::swz(idx / I::C)) * 16 < D * O::SZ;
+      }
+      if (on) {
+        dma16(qa, lds + j * 1024);
+        dma16(qb, lds + S::IMG + j * 1024);
+      }
+      pa[j] += 32 * NW * lda;
+      pb[j] += 32 * NW * ldb;
+    }
+  }
+};
+
 __device__ __forceinline__ void clear_lds(char* p, int bytes) {
   for (int i = threadIdx.x * 16; i < bytes; i += blockDim.x * 16) *reinterpret_cast<uint4*>(p + i) = make_uint4(0, 0, 0, 0);
   __syncthreads();
@@ -348,7 +392,14 @@ static inline bool use_split(long wide, int dtype, long T, long n_seqs) {
 #endif
   return wide < 256 || (wide < 512 && T >= (dtype == MVF_F32 ? 1024 : 4096) * n_seqs);
 }
-static inline unsigned xcd_grid(long units) { return (unsigned)((units + 7) / 8 * 8); }
+// Waves of a split forward's workgroup: eight, a tile each at a time, for walks of 512 and more where two such workgroups fit a unit's LDS
+// (1 x 4096 bf16 D 64 12 heads: 59 us, with four 73; 2 x 1440 fp32 D 32 the same), else four with two tiles each.  The backward, which
+// holds more registers, keeps four (1 x 4096: 173 us, with eight 205; 2 x 1440: 108, 114).
+template <class O, int DP>
+constexpr int SPLIT_WAVES = DP * O::SZ <= 128 ? 8 : 4;
+template <class O, int DP, int NW>
+using SplitTiles = Tiles<O, DP, ((NW == 8 && DP * O::SZ > 64) || DP * O::SZ > 256) ? 1 : 2>;
+static inline bool long_walks(long T, long n_seqs) { return T >= 512 * n_seqs; }
 
 // ---------------------------------------------------------------------------------------------- which rows meet
 struct Span { int lo, hi; };

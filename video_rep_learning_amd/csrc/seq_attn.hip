@@ -185,12 +185,12 @@ __global__ __launch_bounds__(256, DT == MVF_F32 && DP > 64 ? 1 : 2) void packed_
     }
 }
 
-template <int DT, int DP, bool PAD>
-__global__ __launch_bounds__(256, 1) void packed_attn_fwd_split_kernel(FwdArgs a) {
+template <int DT, int DP, bool PAD, int NW>
+__global__ __launch_bounds__(64 * NW, NW / 4) void packed_attn_fwd_split_kernel(FwdArgs a) {
   typedef Op<DT> O;
-  typedef Tiles<O, DP> S;
+  typedef SplitTiles<O, DP, NW> S;
   extern __shared__ __attribute__((aligned(256))) char smem[];
-  __shared__ float s_m[4][32], s_l[4][32];
+  __shared__ float s_m[NW][32], s_l[NW][32];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Unit u = xcd_unit(a.Hq, a.ntiles);
   if (u.head < 0) return;
@@ -202,31 +202,29 @@ __global__ __launch_bounds__(256, 1) void packed_attn_fwd_split_kernel(FwdArgs a
   f.start(a, head, row, lane);                 // (a row of no sequence may hold anything: it stays in its own lanes and is not stored)
   f.own = keys_of(sequence_of(own, a.cu, a.n_seqs, a.T, row), a.frame, row);
   const WaveSpan ws = wave_span(f.own);
-  if constexpr (PAD) clear_lds(smem, 4 * S::NB * S::BUF);
+  if constexpr (PAD) clear_lds(smem, NW * S::NB * S::BUF);
   const int g = a.Hq / a.Hk;
 #pragma unroll
   for (int ks = 0; ks < DP / 16; ++ks) asm volatile("" : "+v"(f.qf[ks]));
   const char *kb = a.k + head / g * a.hsk, *vb = a.v + head / g * a.hsv;
   const uint32_t lds = lds_addr(smem) + wave * S::NB * S::BUF;
+  TileWalk<O, DP, NW, S> walk;
+  walk.start(kb, a.ldk, vb, a.ldv, ws.any.lo + wave * 32, lane);
   auto issue = [&](int key0, int buf) __attribute__((always_inline)) {
-    S::template issue<PAD>(kb, vb, [&](int i, long& oa, long& ob) {
-      const long r = min(key0 + i, ws.any.hi - 1);
-      oa = r * a.ldk;
-      ob = r * a.ldv;
-    }, a.D, lane, lds + buf * S::BUF);
+    walk.template issue<PAD>(key0, ws.any.hi, a.D, lane, lds + buf * S::BUF);
   };
   int key0 = ws.any.lo + wave * 32, buf = 0;
   if (key0 < ws.any.hi) issue(key0, 0);
-  for (; key0 < ws.any.hi; key0 += 128) {
-    const bool more = key0 + 128 < ws.any.hi;
-    if (S::NB == 2 && more) { issue(key0 + 128, buf ^ 1); wait_dma<S::NP>(); }
+  for (; key0 < ws.any.hi; key0 += 32 * NW) {
+    const bool more = key0 + 32 * NW < ws.any.hi;
+    if (S::NB == 2 && more) { issue(key0 + 32 * NW, buf ^ 1); wait_dma<S::NP>(); }
     else wait_dma<0>();
     f.any_tile(ws, lds + buf * S::BUF, lds + buf * S::BUF + S::IMG, key0);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     if (S::NB == 2) buf ^= 1;
-    else if (more) issue(key0 + 128, 0);
+    else if (more) issue(key0 + 32 * NW, 0);
   }
-  if (f.bad) f.slow(a, kb, vb, ws.any.lo + wave * 32, 128, ws.any.hi);
+  if (f.bad) f.slow(a, kb, vb, ws.any.lo + wave * 32, 32 * NW, ws.any.hi);
   if (f.own.hi == 0) {           // rows of no sequence rode along in unmasked tiles
     f.st = RowMax();
 #pragma unroll
@@ -234,7 +232,7 @@ __global__ __launch_bounds__(256, 1) void packed_attn_fwd_split_kernel(FwdArgs a
   }
   __syncthreads();
   const bool stat = a.stat != nullptr;
-  join_waves<DP>(reinterpret_cast<float*>(smem), s_m, s_l, f.o, f.st, own.end - row0, a.D, wave, lane,
+  join_waves<DP, NW>(reinterpret_cast<float*>(smem), s_m, s_l, f.o, f.st, own.end - row0, a.D, wave, lane,
                  [&](int i, int d, const f32x4_t& acc, float mx, float l) {
     const bool some = l != 0.f;
     const float inv = some ? 1.0f / l : 0.f;
@@ -244,16 +242,22 @@ __global__ __launch_bounds__(256, 1) void packed_attn_fwd_split_kernel(FwdArgs a
   });
 }
 
+template <int DT, int DP, bool PAD, int NW>
+int launch_split(FwdArgs a, hipStream_t st) {
+  typedef SplitTiles<Op<DT>, DP, NW> S;
+  const size_t lds = std::max(NW * S::NB * S::BUF, (JOIN_BYTES<DP, NW>));
+  static uint64_t attr = 0;
+  if (int rc = mvf_ensure_lds(reinterpret_cast<const void*>(packed_attn_fwd_split_kernel<DT, DP, PAD, NW>), lds, attr)) return rc;
+  a.ntiles = (int)tile_bound<32>(a.T, a.n_seqs);
+  hipLaunchKernelGGL((packed_attn_fwd_split_kernel<DT, DP, PAD, NW>), dim3(xcd_grid(a.Hq, a.ntiles)), dim3(64 * NW), lds, st, a);
+  return MVF_OK;
+}
 template <int DT, int DP, bool PAD>
 int launch(FwdArgs a, hipStream_t st) {
   typedef Ring<Op<DT>, DP> R;
-  typedef Tiles<Op<DT>, DP> S;
   if (use_split(tile_bound<128>(a.T, a.n_seqs) * a.Hq, DT, a.T, a.n_seqs)) {
-    const size_t lds = std::max(4 * S::NB * S::BUF, JOIN_BYTES<DP>);
-    static uint64_t attr = 0;
-    if (int rc = mvf_ensure_lds(reinterpret_cast<const void*>(packed_attn_fwd_split_kernel<DT, DP, PAD>), lds, attr)) return rc;
-    a.ntiles = (int)tile_bound<32>(a.T, a.n_seqs);
-    hipLaunchKernelGGL((packed_attn_fwd_split_kernel<DT, DP, PAD>), dim3(xcd_grid(a.Hq, a.ntiles)), dim3(256), lds, st, a);
+    constexpr int NW8 = SPLIT_WAVES<Op<DT>, DP>;
+    if (int rc = long_walks(a.T, a.n_seqs) ? launch_split<DT, DP, PAD, NW8>(a, st) : launch_split<DT, DP, PAD, 4>(a, st)) return rc;
   } else {
     const size_t lds = R::NB * R::BUF;
     static uint64_t attr = 0;

@@ -56,7 +56,7 @@ __device__ __forceinline__ void store_rows(char* base, size_t row_elems, const f
 // the fp32 format of the partial sums
 typedef Op<MVF_F32> Part;
 
-// The four waves' sums of the same 32 rows, added in order: wave 0 + 1 + 2 + 3, out as [row][D].  All threads; barriers inside.
+// The waves' sums of the same 32 rows, added in order, out as [row][D].  All threads; barriers inside.
 template <class O, int DP>
 __device__ __forceinline__ void store_joined(float* so, const f32x16_t (&x)[DP / 32], char* base, int row0, int rows, long stride, float f,
                                              int D, int wave, int lane) {
@@ -208,7 +208,7 @@ __global__ __launch_bounds__(256, DT == MVF_F32 && DP > 32 ? 1 : 2) void packed_
 template <int DT, int DP, bool PAD>
 __global__ __launch_bounds__(256, 1) void packed_attn_dq_split_kernel(BwdArgs a) {
   typedef Op<DT> O;
-  typedef Tiles<O, DP> S;
+  typedef SplitTiles<O, DP, 4> S;
   extern __shared__ __attribute__((aligned(256))) char smem[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Unit u = xcd_unit(a.Hq, a.ntiles);
@@ -225,12 +225,10 @@ __global__ __launch_bounds__(256, 1) void packed_attn_dq_split_kernel(BwdArgs a)
   const int g = a.Hq / a.Hk;
   const char *kb = a.k + head / g * a.hsk, *vb = a.v + head / g * a.hsv;
   const uint32_t lds = lds_addr(smem) + wave * S::NB * S::BUF;
+  TileWalk<O, DP, 4, S> walk;
+  walk.start(kb, a.ldk, vb, a.ldv, ws.any.lo + wave * 32, lane);
   auto issue = [&](int key0, int buf) __attribute__((always_inline)) {
-    S::template issue<PAD>(kb, vb, [&](int i, long& oa, long& ob) {
-      const long r = min(key0 + i, ws.any.hi - 1);
-      oa = r * a.ldk;
-      ob = r * a.ldv;
-    }, a.D, lane, lds + buf * S::BUF);
+    walk.template issue<PAD>(key0, ws.any.hi, a.D, lane, lds + buf * S::BUF);
   };
   int key0 = ws.any.lo + wave * 32, buf = 0;
   if (key0 < ws.any.hi) issue(key0, 0);
@@ -439,7 +437,7 @@ __global__ __launch_bounds__(256, DT == MVF_F32 && DP > 32 ? 1 : 2) void packed_
 template <int DT, int DP, bool PAD>
 __global__ __launch_bounds__(256, 1) void packed_attn_dkv_split_kernel(BwdArgs a) {
   typedef Op<DT> O;
-  typedef Tiles<O, DP> S;
+  typedef SplitTiles<O, DP, 4> S;
   constexpr int NF = planes(DT) * 32, NSP = (NF + 63) / 64, SB = NSP * 256;
   extern __shared__ __attribute__((aligned(256))) char smem[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -456,20 +454,21 @@ __global__ __launch_bounds__(256, 1) void packed_attn_dkv_split_kernel(BwdArgs a
   if constexpr (PAD) clear_lds(smem, 4 * S::NB * S::BUF);
   const int g = a.Hq / a.Hk / a.parts, h0 = kh * (a.Hq / a.Hk) + part * g, nt = (ws.any.hi - ws.any.lo + 31) >> 5, total = nt * g;
   const uint32_t lds = lds_addr(smem) + wave * S::NB * S::BUF, stat0 = lds_addr(smem) + 4 * S::NB * S::BUF + wave * S::NB * SB;
-  auto issue = [&](int it, int buf) __attribute__((always_inline)) {
-    const int h = h0 + it / nt, q0 = ws.any.lo + it % nt * 32;
-    const long ldo = (long)a.Hq * a.D * O::SZ;
-    S::template issue<PAD>(a.q + h * a.hsq, a.d_out + (size_t)h * a.D * O::SZ, [&](int i, long& oa, long& ob) {
-      const long r = min(q0 + i, ws.any.hi - 1);
-      oa = r * a.ldq;
-      ob = r * ldo;
-    }, a.D, lane, lds + buf * S::BUF);
+  TileWalk<O, DP, 4, S> walk;
+  int ih = -1, it = wave;                      // the next tile: it of head ih's, wave by wave through (head, tile)
+  auto issue = [&](int n, int buf) __attribute__((always_inline)) {
+    const int h = h0 + n / nt, q0 = ws.any.lo + n % nt * 32;
+    if (h != ih) {
+      ih = h;
+      walk.start(a.q + h * a.hsq, a.ldq, a.d_out + (size_t)h * a.D * O::SZ, (long)a.Hq * a.D * O::SZ, q0, lane);
+    }
+    walk.template issue<PAD>(q0, ws.any.hi, a.D, lane, lds + buf * S::BUF);
 #pragma unroll
     for (int j = 0; j < NSP; ++j) dma4(stat_at(a, h, q0, min(j * 64 + lane, NF - 1), 32), stat0 + buf * SB + j * 256);
   };
   int buf = 0;
-  if (wave < total) issue(wave, 0);
-  for (int it = wave; it < total; it += 4) {
+  if (it < total) issue(it, 0);
+  for (; it < total; it += 4) {
     const bool more = it + 4 < total;
     if (S::NB == 2 && more) { issue(it + 4, buf ^ 1); wait_dma<S::NP + NSP>(); }
     else wait_dma<0>();
@@ -524,29 +523,30 @@ template <int DT, int DP, bool PAD>
 int launch(BwdArgs a, hipStream_t st) {
   typedef Ring<Op<DT>, DP> R;
   typedef DkvRing<DT, DP> R2;
-  typedef Tiles<Op<DT>, DP> S;
+  typedef SplitTiles<Op<DT>, DP, 4> S;
   static uint64_t attr[4] = {0, 0, 0, 0};
-  const int wide = (int)tile_bound<128>(a.T, a.n_seqs), narrow = (int)tile_bound<32>(a.T, a.n_seqs);
-  if (use_split((long)wide * a.Hq, DT, a.T, a.n_seqs)) {
-    const size_t lds = std::max(4 * S::NB * S::BUF, JOIN_BYTES<DP>);
-    if (int rc = mvf_ensure_lds(reinterpret_cast<const void*>(packed_attn_dq_split_kernel<DT, DP, PAD>), lds, attr[0])) return rc;
-    a.ntiles = narrow;
-    hipLaunchKernelGGL((packed_attn_dq_split_kernel<DT, DP, PAD>), dim3(xcd_grid(a.Hq, narrow)), dim3(256), lds, st, a);
+  const int wide = (int)tile_bound<128>(a.T, a.n_seqs);
+  const bool split = use_split((long)wide * a.Hq, DT, a.T, a.n_seqs);
+  if (split) {
+    const size_t lds = std::max(4 * S::NB * S::BUF, (JOIN_BYTES<DP>));
+    if (int rc = mvf_ensure_lds(reinterpret_cast<const void*>(packed_attn_dq_split_kernel<DT, DP, PAD>), lds, attr[2])) return rc;
+    a.ntiles = (int)tile_bound<32>(a.T, a.n_seqs);
+    hipLaunchKernelGGL((packed_attn_dq_split_kernel<DT, DP, PAD>), dim3(xcd_grid(a.Hq, a.ntiles)), dim3(256), lds, st, a);
   } else {
     const size_t lds = R::NB * R::BUF;
-    if (int rc = mvf_ensure_lds(reinterpret_cast<const void*>(packed_attn_dq_kernel<DT, DP, PAD>), lds, attr[1])) return rc;
+    if (int rc = mvf_ensure_lds(reinterpret_cast<const void*>(packed_attn_dq_kernel<DT, DP, PAD>), lds, attr[0])) return rc;
     a.ntiles = wide;
     hipLaunchKernelGGL((packed_attn_dq_kernel<DT, DP, PAD>), dim3(xcd_grid(a.Hq, wide)), dim3(256), lds, st, a);
   }
   MVF_LAUNCH_CHECK();
-  if (use_split((long)wide * a.Hq, DT, a.T, a.n_seqs)) {
-    const size_t lds = std::max(4 * S::NB * (S::BUF + (planes(DT) * 32 + 63) / 64 * 256), JOIN_BYTES<DP>);
-    if (int rc = mvf_ensure_lds(reinterpret_cast<const void*>(packed_attn_dkv_split_kernel<DT, DP, PAD>), lds, attr[2])) return rc;
-    a.ntiles = narrow;
-    hipLaunchKernelGGL((packed_attn_dkv_split_kernel<DT, DP, PAD>), dim3(xcd_grid((long)a.Hk * a.parts, narrow)), dim3(256), lds, st, a);
+  if (split) {
+    const size_t lds = std::max(4 * S::NB * (S::BUF + (planes(DT) * 32 + 63) / 64 * 256), (JOIN_BYTES<DP>));
+    if (int rc = mvf_ensure_lds(reinterpret_cast<const void*>(packed_attn_dkv_split_kernel<DT, DP, PAD>), lds, attr[3])) return rc;
+    a.ntiles = (int)tile_bound<32>(a.T, a.n_seqs);
+    hipLaunchKernelGGL((packed_attn_dkv_split_kernel<DT, DP, PAD>), dim3(xcd_grid((long)a.Hk * a.parts, a.ntiles)), dim3(256), lds, st, a);
   } else {
     const size_t lds = R2::NB * (R2::BUF + (planes(DT) * R2::KB + 63) / 64 * 256) + (V_IN_LDS<DT, DP> ? 128 * Img<Op<DT>, DP>::RB : 0);
-    if (int rc = mvf_ensure_lds(reinterpret_cast<const void*>(packed_attn_dkv_kernel<DT, DP, PAD>), lds, attr[3])) return rc;
+    if (int rc = mvf_ensure_lds(reinterpret_cast<const void*>(packed_attn_dkv_kernel<DT, DP, PAD>), lds, attr[1])) return rc;
     a.ntiles = wide;
     hipLaunchKernelGGL((packed_attn_dkv_kernel<DT, DP, PAD>), dim3(xcd_grid((long)a.Hk * a.parts, wide)), dim3(256), lds, st, a);
   }
