@@ -338,6 +338,9 @@ PAGED = [  # lengths, new, page, hq, hk, d, frame
     ([90, 4], 6, 16, 16, 2, 96, 6),
     ([4, 200], 5, 16, 40, 2, 80, 1),            # 100 rows of one key head: several tiles
     ([3000], 1, 128, 2, 2, 64, 1),
+    ([0] * 66 + [2500] + [0] * 3 + [1, 40, 900] * 20 + [0] * 9, 1, 16, 4, 2, 32, 1),           # 139 streams, many of them empty
+    ([700, 0, 1400] + [130, 5] * 31, 2, 24, 8, 4, 40, 0),                                       # 65 streams, four key heads each
+    ([4100, 300], 9, 64, 8, 2, 64, 1),          # 36 rows of one key head, long
 ]
 
 
