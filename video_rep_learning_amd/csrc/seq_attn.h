@@ -251,25 +251,25 @@ __device__ __forceinline__ void wait_dma() {           // all but the wave's las
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
 }
 
-// A workgroup of four waves streams blocks of KB rows of two matrices (a and b) through a ring of three buffers: waves 0 and 1 fetch a's
-// pieces, waves 2 and 3 b's, block n + 2 is asked for right behind the one barrier of block n (with two buffers: block n + 1).  A row behind the last one repeats it;
-// chunks behind the row's D elements are not fetched (the caller cleared the buffers once).
-template <class O, int DP, int NBUF = 3>
+// A workgroup of NW waves streams blocks of KB rows of two matrices (a and b) through a ring of three buffers: its first half fetches a's
+// pieces, its second half b's, block n + 2 is asked for right behind the one barrier of block n (with two buffers: block n + 1).  A row
+// behind the last one repeats it; chunks behind the row's D elements are not fetched (the caller cleared the buffers once).
+template <class O, int DP, int NBUF = 3, int NW = 4>
 struct Ring {
   typedef Img<O, DP> I;
-  static constexpr int KB = I::RB <= 64 ? 128 : I::RB <= 128 ? 64 : 32;
-  static constexpr int IMG = KB * I::RB, BUF = 2 * IMG, NB = NBUF, PP = IMG / 2048;     // PP: pieces per wave and block
+  static constexpr int KB = I::RB <= 64 ? 128 : I::RB <= 128 || NW == 8 ? 64 : 32;
+  static constexpr int IMG = KB * I::RB, BUF = 2 * IMG, NB = NBUF, HW = NW / 2, PP = IMG / (1024 * HW);     // PP: pieces per wave and block
   const char* p[PP];
   long ld;
   uint32_t on, lds;
   __device__ __forceinline__ void start(const char* a, long lda, const char* b, long ldb, int row, int D, int wave, int lane, uint32_t lds0) {
-    ld = wave < 2 ? lda : ldb;
-    const char* base = (wave < 2 ? a : b) + (long)row * ld;
+    ld = wave < HW ? lda : ldb;
+    const char* base = (wave < HW ? a : b) + (long)row * ld;
     lds = lds0 + wave * PP * 1024;
     on = 0;
 #pragma unroll
     for (int j = 0; j < PP; ++j) {
-      const int idx = ((wave & 1) * PP + j) * 64 + lane, r = idx / I::C, ch = (idx % I::C) ^ I::swz(r);
+      const int idx = (wave % HW * PP + j) * 64 + lane, r = idx / I::C, ch = (idx % I::C) ^ I::swz(r);
       p[j] = base + r * ld + ch * 16;
       on |= (uint32_t)(ch * 16 < D * O::SZ) << j;
     }
@@ -283,7 +283,7 @@ struct Ring {
     for (int j = 0; j < PP; ++j) {
       const char* q = p[j];
       if (last) {
-        const int over = row + (((wave & 1) * PP + j) * 64 + lane) / I::C - (end - 1);
+        const int over = row + ((wave % HW * PP + j) * 64 + lane) / I::C - (end - 1);
         if (over > 0) q -= over * ld;
       }
       if (!PAD || ((on >> j) & 1)) dma16(q, lds + buf * BUF + j * 1024);
@@ -401,6 +401,36 @@ template <class O, int DP, int NW>
 using SplitTiles = Tiles<O, DP, ((NW == 8 && DP * O::SZ > 64) || DP * O::SZ > 256) ? 1 : 2>;
 static inline bool long_walks(long T, long n_seqs) { return T >= 512 * n_seqs; }
 
+// The wide form with eight waves (H = 2): two for each 32 rows, which take the tiles of 64-row blocks in turn and join their sums in LDS.  A walk
+// is half as long and a block half as many barriers, for an unchanged amount of work: it pays where few, long and unequal walks fill the
+// compute units once, at rows of 256 bytes.  Measured, us, forward / backward with one and two waves a row tile, causal: 1 x 2048 bf16 D 128
+// 16 heads on 4: 60 / 195, 45 / 153; 1 x 4096: 117 / 380, 94 / 320; 2 x 2048: 63 / 211, 55 / 195; 4 x 2048 fp32 D 64 8 heads: 210 / 633,
+// 158 / 529; but 1 x 6000, 800 workgroups: forward 193, 191; not causal, 4 x 2048 8 heads D 128: 82, 90; shorter rows, 2 x 4096 D 96 12
+// heads: 108, 115.
+template <class O, int DP>
+constexpr bool PAIRS = DP * O::SZ == 256;
+template <int DP>
+constexpr int HALF = (DP / 8 + 1) * 1024;        // bytes of 32 rows' sums in the accumulators' order, and a float2 for each lane
+template <int DP>
+__device__ __forceinline__ void put_half(char* half, const f32x16_t (&o)[DP / 32]) {
+#pragma unroll
+  for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      *reinterpret_cast<f32x4_t*>(half + (4 * dt + g) * 1024) = (f32x4_t){o[dt][4 * g], o[dt][4 * g + 1], o[dt][4 * g + 2], o[dt][4 * g + 3]};
+}
+template <int DP>
+__device__ __forceinline__ void add_half(const char* half, f32x16_t (&o)[DP / 32]) {
+#pragma unroll
+  for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const f32x4_t x = *reinterpret_cast<const f32x4_t*>(half + (4 * dt + g) * 1024);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[dt][4 * g + j] += x[j];
+    }
+}
+
 // ---------------------------------------------------------------------------------------------- which rows meet
 struct Span { int lo, hi; };
 // Which rows a workgroup owns.  Up to SEQ_TILES sequences every sequence is cut into tiles of its own (a tile across two sequences would walk
@@ -411,6 +441,9 @@ struct OwnTile { int row0, end; Span seq; };      // rows [row0, end); seq: thei
 template <int ROWS>
 static inline long tile_bound(long T, long n) {   // no fewer than the tiles there are
   return n > SEQ_TILES ? (T + ROWS - 1) / ROWS : (T + (ROWS - 1) * (n + 2 < T ? n + 2 : T)) / ROWS;
+}
+static inline bool use_pairs(long T, long n_seqs, long heads, int frame) {
+  return frame > 0 && T >= 1024 * n_seqs && tile_bound<128>(T, n_seqs) * heads <= 640;
 }
 // The t-th tile, found by every wave for itself.  Up to 62 sequences the tiles come in the order of their walks, longest first (causal: the
 // tile's place in its sequence, counted from the end that sees most; else the sequence's length), so that the last workgroups to

@@ -127,26 +127,27 @@ __device__ __forceinline__ void store_stat(const FwdArgs& a, int head, int row, 
   a.stat[(size_t)a.Hq * a.T + at] = some ? 1.0f / l : 0.f;
 }
 
-template <int DT, int DP, bool PAD>
-__global__ __launch_bounds__(256, DT == MVF_F32 && DP > 64 ? 1 : 2) void packed_attn_fwd_kernel(FwdArgs a) {
+// H = 2: eight waves, two for each 32 rows, which take every block's tiles in turn and join their halves at the end
+template <int DT, int DP, bool PAD, int H>
+__global__ __launch_bounds__(256 * H, DT == MVF_F32 && DP > 64 ? H : 2) void packed_attn_fwd_kernel(FwdArgs a) {
   typedef Op<DT> O;
   typedef Img<O, DP> I;
-  typedef Ring<O, DP> R;
+  typedef Ring<O, DP, 3, 4 * H> R;
   extern __shared__ __attribute__((aligned(256))) char smem[];
-  __shared__ int s_span[8];
+  __shared__ int s_span[8 * H];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Unit u = xcd_unit(a.Hq, a.ntiles);
   if (u.head < 0) return;
   const int head = u.head;
   const OwnTile own = find_tile<128>(a.cu, a.n_seqs, a.T, u.tile, a.ntiles, a.frame == 0 ? Walk::ALL : Walk::LATE);
   if (own.row0 >= own.end) return;
-  const int row = own.row0 + wave * 32 + (lane & 31);
+  const int row = own.row0 + (wave & 3) * 32 + (lane & 31);
   Fwd<DT, DP> f;
   f.start(a, head, row, lane);                 // (a row of no sequence may hold anything: it stays in its own lanes and is not stored)
   f.own = keys_of(sequence_of(own, a.cu, a.n_seqs, a.T, row), a.frame, row);
   const WaveSpan ws = wave_span(f.own);
   if constexpr (PAD) clear_lds(smem, R::NB * R::BUF);
-  const Span span = block_span(ws, s_span, lane, wave, 4);
+  const Span span = block_span(ws, s_span, lane, wave, 4 * H);
   const int g = a.Hq / a.Hk;
 #pragma unroll
   for (int ks = 0; ks < DP / 16; ++ks) asm volatile("" : "+v"(f.qf[ks]));      // landed before any DMA is in flight
@@ -163,10 +164,34 @@ __global__ __launch_bounds__(256, DT == MVF_F32 && DP > 64 ? 1 : 2) void packed_
     if (b0 + 2 * R::KB < span.hi) ring.template issue<PAD>(b0 + 2 * R::KB, span.hi, buf == 0 ? 2 : buf - 1, wave, lane);
     const uint32_t ik = lds_addr(smem) + buf * R::BUF;
 #pragma unroll 1
-    for (int t = 0; t < R::KB / 32; ++t) f.any_tile(ws, ik + t * 32 * I::RB, ik + R::IMG + t * 32 * I::RB, b0 + 32 * t);
+    for (int t = wave >> 2; t < R::KB / 32; t += H) f.any_tile(ws, ik + t * 32 * I::RB, ik + R::IMG + t * 32 * I::RB, b0 + 32 * t);
     buf = buf == 2 ? 0 : buf + 1;
   }
-  if (f.bad) f.slow(a, kb, vb, ws.any.lo, 32, ws.any.hi);
+  if (f.bad) f.slow(a, kb, vb, span.lo + 32 * (wave >> 2), 32 * H, ws.any.hi);
+  if constexpr (H == 2) {
+    __syncthreads();
+    char* half = smem + (wave & 3) * HALF<DP> + lane * 16;
+    if (wave >= 4) {
+      put_half<DP>(half, f.o);
+      *reinterpret_cast<float2*>(half + DP / 8 * 1024) = make_float2(f.st.m, f.st.l);
+    }
+    __syncthreads();
+    if (wave >= 4) return;
+    const float2 ml = *reinterpret_cast<const float2*>(half + DP / 8 * 1024);
+    const float to = fmaxf(f.st.m, ml.x);
+    const float f0 = f.st.m == NEG_INF ? 0.f : __builtin_amdgcn_exp2f((f.st.m - to) * a.c);
+    const float f1 = ml.x == NEG_INF ? 0.f : __builtin_amdgcn_exp2f((ml.x - to) * a.c);
+    f.st.nm = to == NEG_INF ? 0.f : -to * a.c;
+    f.st.l = f.st.l * f0 + ml.y * f1;
+#pragma unroll
+    for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4_t x = *reinterpret_cast<const f32x4_t*>(half + (dt * 4 + g) * 1024);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f.o[dt][4 * g + j] = f.o[dt][4 * g + j] * f0 + x[j] * f1;
+      }
+  }
   if (row >= own.end) return;
   const float l = pair_sum(f.st.l);
   const bool some = f.own.hi > f.own.lo && l != 0.f;          // (l is NaN where a score was)
@@ -252,18 +277,24 @@ int launch_split(FwdArgs a, hipStream_t st) {
   hipLaunchKernelGGL((packed_attn_fwd_split_kernel<DT, DP, PAD, NW>), dim3(xcd_grid(a.Hq, a.ntiles)), dim3(64 * NW), lds, st, a);
   return MVF_OK;
 }
+template <int DT, int DP, bool PAD, int H>
+int launch_wide(FwdArgs a, hipStream_t st) {
+  typedef Ring<Op<DT>, DP, 3, 4 * H> R;
+  constexpr size_t lds = std::max<size_t>(R::NB * R::BUF, H == 2 ? 4 * HALF<DP> : 0);
+  static uint64_t attr = 0;
+  if (int rc = mvf_ensure_lds(reinterpret_cast<const void*>(packed_attn_fwd_kernel<DT, DP, PAD, H>), lds, attr)) return rc;
+  a.ntiles = (int)tile_bound<128>(a.T, a.n_seqs);
+  hipLaunchKernelGGL((packed_attn_fwd_kernel<DT, DP, PAD, H>), dim3(xcd_grid(a.Hq, a.ntiles)), dim3(256 * H), lds, st, a);
+  return MVF_OK;
+}
 template <int DT, int DP, bool PAD>
 int launch(FwdArgs a, hipStream_t st) {
-  typedef Ring<Op<DT>, DP> R;
   if (use_split(tile_bound<128>(a.T, a.n_seqs) * a.Hq, DT, a.T, a.n_seqs)) {
     constexpr int NW8 = SPLIT_WAVES<Op<DT>, DP>;
     if (int rc = long_walks(a.T, a.n_seqs) ? launch_split<DT, DP, PAD, NW8>(a, st) : launch_split<DT, DP, PAD, 4>(a, st)) return rc;
   } else {
-    const size_t lds = R::NB * R::BUF;
-    static uint64_t attr = 0;
-    if (int rc = mvf_ensure_lds(reinterpret_cast<const void*>(packed_attn_fwd_kernel<DT, DP, PAD>), lds, attr)) return rc;
-    a.ntiles = (int)tile_bound<128>(a.T, a.n_seqs);
-    hipLaunchKernelGGL((packed_attn_fwd_kernel<DT, DP, PAD>), dim3(xcd_grid(a.Hq, a.ntiles)), dim3(256), lds, st, a);
+    constexpr int H = PAIRS<Op<DT>, DP> ? 2 : 1;
+    if (int rc = use_pairs(a.T, a.n_seqs, a.Hq, a.frame) ? launch_wide<DT, DP, PAD, H>(a, st) : launch_wide<DT, DP, PAD, 1>(a, st)) return rc;
   }
   MVF_LAUNCH_CHECK();
   return MVF_OK;

@@ -164,26 +164,26 @@ struct Dq {
   }
 };
 
-template <int DT, int DP, bool PAD>
-__global__ __launch_bounds__(256, DT == MVF_F32 && DP > 32 ? 1 : 2) void packed_attn_dq_kernel(BwdArgs a) {
+template <int DT, int DP, bool PAD, int H>
+__global__ __launch_bounds__(256 * H, DT == MVF_F32 && DP > 32 ? H : 2) void packed_attn_dq_kernel(BwdArgs a) {
   typedef Op<DT> O;
   typedef Img<O, DP> I;
-  typedef Ring<O, DP> R;
+  typedef Ring<O, DP, 3, 4 * H> R;
   extern __shared__ __attribute__((aligned(256))) char smem[];
-  __shared__ int s_span[8];
+  __shared__ int s_span[8 * H];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Unit u = xcd_unit(a.Hq, a.ntiles);
   if (u.head < 0) return;
   const int head = u.head;
   const OwnTile own = find_tile<128>(a.cu, a.n_seqs, a.T, u.tile, a.ntiles, a.frame == 0 ? Walk::ALL : Walk::LATE);
   if (own.row0 >= own.end) return;
-  const int row = own.row0 + wave * 32 + (lane & 31);
+  const int row = own.row0 + (wave & 3) * 32 + (lane & 31);
   Dq<DT, DP> f;
-  f.start(a, head, row, lane, row < own.end);
+  f.start(a, head, row, lane, row < own.end && wave < 4);
   f.own = keys_of(sequence_of(own, a.cu, a.n_seqs, a.T, row), a.frame, row);
   const WaveSpan ws = wave_span(f.own);
   if constexpr (PAD) clear_lds(smem, R::NB * R::BUF);
-  const Span span = block_span(ws, s_span, lane, wave, 4);
+  const Span span = block_span(ws, s_span, lane, wave, 4 * H);
   const int g = a.Hq / a.Hk;
   const char *kb = a.k + head / g * a.hsk, *vb = a.v + head / g * a.hsv;
   R ring;
@@ -198,10 +198,18 @@ __global__ __launch_bounds__(256, DT == MVF_F32 && DP > 32 ? 1 : 2) void packed_
     if (b0 + 2 * R::KB < span.hi) ring.template issue<PAD>(b0 + 2 * R::KB, span.hi, buf == 0 ? 2 : buf - 1, wave, lane);
     const uint32_t ik = lds_addr(smem) + buf * R::BUF;
 #pragma unroll 1
-    for (int t = 0; t < R::KB / 32; ++t) f.any_tile(ws, ik + t * 32 * I::RB, ik + R::IMG + t * 32 * I::RB, b0 + 32 * t);
+    for (int t = wave >> 2; t < R::KB / 32; t += H) f.any_tile(ws, ik + t * 32 * I::RB, ik + R::IMG + t * 32 * I::RB, b0 + 32 * t);
     buf = buf == 2 ? 0 : buf + 1;
   }
-  if (f.bad) f.slow(a, kb, vb, ws.any.lo, 32, ws.any.hi);
+  if (f.bad) f.slow(a, kb, vb, span.lo + 32 * (wave >> 2), 32 * H, ws.any.hi);
+  if constexpr (H == 2) {
+    __syncthreads();
+    char* half = smem + (wave & 3) * HALF<DP> + lane * 16;
+    if (wave >= 4) put_half<DP>(half, f.dq);
+    __syncthreads();
+    if (wave >= 4) return;
+    add_half<DP>(half, f.dq);
+  }
   if (row < own.end) store_rows<O, DP>(a.dq, ((size_t)row * a.Hq + head) * a.D, f.dq, a.scale, f.own.hi > 0, a.D, lane >> 5);
 }
 
@@ -326,13 +334,13 @@ struct Dkv {
     accumulate<O, DP>(dv, s, cd);
     accumulate<O, DP>(dk, dp, cq);
   }
-  // over tiles it = first, first + step, ... of (head h0 + .. of g, 32-query tile)
-  __device__ __forceinline__ void slow(const BwdArgs& a, int kh, int row, int h0, int g, Span any, int first, int step) {
+  // over tiles it = first, first + step, ... of (head h0 + .. of g, 32-query tile, of which a head has a multiple of `per`)
+  __device__ __forceinline__ void slow(const BwdArgs& a, int kh, int row, int h0, int g, Span any, int first, int step, int per = 1) {
     typename O::Frag vf[DP / 16];
     load_row<O, DP>(vf, a.v + (long)min(row, a.T - 1) * a.ldv + kh * a.hsv, a.D, lane >> 5);
 #pragma unroll
     for (int dt = 0; dt < DP / 32; ++dt) { dk[dt] = zero16(); dv[dt] = zero16(); }
-    const int nt = (any.hi - any.lo + 31) >> 5;
+    const int nt = (((any.hi - any.lo + 31) >> 5) + per - 1) / per * per;
 #pragma unroll 1
     for (int it = first; it < nt * g; it += step) {
       const int h = h0 + it / nt, q0 = any.lo + it % nt * 32;
@@ -364,32 +372,32 @@ __device__ __forceinline__ const float* stat_at(const BwdArgs& a, int h, int row
 
 template <int DT, int DP>
 constexpr bool V_IN_LDS = DT != MVF_F32 && DP == 128;
-template <int DT, int DP>
-using DkvRing = Ring<Op<DT>, DP, V_IN_LDS<DT, DP> ? 2 : 3>;
+template <int DT, int DP, int H>
+using DkvRing = Ring<Op<DT>, DP, V_IN_LDS<DT, DP> ? 2 : 3, 4 * H>;
 
-template <int DT, int DP, bool PAD>
-__global__ __launch_bounds__(256, DT == MVF_F32 && DP > 32 ? 1 : 2) void packed_attn_dkv_kernel(BwdArgs a) {
+template <int DT, int DP, bool PAD, int H>
+__global__ __launch_bounds__(256 * H, DT == MVF_F32 && DP > 32 ? H : 2) void packed_attn_dkv_kernel(BwdArgs a) {
   typedef Op<DT> O;
   typedef Img<O, DP> I;
-  typedef DkvRing<DT, DP> R;
+  typedef DkvRing<DT, DP, H> R;
   constexpr bool VL = V_IN_LDS<DT, DP>;
   constexpr int NF = planes(DT) * R::KB, SB = (NF + 63) / 64 * 256;     // floats of a block's statistics, bytes of their buffer
   static_assert(NF <= 256, "one piece per wave");
   extern __shared__ __attribute__((aligned(256))) char smem[];
-  __shared__ int s_span[8];
+  __shared__ int s_span[8 * H];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Unit u = xcd_unit(a.Hk * a.parts, a.ntiles);
   if (u.head < 0) return;
   const int kh = u.head / a.parts, part = u.head % a.parts;
   const OwnTile own = find_tile<128>(a.cu, a.n_seqs, a.T, u.tile, a.ntiles, a.frame == 0 ? Walk::ALL : Walk::EARLY);
   if (own.row0 >= own.end) return;
-  const int row = own.row0 + wave * 32 + (lane & 31);
+  const int row = own.row0 + (wave & 3) * 32 + (lane & 31);
   Dkv<DT, DP, VL> f;
-  f.start(a, kh, row, lane, smem + R::NB * (R::BUF + SB) + wave * 32 * I::RB);
+  f.start(a, kh, row, lane, smem + R::NB * (R::BUF + SB) + (wave & 3) * 32 * I::RB);      // (two waves write the same V rows)
   f.own = queries_of(sequence_of(own, a.cu, a.n_seqs, a.T, row), a.frame, row);
   const WaveSpan ws = wave_span(f.own);
   if constexpr (PAD) clear_lds(smem, R::NB * R::BUF);
-  const Span span = block_span(ws, s_span, lane, wave, 4);
+  const Span span = block_span(ws, s_span, lane, wave, 4 * H);
   const int g = a.Hq / a.Hk / a.parts, h0 = kh * (a.Hq / a.Hk) + part * g;
   const int nblk = span.hi > span.lo ? (span.hi - span.lo + R::KB - 1) / R::KB : 0, total = nblk * g;
   const uint32_t lds0 = lds_addr(smem), stat0 = lds0 + R::NB * R::BUF;
@@ -414,13 +422,24 @@ __global__ __launch_bounds__(256, DT == MVF_F32 && DP > 32 ? 1 : 2) void packed_
     if (it + R::NB - 1 < total) issue(buf == 0 ? R::NB - 1 : buf - 1);
     const uint32_t iq = lds0 + buf * R::BUF, so = stat0 + buf * SB;
 #pragma unroll 1
-    for (int t = 0; t < R::KB / 32; ++t)
+    for (int t = wave >> 2; t < R::KB / 32; t += H)
       f.any_tile(ws, iq + t * 32 * I::RB, iq + R::IMG + t * 32 * I::RB, so + t * 128, R::KB * 4, b0 + 32 * t);
     buf = buf == R::NB - 1 ? 0 : buf + 1;
     b0 += R::KB;
     if (b0 >= span.hi) b0 = span.lo;
   }
-  if (f.bad) f.slow(a, kh, row, h0, g, ws.any, 0, 1);
+  if (f.bad) f.slow(a, kh, row, h0, g, {span.lo, ws.any.hi}, wave >> 2, H, H);
+  if constexpr (H == 2) {
+    char* half = smem + (wave & 3) * HALF<DP> + lane * 16;
+#pragma unroll 1
+    for (int i = 0; i < 2; ++i) {
+      __syncthreads();
+      if (wave >= 4) put_half<DP>(half, i == 0 ? f.dk : f.dv);
+      __syncthreads();
+      if (wave < 4) add_half<DP>(half, i == 0 ? f.dk : f.dv);
+    }
+    if (wave >= 4) return;
+  }
   if (row >= own.end) return;
   const size_t at = ((size_t)row * a.Hk + kh) * a.D;
   if (a.parts > 1) {
@@ -519,36 +538,47 @@ int head_parts(long T, long n_seqs, int Hq, int Hk, int dtype) {
   return g;
 }
 
+template <int DT, int DP, bool PAD, int H>
+int launch_dq(const BwdArgs& a, hipStream_t st) {
+  typedef Ring<Op<DT>, DP, 3, 4 * H> R;
+  constexpr size_t lds = R::NB * R::BUF;
+  static_assert(H == 1 || lds >= 4 * HALF<DP>);
+  static uint64_t attr = 0;
+  if (int rc = mvf_ensure_lds(reinterpret_cast<const void*>(packed_attn_dq_kernel<DT, DP, PAD, H>), lds, attr)) return rc;
+  hipLaunchKernelGGL((packed_attn_dq_kernel<DT, DP, PAD, H>), dim3(xcd_grid(a.Hq, a.ntiles)), dim3(256 * H), lds, st, a);
+  return MVF_OK;
+}
+template <int DT, int DP, bool PAD, int H>
+int launch_dkv(const BwdArgs& a, hipStream_t st) {
+  typedef DkvRing<DT, DP, H> R;
+  constexpr size_t lds = R::NB * (R::BUF + (planes(DT) * R::KB + 63) / 64 * 256) + (V_IN_LDS<DT, DP> ? 128 * Img<Op<DT>, DP>::RB : 0);
+  static_assert(H == 1 || lds >= 4 * HALF<DP>);
+  static uint64_t attr = 0;
+  if (int rc = mvf_ensure_lds(reinterpret_cast<const void*>(packed_attn_dkv_kernel<DT, DP, PAD, H>), lds, attr)) return rc;
+  hipLaunchKernelGGL((packed_attn_dkv_kernel<DT, DP, PAD, H>), dim3(xcd_grid((long)a.Hk * a.parts, a.ntiles)), dim3(256 * H), lds, st, a);
+  return MVF_OK;
+}
 template <int DT, int DP, bool PAD>
 int launch(BwdArgs a, hipStream_t st) {
-  typedef Ring<Op<DT>, DP> R;
-  typedef DkvRing<DT, DP> R2;
   typedef SplitTiles<Op<DT>, DP, 4> S;
-  static uint64_t attr[4] = {0, 0, 0, 0};
-  const int wide = (int)tile_bound<128>(a.T, a.n_seqs);
-  const bool split = use_split((long)wide * a.Hq, DT, a.T, a.n_seqs);
+  constexpr int H = PAIRS<Op<DT>, DP> ? 2 : 1;
+  static uint64_t attr[2] = {0, 0};
+  const bool split = use_split(tile_bound<128>(a.T, a.n_seqs) * a.Hq, DT, a.T, a.n_seqs);
+  a.ntiles = (int)(split ? tile_bound<32>(a.T, a.n_seqs) : tile_bound<128>(a.T, a.n_seqs));
   if (split) {
     const size_t lds = std::max(4 * S::NB * S::BUF, (JOIN_BYTES<DP>));
-    if (int rc = mvf_ensure_lds(reinterpret_cast<const void*>(packed_attn_dq_split_kernel<DT, DP, PAD>), lds, attr[2])) return rc;
-    a.ntiles = (int)tile_bound<32>(a.T, a.n_seqs);
+    if (int rc = mvf_ensure_lds(reinterpret_cast<const void*>(packed_attn_dq_split_kernel<DT, DP, PAD>), lds, attr[0])) return rc;
     hipLaunchKernelGGL((packed_attn_dq_split_kernel<DT, DP, PAD>), dim3(xcd_grid(a.Hq, a.ntiles)), dim3(256), lds, st, a);
   } else {
-    const size_t lds = R::NB * R::BUF;
-    if (int rc = mvf_ensure_lds(reinterpret_cast<const void*>(packed_attn_dq_kernel<DT, DP, PAD>), lds, attr[0])) return rc;
-    a.ntiles = wide;
-    hipLaunchKernelGGL((packed_attn_dq_kernel<DT, DP, PAD>), dim3(xcd_grid(a.Hq, wide)), dim3(256), lds, st, a);
+    if (int rc = use_pairs(a.T, a.n_seqs, a.Hq, a.frame) ? launch_dq<DT, DP, PAD, H>(a, st) : launch_dq<DT, DP, PAD, 1>(a, st)) return rc;
   }
   MVF_LAUNCH_CHECK();
   if (split) {
     const size_t lds = std::max(4 * S::NB * (S::BUF + (planes(DT) * 32 + 63) / 64 * 256), (JOIN_BYTES<DP>));
-    if (int rc = mvf_ensure_lds(reinterpret_cast<const void*>(packed_attn_dkv_split_kernel<DT, DP, PAD>), lds, attr[3])) return rc;
-    a.ntiles = (int)tile_bound<32>(a.T, a.n_seqs);
+    if (int rc = mvf_ensure_lds(reinterpret_cast<const void*>(packed_attn_dkv_split_kernel<DT, DP, PAD>), lds, attr[1])) return rc;
     hipLaunchKernelGGL((packed_attn_dkv_split_kernel<DT, DP, PAD>), dim3(xcd_grid((long)a.Hk * a.parts, a.ntiles)), dim3(256), lds, st, a);
   } else {
-    const size_t lds = R2::NB * (R2::BUF + (planes(DT) * R2::KB + 63) / 64 * 256) + (V_IN_LDS<DT, DP> ? 128 * Img<Op<DT>, DP>::RB : 0);
-    if (int rc = mvf_ensure_lds(reinterpret_cast<const void*>(packed_attn_dkv_kernel<DT, DP, PAD>), lds, attr[1])) return rc;
-    a.ntiles = wide;
-    hipLaunchKernelGGL((packed_attn_dkv_kernel<DT, DP, PAD>), dim3(xcd_grid((long)a.Hk * a.parts, wide)), dim3(256), lds, st, a);
+    if (int rc = use_pairs(a.T, a.n_seqs, (long)a.Hk * a.parts, a.frame) ? launch_dkv<DT, DP, PAD, H>(a, st) : launch_dkv<DT, DP, PAD, 1>(a, st)) return rc;
   }
   MVF_LAUNCH_CHECK();
   if (a.parts > 1) {
