@@ -382,16 +382,6 @@ static inline unsigned xcd_grid(long heads, long tiles) {
   return (unsigned)((heads & 7) == 0 ? heads * tiles : (heads & 3) == 0 ? heads * ((tiles + 1) / 2 * 2) : (heads * tiles + 7) / 8 * 8);
 }
 
-// Which form: `wide` = the wide one's workgroups.  Below one for each of the 256 compute units the split form is faster (measured, us: 1 x 512
-// bf16 D 128 16 heads, 80 workgroups: wide 20, split 13; 4 x 197 D 64, 96: 10.5, 9.5), above it the wide one (16 x 197 D 64, 384: 13, 23;
-// 4 x 1024 D 128, 544: 43, 96) unless few workgroups walk far: up to two for each unit and 4096 tokens a sequence (1 x 4096 D 64, 408: 99,
-// 82; 1 x 2048 D 128, 304: 62, 69), in fp32, whose walks are 8 times as long, 1024 (4 x 1024 D 128, 280: 157, 131; 8 x 400 D 64, 384: 65, 83).
-static inline bool use_split(long wide, int dtype, long T, long n_seqs) {
-#ifdef MVF_SPLIT_FORCE     // build flag, A/B measurements only
-  return MVF_SPLIT_FORCE;
-#endif
-  return wide < 256 || (wide < 512 && T >= (dtype == MVF_F32 ? 1024 : 4096) * n_seqs);
-}
 // Waves of a split forward's workgroup: eight, a tile each at a time, for walks of 512 and more where two such workgroups fit a unit's LDS
 // (1 x 4096 bf16 D 64 12 heads: 59 us, with four 73; 2 x 1440 fp32 D 32 the same), else four with two tiles each.  The backward, which
 // holds more registers, keeps four (1 x 4096: 173 us, with eight 205; 2 x 1440: 108, 114).
@@ -444,6 +434,17 @@ static inline long tile_bound(long T, long n) {   // no fewer than the tiles the
 }
 static inline bool use_pairs(long T, long n_seqs, long heads, int frame) {
   return frame > 0 && T >= 1024 * n_seqs && tile_bound<128>(T, n_seqs) * heads <= 640;
+}
+// Which form: `wide` = the wide one's workgroups.  Below one for each of the 256 compute units the split form is faster (measured, us: 1 x 512
+// bf16 D 128 16 heads, 80 workgroups: wide 20, split 13; 4 x 197 D 64, 96: 10.5, 9.5), above it the wide one (16 x 197 D 64, 384: 13, 23;
+// 4 x 1024 D 128, 544: 43, 96) unless few workgroups walk far: up to two for each unit and 4096 tokens a sequence (1 x 4096 D 64, 408: 99,
+// 59), in fp32, whose walks are 8 times as long, 1024 (4 x 1024 D 128, 280: 157, 131; 8 x 400 D 64, 384: 65, 83).  Pairs of waves move
+// that border (wide and split, forward / backward, causal: 1 x 2048 bf16 D 128 8 heads, 152: 41 / 139, 37 / 94; 1 x 1300 16 heads, 208:
+// 31 / 108, 43 / 112; 1 x 5000 8 heads, 336: 100 / 324, 167 / 419; 2 x 2048 fp32 D 64, 272: 151 / 487, 128 / 372; 3 x 2048, 408: 151 /
+// 488, 182 / 526).
+static inline bool use_split(long wide, int dtype, long T, long n_seqs, bool pairs) {
+  if (pairs) return wide < (dtype == MVF_F32 ? 352 : 192);
+  return wide < 256 || (wide < 512 && T >= (dtype == MVF_F32 ? 1024 : 4096) * n_seqs);
 }
 // The t-th tile, found by every wave for itself.  Up to 62 sequences the tiles come in the order of their walks, longest first (causal: the
 // tile's place in its sequence, counted from the end that sees most; else the sequence's length), so that the last workgroups to

@@ -289,12 +289,13 @@ int launch_wide(FwdArgs a, hipStream_t st) {
 }
 template <int DT, int DP, bool PAD>
 int launch(FwdArgs a, hipStream_t st) {
-  if (use_split(tile_bound<128>(a.T, a.n_seqs) * a.Hq, DT, a.T, a.n_seqs)) {
+  const bool pairs = PAIRS<Op<DT>, DP> && use_pairs(a.T, a.n_seqs, a.Hq, a.frame);
+  if (use_split(tile_bound<128>(a.T, a.n_seqs) * a.Hq, DT, a.T, a.n_seqs, pairs)) {
     constexpr int NW8 = SPLIT_WAVES<Op<DT>, DP>;
     if (int rc = long_walks(a.T, a.n_seqs) ? launch_split<DT, DP, PAD, NW8>(a, st) : launch_split<DT, DP, PAD, 4>(a, st)) return rc;
   } else {
     constexpr int H = PAIRS<Op<DT>, DP> ? 2 : 1;
-    if (int rc = use_pairs(a.T, a.n_seqs, a.Hq, a.frame) ? launch_wide<DT, DP, PAD, H>(a, st) : launch_wide<DT, DP, PAD, 1>(a, st)) return rc;
+    if (int rc = pairs ? launch_wide<DT, DP, PAD, H>(a, st) : launch_wide<DT, DP, PAD, 1>(a, st)) return rc;
   }
   MVF_LAUNCH_CHECK();
   return MVF_OK;

@@ -531,7 +531,7 @@ __global__ __launch_bounds__(256) void packed_attn_sum_kernel(const float* part,
 // (16 x 64 D 128 32/8: 4 parts 65 us, 1 part 44).
 int head_parts(long T, long n_seqs, int Hq, int Hk, int dtype) {
   const int g = Hq / Hk;
-  const bool split = use_split(tile_bound<128>(T, n_seqs) * Hq, dtype, T, n_seqs);
+  const bool split = use_split(tile_bound<128>(T, n_seqs) * Hq, dtype, T, n_seqs, false);     // near enough: any number of parts is right
   const long units = (split ? tile_bound<32>(T, n_seqs) : tile_bound<128>(T, n_seqs)) * Hk, want = T >= 512 * n_seqs ? 1024 : 256;
   for (int p = 1; p < g; ++p)
     if (g % p == 0 && units * p >= want) return p;
@@ -563,14 +563,15 @@ int launch(BwdArgs a, hipStream_t st) {
   typedef SplitTiles<Op<DT>, DP, 4> S;
   constexpr int H = PAIRS<Op<DT>, DP> ? 2 : 1;
   static uint64_t attr[2] = {0, 0};
-  const bool split = use_split(tile_bound<128>(a.T, a.n_seqs) * a.Hq, DT, a.T, a.n_seqs);
+  const bool pairs = PAIRS<Op<DT>, DP> && use_pairs(a.T, a.n_seqs, a.Hq, a.frame);
+  const bool split = use_split(tile_bound<128>(a.T, a.n_seqs) * a.Hq, DT, a.T, a.n_seqs, pairs);
   a.ntiles = (int)(split ? tile_bound<32>(a.T, a.n_seqs) : tile_bound<128>(a.T, a.n_seqs));
   if (split) {
     const size_t lds = std::max(4 * S::NB * S::BUF, (JOIN_BYTES<DP>));
     if (int rc = mvf_ensure_lds(reinterpret_cast<const void*>(packed_attn_dq_split_kernel<DT, DP, PAD>), lds, attr[0])) return rc;
     hipLaunchKernelGGL((packed_attn_dq_split_kernel<DT, DP, PAD>), dim3(xcd_grid(a.Hq, a.ntiles)), dim3(256), lds, st, a);
   } else {
-    if (int rc = use_pairs(a.T, a.n_seqs, a.Hq, a.frame) ? launch_dq<DT, DP, PAD, H>(a, st) : launch_dq<DT, DP, PAD, 1>(a, st)) return rc;
+    if (int rc = pairs ? launch_dq<DT, DP, PAD, H>(a, st) : launch_dq<DT, DP, PAD, 1>(a, st)) return rc;
   }
   MVF_LAUNCH_CHECK();
   if (split) {
@@ -578,7 +579,8 @@ int launch(BwdArgs a, hipStream_t st) {
     if (int rc = mvf_ensure_lds(reinterpret_cast<const void*>(packed_attn_dkv_split_kernel<DT, DP, PAD>), lds, attr[1])) return rc;
     hipLaunchKernelGGL((packed_attn_dkv_split_kernel<DT, DP, PAD>), dim3(xcd_grid((long)a.Hk * a.parts, a.ntiles)), dim3(256), lds, st, a);
   } else {
-    if (int rc = use_pairs(a.T, a.n_seqs, (long)a.Hk * a.parts, a.frame) ? launch_dkv<DT, DP, PAD, H>(a, st) : launch_dkv<DT, DP, PAD, 1>(a, st)) return rc;
+    const bool two = use_pairs(a.T, a.n_seqs, (long)a.Hk * a.parts, a.frame);
+    if (int rc = two ? launch_dkv<DT, DP, PAD, H>(a, st) : launch_dkv<DT, DP, PAD, 1>(a, st)) return rc;
   }
   MVF_LAUNCH_CHECK();
   if (a.parts > 1) {
