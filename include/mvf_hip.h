@@ -648,7 +648,8 @@ int mvf_rotary(int dtype, const void* q, long ldq, long hsq, const void* k, long
                int Hk, int D, hipStream_t stream);
 /* The same for new tokens of streams with a paged cache: q_out [T, Hq, D]; turned k and plain v go to row index[t] % page of page
  * block_table[seq[t]][index[t] / page] of k_cache, v_cache [n_pages, page, Hk, D].  block_table [n_seqs][table_width].  A token whose seq,
- * index or page lies outside (seq = -1: padding) is not written.  Two tokens of one slot: either may win. */
+ * index or page lies outside (seq = -1: padding) is not written.  Two tokens of one call must not have
+ * the same slot (it would hold a mixture of them). */
 int mvf_rotary_append(int dtype, const void* q, long ldq, long hsq, const void* k, long ldk, long hsk, const void* v, long ldv, long hsv,
                       const void* pos, int pos_type, const double* freqs, int s0, int s1, int s2, int interleaved, void* q_out,
                       void* k_cache, void* v_cache, const int* block_table, int table_width, int n_seqs, const int* seq,

@@ -526,6 +526,32 @@ def test_training_through_rotary_and_attention():
 
 
 # ------------------------------------------------------------------------------------------------ streams, graphs, repetition
+def test_a_second_derivative_is_refused():
+    q, k, v, do = (randn(40, 2, 32, dtype=torch.float32, seed=300 + i).requires_grad_() for i in range(4))
+    out = ops.packed_attention(q, k, v, cu_tensor([0, 40]), frame=1)
+    dq, = torch.autograd.grad(out, q, do, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(dq.sum(), q)
+    turned, _ = ops.rotary(q, k, torch.arange(40, device=DEV)[:, None].contiguous(), ops.rotary_freqs((16,)), (16,))
+    dq, = torch.autograd.grad(turned, q, do, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(dq.sum(), do)
+
+
+def test_append_ignores_slots_outside_32_bits_and_one_cache_for_both():
+    kc, vc = make_cache(4, 16, 2, 32, torch.float32, 310)
+    before = kc.clone()
+    q = randn(3, 2, 32, dtype=torch.float32, seed=311)
+    pos, freqs = torch.zeros(3, 1, dtype=torch.int64, device=DEV), ops.rotary_freqs((16,))
+    table = torch.tensor([[0, 1, 2, 3]], dtype=torch.int32, device=DEV)
+    seq = torch.tensor([0, 2 ** 32, 0], device=DEV)
+    index = torch.tensor([2 ** 32 + 5, 9, -2 ** 32 + 1], device=DEV)
+    ops.rotary_append(q, q, q, pos, freqs, (16,), kc, vc, table, seq, index)
+    assert torch.equal(kc, before)
+    with pytest.raises(ValueError):
+        ops.rotary_append(q, q, q, pos, freqs, (16,), kc, kc, table, seq, index)
+
+
 def test_same_bits_every_time():
     c = cum([700, 3, 1000])
     t = c[-1]

@@ -183,3 +183,25 @@ def test_paged_workspace_is_asked_for_and_checked(lib):
     assert lib.mvf_paged_attn_workspace_bytes(1, 1, 3, 2, 32, 4096, 16) == 0
     assert lib.mvf_paged_attn_workspace_bytes(64, 1, 8, 8, 128, 1, 16) == 0          # one page per stream: nothing to join
     assert isinstance(ctypes.c_size_t(size).value, int)
+
+
+def test_indices_outside_32_bits_stay_outside():
+    """int64 indices are not cut to their low bits: 2^32 + 3 is not slot 3."""
+    q = heads()
+    got = ops._index_operand(torch.tensor([2 ** 32 + 3, -2 ** 40, 7, -1]), q, (4,), 'index')
+    assert got.dtype == torch.int32 and got.tolist() == [2 ** 31 - 1, -2 ** 31, 7, -1]
+    i32 = torch.tensor([1, 2], dtype=torch.int32)
+    assert ops._index_operand(i32, q, (2,), 'seq') is i32
+
+
+def test_sizes_beyond_the_kernels_counters_are_refused():
+    far = torch.zeros(1, dtype=torch.bfloat16).expand(2 ** 30, 1, 8)
+    with pytest.raises(ValueError):
+        ops._heads(far, 'q')
+    ops._heads(far[1:], 'q')
+    with pytest.raises(ValueError):
+        ops.packed_attention(far, far, far, torch.tensor([0, 4], dtype=torch.int32))
+
+
+def test_paged_entry_point_refuses_more_keys_than_it_counts(lib):
+    assert lib.mvf_paged_attn(*dict(PAGED, width=2 ** 21, page=1024).values(), None) == 10001

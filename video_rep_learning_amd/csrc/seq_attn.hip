@@ -1,13 +1,19 @@
 // Self-attention over packed sequences of different lengths, grouped heads, causal by token or by frame:
 //   out[i, h] = sum_j softmax_j(scale q[i, h] . k[j, h / g]) v[j, h / g],   j in i's sequence, j < (i / frame + 1) frame inside it
-// Tiles are cut out of the packed rows, not out of each sequence: a tile may hold the end of one sequence and the start of the next,
-// every row has its own [lo, hi) of keys, and a tile walks the union.  So nothing but the number of rows sizes the grid (no host copy
-// of the lengths), empty sequences cost nothing, short ones share a tile, and rows behind the last sequence come out as zeros.
+// The running maximum and sum of a row's softmax stay in the row's lane, scores and weights in registers between the two products.
+// Every sequence is cut into row tiles of its own, found on the device: nothing but the numbers of rows and sequences sizes the grid (no
+// host copy of the lengths), empty sequences cost nothing, and rows outside every sequence come out as zeros.
 //
-// Two forms of the same tile arithmetic:
+// Three forms of the same tile arithmetic, chosen by use_split and use_pairs:
 //   wide:   a workgroup owns 128 rows of one head (32 per wave) and its waves share each block of keys;
-//   split:  a workgroup owns 32 rows, each wave walks every fourth 32-key tile by itself, the four partial softmaxes are joined at the
-//           end: four times as many workgroups and a quarter of the dependent steps, for four times the key traffic.
+//   pairs:  the same with two waves for each 32 rows, which take a block's tiles in turn and join their sums at the end;
+//   split:  a workgroup owns 32 rows, each wave walks every fourth (or eighth) 32-key tile by itself, the partial softmaxes are joined at
+//           the end: four times as many workgroups and a quarter of the dependent steps, for four times the key traffic.
+// The weights are rounded to the operands' format for the second product (relative 2^-9 in bf16, random in sign, so the sum is off by that
+// much of its size, as the rounding of the result is); their sum is taken before, in 32 bits.
+// Measured: 2 x 8192 causal bf16, 16 query heads of 128 on 4: 0.60 ms, 916 TFLOP/s of visible pairs (a large bf16 matrix product: 1130 to
+// 1150); 32 x 785, 12 of 64: 114 us, 530; 8 x 1440 fp32 causal by 6, 8 of 32: 119 us, 72 (a large fp32 product: 148).  Bound by the waves'
+// own chains: at D 96 the matrix pipe is busy 24 % of the cycles, the vector unit 31 %, and 32 % of the waves' time goes into waits.
 #include "mvf_hip_internal.h"
 #include "seq_attn.h"
 

@@ -10,6 +10,7 @@ import ctypes
 
 import torch
 import torch.distributed as dist
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import call, ptr, stream, F32, BF16, FP8, F16
@@ -2211,6 +2212,8 @@ def _index_operand(t, like, shape, what):
         raise ValueError('%s must be int32 (or int64), got %s' % (what, t.dtype))
     if t.dim() != len(shape) or any(n >= 0 and n != m for n, m in zip(shape, t.shape)):
         raise ValueError('%s: expected shape %s, got %s' % (what, shape, tuple(t.shape)))
+    if t.dtype is torch.int64:
+        t = t.clamp(-2 ** 31, 2 ** 31 - 1)         # what lies outside 32 bits stays outside every range
     return t if t.dtype is torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
 
 
@@ -2233,6 +2236,8 @@ def _heads(t, what, tokens=None, size=None):
                                                                  'head size' if size is None else size, tuple(t.shape)))
     if t.shape[1] == 0 or t.shape[2] == 0 or t.shape[2] % 8:
         raise ValueError('%s: at least one head of a size that is a multiple of 8, got %s' % (what, tuple(t.shape)))
+    if t.shape[0] >= 2 ** 30:
+        raise ValueError('%s: fewer than 2^30 tokens, got %d' % (what, t.shape[0]))
 
 
 def _frame_arg(frame):
@@ -2299,6 +2304,7 @@ class _Rotary(torch.autograd.Function):
         return _rotary_call(q, k, pos, freqs, sections, interleaved, False)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dq, dk):
         pos, freqs = ctx.saved_tensors
         a = (pos, freqs) + ctx.cfg + (True,)
@@ -2312,7 +2318,7 @@ def rotary(q, k, pos, freqs, sections, interleaved=False):
     """Rotary positions with one to three axes (time, row, column; or time, entity): q [T, Hq, D], k [T, Hk, D] (or None) turned by
     pos[t, axis] * freqs[pair] -> new (q, k).  `sections`: pairs of each axis, in the order of pos's columns; channels behind
     2 * sum(sections) stay.  interleaved: a pair is two neighbouring channels, otherwise channels p and p + sum(sections).  pos [T, axes]
-    int32 / int64 / float32; freqs: rotary_freqs(sections).  fp32, bf16 or fp16; differentiable in q and k."""
+    int32 / int64 / float32; freqs: rotary_freqs(sections).  fp32, bf16 or fp16; differentiable (once) in q and k."""
     _heads(q, 'q')
     if k is not None:
         _heads(k, 'k', q.shape[0], q.shape[2])
@@ -2332,12 +2338,15 @@ def _cache_args(q, k_cache, v_cache):
                 what, q.shape[-1], q.shape[-2], tuple(c.shape)))
         if not c.is_contiguous() or c.data_ptr() % 16:
             raise ValueError('%s must be contiguous and start at a multiple of 16 bytes' % what)
+        if c.shape[0] >= 2 ** 31 or c.shape[1] >= 2 ** 31:
+            raise ValueError('%s: fewer than 2^31 pages of fewer than 2^31 tokens, got %s' % (what, tuple(c.shape)))
 
 
 def rotary_append(q, k, v, pos, freqs, sections, k_cache, v_cache, block_table, seq, index, interleaved=False):
     """rotary() for new tokens of streams with a paged cache: returns the turned q; the turned k and v go into k_cache, v_cache
     [pages, page, Hk, D] at index[t] of stream seq[t], i.e. row index % page of page block_table[seq, index // page].  A token whose seq
-    (-1: padding), index or page lies outside is not written.  For inference: no gradient."""
+    (-1: padding), index or page lies outside is not written; two tokens of one call must not have the same slot (it would hold a mixture of
+    them).  For inference: no gradient."""
     _heads(q, 'q')
     _heads(k, 'k', q.shape[0], q.shape[2])
     _heads(v, 'v', q.shape[0], q.shape[2])
@@ -2355,8 +2364,10 @@ def rotary_append(q, k, v, pos, freqs, sections, k_cache, v_cache, block_table, 
     qo = torch.empty(T, Hq, D, device=q.device, dtype=q.dtype)
     if T == 0:
         return qo
-    if 0 in table.shape:
-        raise ValueError('block_table is empty: %s' % (tuple(table.shape),))
+    if 0 in table.shape or max(table.shape) >= 2 ** 31:
+        raise ValueError('block_table is empty or too large: %s' % (tuple(table.shape),))
+    if k_cache.data_ptr() == v_cache.data_ptr():
+        raise ValueError('k_cache and v_cache are the same memory')
     _launch('mvf_rotary_append', q, code, q.data_ptr(), *q.stride()[:2], k.data_ptr(), *k.stride()[:2], v.data_ptr(), *v.stride()[:2],
             pos.data_ptr(), _POS_DT[pos.dtype], freqs.data_ptr(), *sections, bool(interleaved), qo.data_ptr(), k_cache.data_ptr(),
             v_cache.data_ptr(), table.data_ptr(), table.shape[1], table.shape[0], seq.data_ptr(), index.data_ptr(), k_cache.shape[0],
@@ -2385,6 +2396,7 @@ class _PackedAttention(torch.autograd.Function):
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, d_out):
         q, k, v, cu, out, stat = ctx.saved_tensors
         frame, scale = ctx.cfg
@@ -2408,7 +2420,8 @@ def packed_attention(q, k, v, cu_seqlens, frame=0, scale=None):
     Hk: query head h reads key head h // (Hq // Hk)), sequence b in rows cu_seqlens[b] .. cu_seqlens[b + 1] -> [T, Hq, D].
     frame = 0: a token sees its whole sequence; frame = n: its own and all earlier groups of n tokens of it (1: causal by token; the
     number of entities: causal by frame).  Rows of no sequence give zeros and get zero gradients.  fp32, bf16 or fp16, D a multiple of 8
-    up to 128; scale: 1 / sqrt(D).  Differentiable in q, k, v, the same bits every time."""
+    up to 128; scale: 1 / sqrt(D).  Differentiable (once) in q, k, v, the same bits every time.  In the backward the weights and dS are operands
+    of products in the tensors' type: fp16 wants a scaled loss, as everywhere."""
     _heads(q, 'q')
     _heads(k, 'k', q.shape[0], q.shape[2])
     _heads(v, 'v', q.shape[0], q.shape[2])
@@ -2444,8 +2457,8 @@ def paged_attention(q, k_cache, v_cache, block_table, lengths, frame=1, scale=No
     if B == 0:
         return out
     n_pages, page, Hk, width = k_cache.shape[0], k_cache.shape[1], k_cache.shape[2], table.shape[1]
-    if width == 0:
-        raise ValueError('block_table has no columns')
+    if width == 0 or width * page >= 2 ** 31 - 4096 or B >= 2 ** 30:
+        raise ValueError('block_table: at least one column, fewer than 2^31 - 4096 keys and 2^30 streams, got %s pages of %d' % (tuple(table.shape), page))
     q = _aligned(q)
     need = _lib.load().mvf_paged_attn_workspace_bytes(B, n, Hq, Hk, D, width, page)
     ws = torch.empty(need, device=q.device, dtype=torch.uint8) if need else None
