@@ -2210,7 +2210,10 @@ def _index_operand(t, like, shape, what):
         raise _lib.MvfError('%s on %s, the operands on %s' % (what, t.device, like.device))
     if t.dtype not in (torch.int32, torch.int64):
         raise ValueError('%s must be int32 (or int64), got %s' % (what, t.dtype))
-    if t.dim() != len(shape) or any(n >= 0 and n != m for n, m in zip(shape, t.shape)):
+    bad = t.dim() != len(shape)
+    for n, m in zip(shape, t.shape):
+        bad = bad or n != m and n >= 0
+    if bad:
         raise ValueError('%s: expected shape %s, got %s' % (what, shape, tuple(t.shape)))
     if t.dtype is torch.int64:
         t = t.clamp(-2 ** 31, 2 ** 31 - 1)         # what lies outside 32 bits stays outside every range
@@ -2332,14 +2335,14 @@ def rotary(q, k, pos, freqs, sections, interleaved=False):
 
 
 def _cache_args(q, k_cache, v_cache):
-    for c, what in ((k_cache, 'k_cache'), (v_cache, 'v_cache')):
-        if c.dim() != 4 or c.shape != k_cache.shape or c.shape[3] != q.shape[-1] or 0 in c.shape or q.shape[-2] % c.shape[2]:
-            raise ValueError('%s: expected [pages, page, key heads, %d], key heads dividing %d, got %s' % (
-                what, q.shape[-1], q.shape[-2], tuple(c.shape)))
-        if not c.is_contiguous() or c.data_ptr() % 16:
-            raise ValueError('%s must be contiguous and start at a multiple of 16 bytes' % what)
-        if c.shape[0] >= 2 ** 31 or c.shape[1] >= 2 ** 31:
-            raise ValueError('%s: fewer than 2^31 pages of fewer than 2^31 tokens, got %s' % (what, tuple(c.shape)))
+    shape = k_cache.shape
+    if len(shape) != 4 or v_cache.shape != shape or 0 in shape or shape[3] != q.shape[-1] or q.shape[-2] % shape[2]:
+        raise ValueError('caches: expected two of [pages, page, key heads, %d], key heads dividing %d, got %s and %s' % (
+            q.shape[-1], q.shape[-2], tuple(shape), tuple(v_cache.shape)))
+    if not (k_cache.is_contiguous() and v_cache.is_contiguous()) or (k_cache.data_ptr() | v_cache.data_ptr()) & 15:
+        raise ValueError('k_cache and v_cache must be contiguous and start at multiples of 16 bytes')
+    if shape[0] >= 2 ** 31 or shape[1] >= 2 ** 31:
+        raise ValueError('caches: fewer than 2^31 pages of fewer than 2^31 tokens, got %s' % (tuple(shape),))
 
 
 def rotary_append(q, k, v, pos, freqs, sections, k_cache, v_cache, block_table, seq, index, interleaved=False):
