@@ -11,6 +11,7 @@
 #pragma once
 #include <hip/hip_runtime.h>
 #include <math.h>
+#include <algorithm>
 #include <type_traits>
 #include "../../include/mvf_hip.h"
 #include "common.h"
@@ -363,10 +364,21 @@ __device__ __forceinline__ void clear_lds(char* p, int bytes) {
 
 // blockIdx -> (head, tile).  Workgroups go round the 8 XCDs; a head's keys and values should stay in one XCD's cache, every XCD should get the
 // same share of long and short tiles, and the tiles should start in their order.  Heads a multiple of 8: an eighth of them on each XCD; of
-// 4: a quarter on each pair of XCDs, which take the tiles in turn; else: runs of (head, tile) units.
+// 4: a quarter on each pair of XCDs, which take the tiles in turn; else: all heads' tiles in turn.  (Runs of one head's tiles after the other
+// instead share more of a cache, but start long tiles late: 2 x 8192 causal D 128, 10 heads on 2, forward / backward 458 / 1639 us, in
+// turn 376 / 1310; not causal, 32 x 785 D 64, 6 heads: 65 / 187, 68 / 197.)
+// `level`: all workgroups are on the card at once, nobody comes later to even out what a compute unit got.  An XCD's units then go out to its 32
+// compute units there and back, so that who got the longest of one round gets the shortest of the next (1 x 7000 causal D 80, 15 heads:
+// 206 / 660, with it 178 / 534; 8 x 1440 fp32 D 32, 6 heads on 3: 98 / 314, 80 / 254; where later workgroups even out, it costs: 1 x 4096
+// D 128 with two waves a tile 101, 118).
 struct Unit { int head, tile; };
-__device__ __forceinline__ Unit xcd_unit(int heads, int tiles) {
-  const int x = blockIdx.x & 7, s = blockIdx.x >> 3;
+__device__ __forceinline__ Unit xcd_unit(int heads, int tiles, bool level = false) {
+  const int x = blockIdx.x & 7;
+  int s = blockIdx.x >> 3;
+  if (level && (s & 32)) {
+    const int row = s & ~31;
+    s = row + min(32, (int)(gridDim.x >> 3) - row) - 1 - (s - row);
+  }
   if ((heads & 7) == 0) {
     const int h = heads >> 3;
     return {x * h + s % h, s / h};
@@ -375,8 +387,21 @@ __device__ __forceinline__ Unit xcd_unit(int heads, int tiles) {
     const int h = heads >> 2, t = 2 * (s / h) + (x >> 2);
     return {t < tiles ? (x & 3) * h + s % h : -1, t};
   }
-  const int units = heads * tiles, per = (units + 7) >> 3, u = x * per + s;
-  return {s < per && u < units ? u / tiles : -1, u % tiles};
+  const int u = s * 8 + x;
+  return {u < heads * tiles ? u % heads : -1, u / heads};
+}
+// how many workgroups of a kernel the card holds (found once), and a sixteenth: so many of a grid's last ones own no rows
+static inline long card_holds(const void* f, int threads, size_t lds, long& n) {
+  if (n == 0) {
+    hipFuncAttributes at;
+    if (hipFuncGetAttributes(&at, f) != hipSuccess) {
+      (void)hipGetLastError();
+      return 0;
+    }
+    const long waves = std::min(8, 512 / std::max(8, (at.numRegs + 7) / 8 * 8)) * 4;
+    n = 272 * std::min<long>(163840 / std::max<size_t>(lds + at.sharedSizeBytes, 1), waves * 64 / threads);
+  }
+  return n;
 }
 static inline unsigned xcd_grid(long heads, long tiles) {
   return (unsigned)((heads & 7) == 0 ? heads * tiles : (heads & 3) == 0 ? heads * ((tiles + 1) / 2 * 2) : (heads * tiles + 7) / 8 * 8);

@@ -27,7 +27,7 @@ struct FwdArgs {
   int n_seqs;
   char* out;                           // [T, Hq, D]
   float* stat;                         // NULL, or [2][Hq][T]: see finish()
-  int T, Hq, Hk, D, frame, ntiles;
+  int T, Hq, Hk, D, frame, ntiles, level;
   float c;                             // scale * log2(e)
 };
 
@@ -142,7 +142,7 @@ __global__ __launch_bounds__(256 * H, DT == MVF_F32 && DP > 64 ? H : 2) void pac
   extern __shared__ __attribute__((aligned(256))) char smem[];
   __shared__ int s_span[8 * H];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const Unit u = xcd_unit(a.Hq, a.ntiles);
+  const Unit u = xcd_unit(a.Hq, a.ntiles, a.level);
   if (u.head < 0) return;
   const int head = u.head;
   const OwnTile own = find_tile<128>(a.cu, a.n_seqs, a.T, u.tile, a.ntiles, a.frame == 0 ? Walk::ALL : Walk::LATE);
@@ -290,7 +290,10 @@ int launch_wide(FwdArgs a, hipStream_t st) {
   static uint64_t attr = 0;
   if (int rc = mvf_ensure_lds(reinterpret_cast<const void*>(packed_attn_fwd_kernel<DT, DP, PAD, H>), lds, attr)) return rc;
   a.ntiles = (int)tile_bound<128>(a.T, a.n_seqs);
-  hipLaunchKernelGGL((packed_attn_fwd_kernel<DT, DP, PAD, H>), dim3(xcd_grid(a.Hq, a.ntiles)), dim3(256 * H), lds, st, a);
+  static long holds = 0;
+  const unsigned grid = xcd_grid(a.Hq, a.ntiles);
+  a.level = grid <= card_holds(reinterpret_cast<const void*>(packed_attn_fwd_kernel<DT, DP, PAD, H>), 256 * H, lds, holds);
+  hipLaunchKernelGGL((packed_attn_fwd_kernel<DT, DP, PAD, H>), dim3(grid), dim3(256 * H), lds, st, a);
   return MVF_OK;
 }
 template <int DT, int DP, bool PAD>
@@ -327,6 +330,6 @@ extern "C" int mvf_packed_attn_fwd(int dtype, const void* q, long ldq, long hsq,
   for (long x : s) MVF_CHECK_ARG(x > 0 && x % 16 == 0);
   MVF_CHECK_ARG((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) & 15) == 0);
   FwdArgs a = {(const char*)q, (const char*)k, (const char*)v, s[0], s[1], s[2], s[3], s[4], s[5], cu_seqlens, n_seqs, (char*)out, stat,
-               T, Hq, Hk, D, frame, 0, scale * LOG2E};
+               T, Hq, Hk, D, frame, 0, 0, scale * LOG2E};
   return dtype == MVF_F32 ? launch_d<MVF_F32>(a, st) : dtype == MVF_BF16 ? launch_d<MVF_BF16>(a, st) : launch_d<MVF_F16>(a, st);
 }

@@ -28,7 +28,7 @@ struct BwdArgs {
   float* part;                         // parts > 1: [parts][2 (dk, dv)][T][Hk][D]
   int parts;                           // workgroups that share a group's heads
   char *dq, *dk, *dv;                  // [T, Hq, D], [T, Hk, D] x 2
-  int T, Hq, Hk, D, frame, ntiles;
+  int T, Hq, Hk, D, frame, ntiles, level;
   float c, scale;
 };
 
@@ -178,7 +178,7 @@ __global__ __launch_bounds__(256 * H, DT == MVF_F32 && DP > 32 ? H : 2) void pac
   extern __shared__ __attribute__((aligned(256))) char smem[];
   __shared__ int s_span[8 * H];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const Unit u = xcd_unit(a.Hq, a.ntiles);
+  const Unit u = xcd_unit(a.Hq, a.ntiles, a.level);
   if (u.head < 0) return;
   const int head = u.head;
   const OwnTile own = find_tile<128>(a.cu, a.n_seqs, a.T, u.tile, a.ntiles, a.frame == 0 ? Walk::ALL : Walk::LATE);
@@ -392,7 +392,7 @@ __global__ __launch_bounds__(256 * H, DT == MVF_F32 && DP > 32 ? H : 2) void pac
   extern __shared__ __attribute__((aligned(256))) char smem[];
   __shared__ int s_span[8 * H];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const Unit u = xcd_unit(a.Hk * a.parts, a.ntiles);
+  const Unit u = xcd_unit(a.Hk * a.parts, a.ntiles, a.level);
   if (u.head < 0) return;
   const int kh = u.head / a.parts, part = u.head % a.parts;
   const OwnTile own = find_tile<128>(a.cu, a.n_seqs, a.T, u.tile, a.ntiles, a.frame == 0 ? Walk::ALL : Walk::EARLY);
@@ -545,23 +545,29 @@ int head_parts(long T, long n_seqs, int Hq, int Hk, int dtype) {
 }
 
 template <int DT, int DP, bool PAD, int H>
-int launch_dq(const BwdArgs& a, hipStream_t st) {
+int launch_dq(BwdArgs a, hipStream_t st) {
   typedef Ring<Op<DT>, DP, 3, 4 * H> R;
   constexpr size_t lds = R::NB * R::BUF;
   static_assert(H == 1 || lds >= 4 * HALF<DP>);
   static uint64_t attr = 0;
   if (int rc = mvf_ensure_lds(reinterpret_cast<const void*>(packed_attn_dq_kernel<DT, DP, PAD, H>), lds, attr)) return rc;
-  hipLaunchKernelGGL((packed_attn_dq_kernel<DT, DP, PAD, H>), dim3(xcd_grid(a.Hq, a.ntiles)), dim3(256 * H), lds, st, a);
+  static long holds = 0;
+  const unsigned grid = xcd_grid(a.Hq, a.ntiles);
+  a.level = grid <= card_holds(reinterpret_cast<const void*>(packed_attn_dq_kernel<DT, DP, PAD, H>), 256 * H, lds, holds);
+  hipLaunchKernelGGL((packed_attn_dq_kernel<DT, DP, PAD, H>), dim3(grid), dim3(256 * H), lds, st, a);
   return MVF_OK;
 }
 template <int DT, int DP, bool PAD, int H>
-int launch_dkv(const BwdArgs& a, hipStream_t st) {
+int launch_dkv(BwdArgs a, hipStream_t st) {
   typedef DkvRing<DT, DP, H> R;
   constexpr size_t lds = R::NB * (R::BUF + (planes(DT) * R::KB + 63) / 64 * 256) + (V_IN_LDS<DT, DP> ? 128 * Img<Op<DT>, DP>::RB : 0);
   static_assert(H == 1 || lds >= 4 * HALF<DP>);
   static uint64_t attr = 0;
   if (int rc = mvf_ensure_lds(reinterpret_cast<const void*>(packed_attn_dkv_kernel<DT, DP, PAD, H>), lds, attr)) return rc;
-  hipLaunchKernelGGL((packed_attn_dkv_kernel<DT, DP, PAD, H>), dim3(xcd_grid((long)a.Hk * a.parts, a.ntiles)), dim3(256 * H), lds, st, a);
+  static long holds = 0;
+  const unsigned grid = xcd_grid((long)a.Hk * a.parts, a.ntiles);
+  a.level = grid <= card_holds(reinterpret_cast<const void*>(packed_attn_dkv_kernel<DT, DP, PAD, H>), 256 * H, lds, holds);
+  hipLaunchKernelGGL((packed_attn_dkv_kernel<DT, DP, PAD, H>), dim3(grid), dim3(256 * H), lds, st, a);
   return MVF_OK;
 }
 template <int DT, int DP, bool PAD>
@@ -631,6 +637,7 @@ extern "C" int mvf_packed_attn_bwd(int dtype, const void* q, long ldq, long hsq,
   const int parts = head_parts(T, n_seqs, Hq, Hk, dtype);
   MVF_CHECK_ARG(tile_bound<32>(T, n_seqs) * Hk * parts < (1l << 30) && (size_t)T * Hk * D / 512 < (1ul << 31));
   BwdArgs a = {(const char*)q, (const char*)k, (const char*)v, s[0], s[1], s[2], s[3], s[4], s[5], cu_seqlens, n_seqs, (const char*)out,
-               (const char*)d_out, stat, delta, delta + ((size_t)Hq * T + 3) / 4 * 4, parts, (char*)dq, (char*)dk, (char*)dv, T, Hq, Hk, D, frame, 0, scale * LOG2E, scale};
+               (const char*)d_out, stat, delta, delta + ((size_t)Hq * T + 3) / 4 * 4, parts, (char*)dq, (char*)dk, (char*)dv, T, Hq, Hk, D,
+               frame, 0, 0, scale * LOG2E, scale};
   return dtype == MVF_F32 ? launch_d<MVF_F32>(a, st) : dtype == MVF_BF16 ? launch_d<MVF_BF16>(a, st) : launch_d<MVF_F16>(a, st);
 }
