@@ -60,13 +60,15 @@ struct Line {                                    // by one whole wave
 #pragma unroll 1
     for (int b = 64; b < a.B; b += 64) total += __builtin_amdgcn_readlane(scan(of(a, length(a, b + lane)), lane), 63);
   }
-  // the unit that place `pos` of the line lies in (pos < total * units of a stream)
+  // the unit that place `pos` of the line lies in (pos < total * units of a stream; length 0: there is none, so the lengths were changed
+  // while this ran, which must not keep it here)
   __device__ __forceinline__ Piece find(const PagedArgs& a, int pos) const {
     const int per = a.Hk * a.rt, p = pos / per;
     int x = len, s = sum, base = 0, b0 = 0;
     uint64_t m = __builtin_amdgcn_ballot_w64(s > p);
 #pragma unroll 1
     while (m == 0) {
+      if (b0 >= a.B) return {0, 0, 0, 0};
       base += __builtin_amdgcn_readlane(s, 63);
       b0 += 64;
       x = length(a, b0 + lane);
@@ -74,7 +76,7 @@ struct Line {                                    // by one whole wave
       m = __builtin_amdgcn_ballot_w64(base + s > p);
     }
     const int j = __builtin_ctzll(m), l = __builtin_amdgcn_readlane(x, j), w = of(a, l);
-    const int s0 = (base + __builtin_amdgcn_readlane(s, j) - w) * per, unit = (pos - s0) / w;
+    const int s0 = (base + __builtin_amdgcn_readlane(s, j) - w) * per, unit = max((pos - s0) / w, 0);
     return {b0 + j, unit, l, s0 + unit * w};
   }
 };
@@ -285,6 +287,7 @@ __global__ __launch_bounds__(64 * NW, 1) void paged_attn_kernel(PagedArgs a) {
 #pragma unroll 1
     for (int pos = blockIdx.x * per; pos < end;) {
       const Piece u = line.find(a, pos);
+      if (u.len == 0) break;
       const int n = rounds_of(u.len), first = u.start + a.extra;       // place of the first round
       const int r0 = max(pos - first, 0), r1 = min(end - first, n);
       if (r1 > r0) {

@@ -420,8 +420,8 @@ static inline bool long_walks(long T, long n_seqs) { return T >= 512 * n_seqs; }
 // is half as long and a block half as many barriers, for an unchanged amount of work: it pays where few, long and unequal walks fill the
 // compute units once, at rows of 256 bytes.  Measured, us, forward / backward with one and two waves a row tile, causal: 1 x 2048 bf16 D 128
 // 16 heads on 4: 60 / 195, 45 / 153; 1 x 4096: 117 / 380, 94 / 320; 2 x 2048: 63 / 211, 55 / 195; 4 x 2048 fp32 D 64 8 heads: 210 / 633,
-// 158 / 529; 2 x 1600 50 / 170, 44 / 150; but 3 x 1300, 560 workgroups: 48 / 168, 57 / 183; 1 x 6000, 800 workgroups: forward 193, 191; not causal, 4 x 2048 8 heads D 128: 82, 90; shorter rows, 2 x 4096 D 96 12
-// heads: 108, 115.
+// 158 / 529; 2 x 1600: 50 / 170, 44 / 150; but 3 x 1300, 560 workgroups: 48 / 168, 57 / 183; 1 x 6000, 800 workgroups: forward 193, 191;
+// not causal, 4 x 2048 8 heads D 128: 82, 90; shorter rows, 2 x 4096 D 96 12 heads: 108, 115.
 template <class O, int DP>
 constexpr bool PAIRS = DP * O::SZ == 256;
 template <int DP>
