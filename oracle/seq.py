@@ -39,17 +39,18 @@ def limit(p, frame, length):
     return length if frame == 0 else max(0, min(length, (p // frame + 1) * frame))
 
 
-def attend(q, k, v, limits, scale, dtype, do=None):
+def attend(q, k, v, limits, scale, dtype, do=None, low=False):
     """One head: q [n, D], k, v [L, D], limits [n] keys seen by each row; do [n, D].  -> dict of 64-bit results and of bounds.
 
     The bounds follow the kernels' roundings.  A score is a 32-bit sum of D products (at most D / 8 + 8 dependent additions); the exponent
     and its power of two round a few times more; so a probability is off by 2 * es relative (numerator and denominator), es the
     score's absolute error + 8 steps.  Probabilities and dS round once to a 16-bit operand (up).  A sum over n terms is off by at most
-    (n / 16 + 40) steps of 32 bits of the sum of magnitudes.  delta reads the stored, rounded output."""
+    (n / 16 + 40) steps of 32 bits of the sum of magnitudes.  delta reads the stored, rounded output.  low: a probability enters its
+    product as the 16-bit operand and the rounded rest (at most up of it, so the two are off by up * up)."""
     q, k, v = (t.detach().double().cpu() for t in (q, k, v))
     n, L, D = q.shape[0], k.shape[0], q.shape[1]
     u = HALF_STEP[dtype]
-    up, tiny = (0.0, 0.0) if dtype == torch.float32 else (u, TINY[dtype])
+    up, tiny = (0.0, 0.0) if dtype == torch.float32 else (u * u if low else u, TINY[dtype])
     seen = torch.arange(L)[None] < torch.as_tensor(limits)[:, None]
     if L == 0:
         z = torch.zeros(n, D, dtype=torch.float64)
@@ -115,8 +116,8 @@ def packed(q, k, v, cu, frame, scale=None, do=None):
     return r
 
 
-def paged(q, k_cache, v_cache, table, lengths, frame, scale=None):
-    """q [B, n, Hq, D] against the pages: (out, bound) [B, n, Hq, D].  A page outside the cache holds no keys."""
+def paged(q, k_cache, v_cache, table, lengths, frame, scale=None, low=False):
+    """q [B, n, Hq, D] against the pages: (out, bound) [B, n, Hq, D].  A page outside the cache holds no keys.  low: as in attend()."""
     B, n, Hq, D = q.shape
     pages, page, Hk = k_cache.shape[:3]
     g, scale = Hq // Hk, D ** -0.5 if scale is None else scale
@@ -128,6 +129,6 @@ def paged(q, k_cache, v_cache, table, lengths, frame, scale=None):
         pg, row = [x[0] for x in at], [x[1] for x in at]
         limits = [sum(1 for x in at if x[2] < limit(length - n + i, frame, length)) for i in range(n)]
         for h in range(Hq):
-            one = attend(q[b, :, h], k_cache[pg, row, h // g], v_cache[pg, row, h // g], limits, scale, q.dtype)
+            one = attend(q[b, :, h], k_cache[pg, row, h // g], v_cache[pg, row, h // g], limits, scale, q.dtype, low=low)
             out[b, :, h], bound[b, :, h] = one['out'], one['out_b']
     return out, bound

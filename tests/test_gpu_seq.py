@@ -421,6 +421,15 @@ def test_paged_attention_hides_later_new_tokens(dtype):
     assert torch.isnan(out[:, 2]).all()
 
 
+@pytest.mark.parametrize('dtype', DTYPES[1:], ids=IDS[1:])
+@pytest.mark.parametrize('lengths,new,page,hq,hk,d,frame', [PAGED[2], PAGED[4], PAGED[5], PAGED[6], PAGED[7], PAGED[11]])
+def test_paged_attention_rounds_once(dtype, lengths, new, page, hq, hk, d, frame):
+    """16-bit results are the one rounding of a 32-bit sum: the weights lose no bits that count on the way into their product."""
+    q, kc, vc, table, lens = make_paged(lengths, new, page, hq, hk, d, dtype, 110)
+    want, bound = OS.paged(q, kc, vc, table, lens, frame, low=True)
+    within(ops.paged_attention(q, kc, vc, table, lens, frame=frame), want, bound, 'out')
+
+
 def test_paged_attention_far_pages():
     """Pages behind 2^31 elements of the cache, written by rotary_append and read back."""
     page, hk, d = 64, 8, 128

@@ -15,6 +15,11 @@ using namespace seq_attn;
 
 constexpr int NW = 4;                  // waves per workgroup
 constexpr int MAX_GROUPS = 512;        // workgroups that share a call's work
+// The weights of 16-bit tensors enter the second product as two operands, the rounded weight and the rounded rest: the matrix pipe waits for
+// keys most of the time anyway (12 streams of 32768 bf16: 302 us a call, with one operand 301; 64 of 1 to 4096 fp16: 25.4, 25.0), and the
+// result is one rounding of the 32-bit sum (bf16 1.7e-3 of its size, with one operand 2.3e-3; fp16 1.8e-4, 2.0e-4).
+template <class O>
+constexpr bool LOW = O::SZ == 2;
 
 struct PagedArgs {
   const char* q;                       // [B, n, Hq, D], strides in BYTES
@@ -184,7 +189,7 @@ __device__ __forceinline__ void walk_unit(const PagedArgs& a, const Piece& u, in
       s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.c, st.nm));
       st.l += s[e];
     }
-    accumulate<O, DP>(o, s, cl);
+    accumulate<O, DP, LOW<O>>(o, s, cl);
   };
 
   // Per tile: its page ids are asked for two tiles ahead, its rows one tile ahead (where the buffers allow two tiles).

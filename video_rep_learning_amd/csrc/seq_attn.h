@@ -58,6 +58,13 @@ struct Op16 {
     for (int j = 0; j < 4; ++j) f.u[j] = pack16x2<F16>(x[8 * s + 2 * j], x[8 * s + 2 * j + 1]);
     return f.v;
   }
+  // what pack() rounded away (exact in 32 bits), rounded in turn
+  static __device__ __forceinline__ Frag pack_rest(const f32x16_t& x, const Frag& b, int s) {
+    union { Frag v; uint32_t u[4]; } f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f.u[j] = pack16x2<F16>(x[8 * s + 2 * j] - get(b, 2 * j), x[8 * s + 2 * j + 1] - get(b, 2 * j + 1));
+    return f.v;
+  }
   // a 16-byte chunk holds a NaN or an infinity: an all-ones exponent carries into the sign bit
   static __device__ __forceinline__ bool nonfinite(const u32x4_t& x) {
     constexpr uint32_t EXP = F16 ? 0x7c007c00u : 0x7f807f80u, ONE = F16 ? 0x04000400u : 0x00800080u;
@@ -189,13 +196,20 @@ struct Img {
 // places, but 0 * NaN is NaN: through the product a NaN or infinity of a row would reach the columns that must not see it.  So in
 // tiles with masked places the kernels look for non-finite values, and a wave that met one goes over its rows again, element by
 // element and visible pairs only (their slow()), after the loop.
-template <class O, int DP>
+// LOW: what the rounding of w to the operands' 16 bits left over goes through a second product, so that w counts with 16 bits and more.
+template <class O, int DP, bool LOW = false>
 __device__ __forceinline__ void accumulate(f32x16_t (&acc)[DP / 32], const f32x16_t& w, uint32_t lane) {
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
     const typename O::Frag b = O::pack(w, s);
+    typename O::Frag low;
+    if constexpr (LOW) low = O::pack_rest(w, b, s);
 #pragma unroll
-    for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = O::mma(Img<O, DP>::cols(lane, s, dt), b, acc[dt]);
+    for (int dt = 0; dt < DP / 32; ++dt) {
+      const typename O::Frag x = Img<O, DP>::cols(lane, s, dt);
+      acc[dt] = O::mma(x, b, acc[dt]);
+      if constexpr (LOW) acc[dt] = O::mma(x, low, acc[dt]);
+    }
   }
 }
 template <class O, int DP>
