@@ -311,6 +311,33 @@ def test_packed_attention_other_strides(dtype):
     within(g[:, 0], want['dk'].sum(1), want['dk_b'].sum(1) + OS.U32 * want['dk'].abs().sum(1), 'broadcast key')
 
 
+@pytest.mark.parametrize('dtype', DTYPES, ids=IDS)
+@pytest.mark.parametrize('t,h,d', [(1, 8, 32), (5, 1, 32), (1, 1, 8)])
+def test_one_token_or_one_head_in_any_memory_order(dtype, t, h, d):
+    """A dimension of size 1 may have any stride (channels first, narrow slices): the same bits as from a tensor of its own."""
+    qkv = [randn(t, h, d, dtype=dtype, seed=95 + i) for i in range(3)]
+    pos, freqs, cu = positions(t, 1, torch.int64, 3, 98), ops.rotary_freqs((d // 2,)), cu_tensor([0, t])
+    table, n = torch.tensor([[1, 0, 2]], dtype=torch.int32, device=DEV), torch.tensor([t], device=DEV)
+    seq, index = torch.zeros(t, dtype=torch.int32, device=DEV), torch.arange(t, dtype=torch.int32, device=DEV)
+
+    def all_of_them(q, k, v):
+        q, k, v = (x.detach().requires_grad_() for x in (q, k, v))
+        a, b = ops.rotary(q, k, pos, freqs, (d // 2,))
+        got = [a, b, *torch.autograd.grad((a, b), (q, k), (v, q))]
+        got += run_packed(q, k, v, cu, 1, v.detach())
+        with torch.no_grad():
+            kc, vc = make_cache(3, 2, h, d, dtype, 99)
+            got += [ops.rotary_append(q, k, v, pos, freqs, (d // 2,), kc, vc, table, seq, index), kc, vc]
+            got += [ops.paged_attention(q[None], kc, vc, table, n), ops.paged_attention(q[:, None], kc, vc, table.expand(t, 3), n.expand(t))]
+        return got
+    want = all_of_them(*qkv)
+    for order in ((2, 0, 1), (0, 2, 1), (1, 2, 0)):
+        xs = [x.permute(order).contiguous().permute([order.index(i) for i in range(3)]) for x in qkv]
+        assert all(torch.equal(a, b) for a, b in zip(want, all_of_them(*xs)))
+    xs = [torch.cat([x, x[..., :4]], 2)[..., :d] for x in qkv]
+    assert all(torch.equal(a, b) for a, b in zip(want, all_of_them(*xs)))
+
+
 def test_packed_attention_nothing_to_do():
     z = torch.zeros(0, 2, 32, device=DEV).requires_grad_()
     out = ops.packed_attention(z, z, z, cu_tensor([0, 0]), frame=1)

@@ -98,6 +98,17 @@ def test_aligned_copies_only_what_it_must():
         assert z.data_ptr() != y.data_ptr() and z.data_ptr() % 16 == 0 and z.is_contiguous() and torch.equal(z, y)
 
 
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16, torch.float16])
+def test_aligned_gives_dimensions_of_size_one_strides_of_their_own(dtype):
+    """torch calls these contiguous whatever stride the dimension of size 1 has: one token held channels first, one head, a narrow slice."""
+    for y in (torch.randn(8, 32, 1).to(dtype).permute(2, 0, 1), torch.randn(4, 32, 1).to(dtype).transpose(1, 2),
+              torch.randn(1, 1, 12 if dtype != torch.float32 else 10).to(dtype)[..., :8], torch.randn(1, 1, 8).to(dtype).expand(1, 1, 8),
+              torch.randn(1, 8, 32, 1).to(dtype).permute(0, 3, 1, 2), torch.randn(2, 5, 16, 1).to(dtype).transpose(2, 3)):
+        z = ops._aligned(y)
+        a = 16 // y.element_size()
+        assert torch.equal(z, y) and z.data_ptr() % 16 == 0 and z.stride(-1) == 1 and all(s > 0 and s % a == 0 for s in z.stride()[:-1])
+
+
 FWD = dict(dtype=_lib.BF16, q=P, ldq=64, hsq=32, k=P, ldk=64, hsk=32, v=P, ldv=64, hsv=32, cu=P, n=1, out=P, stat=None, T=4, Hq=2, Hk=2, D=32,
            frame=1, scale=1.0)
 BAD_ATTN = [('dtype', 2), ('q', None), ('q', P + 8), ('k', None), ('v', None), ('cu', None), ('out', None), ('out', P + 4), ('ldq', 0), ('ldq', 63),

@@ -2229,8 +2229,7 @@ def _aligned(t):
         bad = bad or s <= 0 or s & a
     if not bad:
         return t
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+    return torch.empty(t.shape, device=t.device, dtype=t.dtype).copy_(t)    # (contiguous() keeps any stride of a dimension of size 1)
 
 
 def _heads(t, what, tokens=None, size=None):
