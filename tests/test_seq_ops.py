@@ -109,6 +109,41 @@ def test_aligned_gives_dimensions_of_size_one_strides_of_their_own(dtype):
         assert torch.equal(z, y) and z.data_ptr() % 16 == 0 and z.stride(-1) == 1 and all(s > 0 and s % a == 0 for s in z.stride()[:-1])
 
 
+@pytest.fixture
+def on_cpu(monkeypatch):
+    """The operators' Python side on CPU tensors: no device check; a launch leaves its results as they were allocated."""
+    monkeypatch.setattr(ops, '_seq_operands', lambda first, *others: ops._SEQ_DT[first.dtype])
+    return monkeypatch
+
+
+def calls(grad):
+    q, k, v = (torch.randn(4, 2, 32, requires_grad=grad) for _ in range(3))
+    pos, freqs, cu = torch.zeros(4, 1, dtype=torch.int64), ops.rotary_freqs((16,), device='cpu'), torch.tensor([0, 4], dtype=torch.int32)
+    kc, vc, table, i = torch.zeros(2, 4, 2, 32), torch.zeros(2, 4, 2, 32), torch.zeros(1, 2, dtype=torch.int32), torch.zeros(4, dtype=torch.int32)
+    return (q, k, v), {
+        'rotary': lambda q, k, v: ops.rotary(q, k, pos, freqs, (16,))[0],
+        'rotary, keys': lambda q, k, v: ops.rotary(q.detach(), k, pos, freqs, (16,))[1],
+        'packed_attention': lambda q, k, v: ops.packed_attention(q, k, v, cu),
+        'rotary_append': lambda q, k, v: ops.rotary_append(q, k, v, pos, freqs, (16,), kc, vc, table, i, i),
+        'paged_attention': lambda q, k, v: ops.paged_attention(q[None], kc, vc, table, cu[1:])}
+
+
+@pytest.mark.parametrize('which', range(3))
+def test_forward_mode_derivatives_are_refused(on_cpu, which):
+    """A dual operand has no requires_grad; its tangent must not be dropped without a word."""
+    on_cpu.setattr(ops, '_launch', lambda *a: None)
+    xs, fns = calls(False)
+    for name, fn in fns.items():
+        if name == 'rotary' and which != 0 or name == 'rotary, keys' and which != 1 or name == 'paged_attention' and which != 0:
+            continue
+        for mode in (True, False):
+            with torch.set_grad_enabled(mode), torch.autograd.forward_ad.dual_level():
+                dual = [torch.autograd.forward_ad.make_dual(x, torch.ones_like(x)) if i == which else x for i, x in enumerate(xs)]
+                with pytest.raises((NotImplementedError, ValueError)):
+                    fn(*dual)
+                fn(*xs)                                 # an open level alone changes nothing
+
+
 FWD = dict(dtype=_lib.BF16, q=P, ldq=64, hsq=32, k=P, ldk=64, hsk=32, v=P, ldv=64, hsv=32, cu=P, n=1, out=P, stat=None, T=4, Hq=2, Hk=2, D=32,
            frame=1, scale=1.0)
 BAD_ATTN = [('dtype', 2), ('q', None), ('q', P + 8), ('k', None), ('v', None), ('cu', None), ('out', None), ('out', P + 4), ('ldq', 0), ('ldq', 63),

@@ -10,6 +10,7 @@ import ctypes
 
 import torch
 import torch.distributed as dist
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -2255,6 +2256,16 @@ def _scale_arg(scale, d):
     return scale
 
 
+def _tracked(*operands):
+    """Some operand carries a derivative: it wants a gradient, or a level of forward-mode derivatives is open (whose tangents show in
+    nothing but the operand itself)."""
+    dual, grad = forward_ad._current_level >= 0, torch.is_grad_enabled()
+    for t in operands:
+        if grad and t.requires_grad or dual and forward_ad.unpack_dual(t).tangent is not None:
+            return True
+    return False
+
+
 def _launch(name, like, *args):
     """call() on the current stream of the operands' device, whichever device is current."""
     dev = like.get_device()
@@ -2328,7 +2339,7 @@ def rotary(q, k, pos, freqs, sections, interleaved=False):
     else:
         _seq_operands(q)
     pos, freqs, sections = _rotary_args(pos, freqs, sections, q.shape[0], q.shape[2], q)
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+    if _tracked(q) or (k is not None and _tracked(k)):
         return _Rotary.apply(q, k, pos, freqs, sections, bool(interleaved))
     return _rotary_call(q, k, pos, freqs, sections, bool(interleaved), False)
 
@@ -2353,7 +2364,7 @@ def rotary_append(q, k, v, pos, freqs, sections, k_cache, v_cache, block_table, 
     _heads(k, 'k', q.shape[0], q.shape[2])
     _heads(v, 'v', q.shape[0], q.shape[2])
     code = _seq_operands(q, k, v, k_cache, v_cache)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    if _tracked(q, k, v):
         raise ValueError('rotary_append has no gradient: call it under torch.no_grad()')
     _cache_args(q, k_cache, v_cache)
     if k.shape[1] != k_cache.shape[2] or v.shape[1] != k_cache.shape[2]:
@@ -2436,7 +2447,7 @@ def packed_attention(q, k, v, cu_seqlens, frame=0, scale=None):
     if cu.shape[0] < 2:
         raise ValueError('cu_seqlens needs the bounds of at least one sequence, got %s' % (tuple(cu.shape),))
     frame, scale = _frame_arg(frame), _scale_arg(scale, q.shape[2])
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    if _tracked(q, k, v):
         return _PackedAttention.apply(q, k, v, cu, frame, scale)
     return _packed_fwd(_aligned(q), _aligned(k), _aligned(v), cu, frame, scale, False)[0]
 
@@ -2449,7 +2460,7 @@ def paged_attention(q, k_cache, v_cache, block_table, lengths, frame=1, scale=No
     if q.dim() != 4 or 0 in q.shape[1:] or q.shape[3] % 8 or q.shape[3] > 128:
         raise ValueError('q: expected [streams, new tokens, heads, head size (a multiple of 8 up to 128)], got %s' % (tuple(q.shape),))
     code = _seq_operands(q, k_cache, v_cache)
-    if torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad):
+    if _tracked(q, k_cache, v_cache):
         raise ValueError('paged_attention has no gradient: call it under torch.no_grad()')
     _cache_args(q, k_cache, v_cache)
     B, n, Hq, D = q.shape
