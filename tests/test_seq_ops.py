@@ -144,6 +144,19 @@ def test_forward_mode_derivatives_are_refused(on_cpu, which):
                 fn(*xs)                                 # an open level alone changes nothing
 
 
+@pytest.mark.filterwarnings('ignore::torch.jit.TracerWarning')
+@pytest.mark.parametrize('name', ['rotary', 'rotary, keys', 'packed_attention', 'rotary_append', 'paged_attention'])
+def test_tracing_is_refused(on_cpu, name):
+    """A trace would hold the allocation of the results only."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    for grad in (False, True):
+        xs, fns = calls(grad and not name.startswith(('rotary_append', 'paged')))
+        with pytest.raises(_lib.MvfError):
+            torch.jit.trace(fns[name], xs)
+        with pytest.raises(_lib.MvfError):
+            make_fx(fns[name])(*xs)
+
+
 FWD = dict(dtype=_lib.BF16, q=P, ldq=64, hsq=32, k=P, ldk=64, hsk=32, v=P, ldv=64, hsv=32, cu=P, n=1, out=P, stat=None, T=4, Hq=2, Hk=2, D=32,
            frame=1, scale=1.0)
 BAD_ATTN = [('dtype', 2), ('q', None), ('q', P + 8), ('k', None), ('v', None), ('cu', None), ('out', None), ('out', P + 4), ('ldq', 0), ('ldq', 63),

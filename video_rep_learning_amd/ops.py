@@ -2268,6 +2268,10 @@ def _tracked(*operands):
 
 def _launch(name, like, *args):
     """call() on the current stream of the operands' device, whichever device is current."""
+    # a tracer (torch.jit.trace, make_fx) records the allocation of the results and nothing of what fills them
+    if torch._C._get_tracing_state() is not None or (torch._C._len_torch_dispatch_stack() and
+                                                     torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None):
+        raise _lib.MvfError('%s cannot be traced: a trace would return memory that nothing has written' % name)
     dev = like.get_device()
     if dev == torch.cuda.current_device():
         call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
