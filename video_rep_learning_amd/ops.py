@@ -2368,7 +2368,7 @@ def rotary_append(q, k, v, pos, freqs, sections, k_cache, v_cache, block_table, 
     _heads(k, 'k', q.shape[0], q.shape[2])
     _heads(v, 'v', q.shape[0], q.shape[2])
     code = _seq_operands(q, k, v, k_cache, v_cache)
-    if _tracked(q, k, v):
+    if _tracked(q, k, v, k_cache, v_cache):
         raise ValueError('rotary_append has no gradient: call it under torch.no_grad()')
     _cache_args(q, k_cache, v_cache)
     if k.shape[1] != k_cache.shape[2] or v.shape[1] != k_cache.shape[2]:
