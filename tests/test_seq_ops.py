@@ -170,6 +170,20 @@ def test_append_refuses_caches_that_want_a_gradient(on_cpu, which):
         ops.rotary_append(*args[:5], (16,), *args[5:], *rest)
 
 
+def test_append_tells_autograd_that_the_caches_changed(on_cpu):
+    """A graph that saved a cache refuses to run backward over other values than it saw."""
+    on_cpu.setattr(ops, '_launch', lambda *a: None)
+    q, pos, i = heads(), torch.zeros(4, 1, dtype=torch.int64), torch.zeros(4, dtype=torch.int32)
+    freqs, kc, vc = ops.rotary_freqs((16,), device='cpu'), torch.zeros(2, 4, 2, 32), torch.zeros(2, 4, 2, 32)
+    for cache in (kc, vc):
+        w = torch.ones(32, requires_grad=True)
+        y = (cache * w).sum()
+        with torch.no_grad():
+            ops.rotary_append(q, q, q, pos, freqs, (16,), kc, vc, torch.zeros(1, 2, dtype=torch.int32), i, i)
+        with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+            y.backward()
+
+
 FWD = dict(dtype=_lib.BF16, q=P, ldq=64, hsq=32, k=P, ldk=64, hsk=32, v=P, ldv=64, hsv=32, cu=P, n=1, out=P, stat=None, T=4, Hq=2, Hk=2, D=32,
            frame=1, scale=1.0)
 BAD_ATTN = [('dtype', 2), ('q', None), ('q', P + 8), ('k', None), ('v', None), ('cu', None), ('out', None), ('out', P + 4), ('ldq', 0), ('ldq', 63),

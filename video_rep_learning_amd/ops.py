@@ -12,6 +12,7 @@ import torch
 import torch.distributed as dist
 from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
+from torch.autograd.graph import increment_version
 
 from . import _lib
 from ._lib import call, ptr, stream, F32, BF16, FP8, F16
@@ -2389,6 +2390,7 @@ def rotary_append(q, k, v, pos, freqs, sections, k_cache, v_cache, block_table, 
             pos.data_ptr(), _POS_DT[pos.dtype], freqs.data_ptr(), *sections, bool(interleaved), qo.data_ptr(), k_cache.data_ptr(),
             v_cache.data_ptr(), table.data_ptr(), table.shape[1], table.shape[0], seq.data_ptr(), index.data_ptr(), k_cache.shape[0],
             k_cache.shape[1], T, Hq, k.shape[1], D)
+    increment_version((k_cache, v_cache))           # what autograd keeps of them is out of date
     return qo
 
 
