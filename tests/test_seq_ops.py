@@ -184,6 +184,19 @@ def test_append_tells_autograd_that_the_caches_changed(on_cpu):
             y.backward()
 
 
+def test_rotary_refuses_angles_that_want_a_gradient(on_cpu):
+    on_cpu.setattr(ops, '_launch', lambda *a: None)
+    q, pos, freqs = heads(), torch.zeros(4, 1), ops.rotary_freqs((16,), device='cpu')
+    for p, f in ((pos.clone().requires_grad_(), freqs), (pos, freqs.clone().requires_grad_())):
+        for x in (q, q.clone().requires_grad_()):
+            with pytest.raises(ValueError, match='no gradient'):
+                ops.rotary(x, x, p, f, (16,))
+        with torch.no_grad():
+            ops.rotary(q, q, p, f, (16,))
+    with torch.autograd.forward_ad.dual_level(), pytest.raises(ValueError, match='no gradient'):
+        ops.rotary(q, q, pos, torch.autograd.forward_ad.make_dual(freqs, torch.ones_like(freqs)), (16,))
+
+
 FWD = dict(dtype=_lib.BF16, q=P, ldq=64, hsq=32, k=P, ldk=64, hsk=32, v=P, ldv=64, hsv=32, cu=P, n=1, out=P, stat=None, T=4, Hq=2, Hk=2, D=32,
            frame=1, scale=1.0)
 BAD_ATTN = [('dtype', 2), ('q', None), ('q', P + 8), ('k', None), ('v', None), ('cu', None), ('out', None), ('out', P + 4), ('ldq', 0), ('ldq', 63),

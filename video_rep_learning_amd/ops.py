@@ -2296,6 +2296,8 @@ def _rotary_args(pos, freqs, sections, tokens, size, like):
         raise ValueError('pos: expected [%d, %d] of int32, int64 or float32, got %s %s' % (tokens, len(sections), tuple(pos.shape), pos.dtype))
     if freqs.dtype != torch.float64 or tuple(freqs.shape) != (sum(sections),):
         raise ValueError('freqs: expected [%d] float64, got %s %s' % (sum(sections), tuple(freqs.shape), freqs.dtype))
+    if _tracked(pos, freqs):
+        raise ValueError('pos and freqs have no gradient: detach() them')
     return pos.contiguous(), freqs.contiguous(), sections + (0, 0, 0)[len(sections):]
 
 
@@ -2336,7 +2338,8 @@ def rotary(q, k, pos, freqs, sections, interleaved=False):
     """Rotary positions with one to three axes (time, row, column; or time, entity): q [T, Hq, D], k [T, Hk, D] (or None) turned by
     pos[t, axis] * freqs[pair] -> new (q, k).  `sections`: pairs of each axis, in the order of pos's columns; channels behind
     2 * sum(sections) stay.  interleaved: a pair is two neighbouring channels, otherwise channels p and p + sum(sections).  pos [T, axes]
-    int32 / int64 / float32; freqs: rotary_freqs(sections).  fp32, bf16 or fp16; differentiable (once) in q and k."""
+    int32 / int64 / float32; freqs: rotary_freqs(sections).  fp32, bf16 or fp16; differentiable (once) in q and k, not in pos and freqs
+    (refused if they ask for it)."""
     _heads(q, 'q')
     if k is not None:
         _heads(k, 'k', q.shape[0], q.shape[2])
