@@ -197,6 +197,34 @@ def test_rotary_refuses_angles_that_want_a_gradient(on_cpu):
         ops.rotary(q, q, pos, torch.autograd.forward_ad.make_dual(freqs, torch.ones_like(freqs)), (16,))
 
 
+def test_append_refuses_memory_that_it_would_read_and_write(on_cpu):
+    on_cpu.setattr(ops, '_launch', lambda *a: None)
+    pos, freqs, i = torch.zeros(4, 1, dtype=torch.int64), ops.rotary_freqs((16,), device='cpu'), torch.zeros(4, dtype=torch.int32)
+    table, n = torch.zeros(1, 2, dtype=torch.int32), 2 * 4 * 2 * 32
+    pool = torch.zeros(4 * n)
+
+    def cache(at):
+        return pool[at:at + n].view(2, 4, 2, 32)
+
+    def rows(at):
+        return pool[at:].as_strided((4, 2, 32), (64, 32, 1))
+
+    def append(q, k, v, kc, vc):
+        return ops.rotary_append(q, k, v, pos, freqs, (16,), kc, vc, table, i, i)
+    x = torch.zeros(4, 2, 32)
+    append(x, x, x, cache(0), cache(n))                                   # neighbours
+    append(rows(2 * n), rows(2 * n), rows(2 * n + 256), cache(n), cache(0))
+    for off in (0, 4, n // 2, n - 4):
+        with pytest.raises(ValueError, match='share memory'):
+            append(x, x, x, cache(off), cache(0))
+        with pytest.raises(ValueError, match='share memory'):
+            append(x, x, x, cache(0), cache(off))
+    for bad in (rows(0), rows(2 * n - 64), rows(n + 64)):
+        for at in range(3):
+            with pytest.raises(ValueError, match='memory of a cache'):
+                append(*(bad if j == at else x for j in range(3)), cache(0), cache(n))
+
+
 FWD = dict(dtype=_lib.BF16, q=P, ldq=64, hsq=32, k=P, ldk=64, hsk=32, v=P, ldv=64, hsv=32, cu=P, n=1, out=P, stat=None, T=4, Hq=2, Hk=2, D=32,
            frame=1, scale=1.0)
 BAD_ATTN = [('dtype', 2), ('q', None), ('q', P + 8), ('k', None), ('v', None), ('cu', None), ('out', None), ('out', P + 4), ('ldq', 0), ('ldq', 63),

@@ -2367,7 +2367,7 @@ def rotary_append(q, k, v, pos, freqs, sections, k_cache, v_cache, block_table, 
     """rotary() for new tokens of streams with a paged cache: returns the turned q; the turned k and v go into k_cache, v_cache
     [pages, page, Hk, D] at index[t] of stream seq[t], i.e. row index % page of page block_table[seq, index // page].  A token whose seq
     (-1: padding), index or page lies outside is not written; two tokens of one call must not have the same slot (it would hold a mixture of
-    them).  For inference: no gradient."""
+    them).  The caches share no memory with each other or with q, k, v.  For inference: no gradient."""
     _heads(q, 'q')
     _heads(k, 'k', q.shape[0], q.shape[2])
     _heads(v, 'v', q.shape[0], q.shape[2])
@@ -2387,8 +2387,14 @@ def rotary_append(q, k, v, pos, freqs, sections, k_cache, v_cache, block_table, 
         return qo
     if 0 in table.shape or max(table.shape) >= 2 ** 31:
         raise ValueError('block_table is empty or too large: %s' % (tuple(table.shape),))
-    if k_cache.data_ptr() == v_cache.data_ptr():
-        raise ValueError('k_cache and v_cache are the same memory')
+    kc, vc, size, width = k_cache.data_ptr(), v_cache.data_ptr(), k_cache.numel() * q.element_size(), q.element_size()
+    if abs(kc - vc) < size:
+        raise ValueError('k_cache and v_cache share memory')
+    for t in (q, k, v):
+        lo, (ld, hs, _) = t.data_ptr(), t.stride()
+        hi = lo + ((T - 1) * ld + (t.shape[1] - 1) * hs + D) * width
+        if lo < kc + size and hi > kc or lo < vc + size and hi > vc:
+            raise ValueError('an operand lies in the memory of a cache, which is written while it is read')
     _launch('mvf_rotary_append', q, code, q.data_ptr(), *q.stride()[:2], k.data_ptr(), *k.stride()[:2], v.data_ptr(), *v.stride()[:2],
             pos.data_ptr(), _POS_DT[pos.dtype], freqs.data_ptr(), *sections, bool(interleaved), qo.data_ptr(), k_cache.data_ptr(),
             v_cache.data_ptr(), table.data_ptr(), table.shape[1], table.shape[0], seq.data_ptr(), index.data_ptr(), k_cache.shape[0],
