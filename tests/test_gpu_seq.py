@@ -338,6 +338,21 @@ def test_one_token_or_one_head_in_any_memory_order(dtype, t, h, d):
     assert all(torch.equal(a, b) for a, b in zip(want, all_of_them(*xs)))
 
 
+@pytest.mark.parametrize('scale', [1e-39, 3e-38, 1e-20])
+def test_scales_that_leave_no_difference_between_scores(scale):
+    """Every visible key weighs the same, in each form."""
+    for lengths, hq in ((LENGTHS['short'], 2), (LENGTHS['far'], 2), (LENGTHS['wide'], 16), ([2600, 35], 16)):
+        c, d = cum(lengths), 64
+        q, k, v = (randn(c[-1], hq, d, dtype=torch.float32, seed=310 + i) for i in range(3))
+        out = ops.packed_attention(q, k, v, cu_tensor(c), frame=1, scale=scale)
+        want = OS.packed(q[:, :1], k[:, :1], v[:, :1], c, 1, scale=scale)
+        within(out[:, :1], want['out'], want['out_b'], 'out of %d heads' % hq)
+    for lengths in ([99, 0, 1], [5000]):
+        q, kc, vc, table, lens = make_paged(lengths, 1, 16, 2, 2, 64, torch.float32, 315)
+        want, bound = OS.paged(q, kc, vc, table, lens, 1, scale=scale)
+        within(ops.paged_attention(q, kc, vc, table, lens, scale=scale), want, bound, 'paged')
+
+
 def test_packed_attention_nothing_to_do():
     z = torch.zeros(0, 2, 32, device=DEV).requires_grad_()
     out = ops.packed_attention(z, z, z, cu_tensor([0, 0]), frame=1)

@@ -137,7 +137,7 @@ __device__ __forceinline__ void walk_unit(const PagedArgs& a, const Piece& u, in
 #pragma unroll
   for (int dt = 0; dt < DP / 32; ++dt) o[dt] = zero16();
   RowMax st;
-  const float thr = 8.f / a.c;
+  const float thr = RowMax::threshold(a.c);
   const long row_bytes = (long)a.Hk * a.D * O::SZ;
   const char* kb = a.k + (long)kh * a.D * O::SZ;
   const char* vb = a.v + (long)kh * a.D * O::SZ;

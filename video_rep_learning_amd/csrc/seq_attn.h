@@ -627,6 +627,8 @@ __device__ __forceinline__ WaveSpan wave_span(Span s) {
 // m: the maximum its exponents are taken against (raw scores), nm = -m * c, l: this lane's share of the row sum.
 struct RowMax {
   float m = NEG_INF, nm = 0.f, l = 0.f;
+  // (finite, also for a scale so small that no scores differ: -infinity + infinity would compare as no growth at all)
+  static __device__ __forceinline__ float threshold(float c) { return fminf(8.f / c, 3e38f); }
   // mx: the row's maximum over the new scores.  The accumulators are only rescaled when some row's maximum grew by more than `thr`
   // (2^8 in the probability: far from any format's limit); returns true with the factor in alpha then.
   __device__ __forceinline__ bool grow(float mx, float c, float thr, float& alpha) {

@@ -49,7 +49,7 @@ struct Fwd {
     rpart = I::row_part(lane);
     cpart = I::col_part(lane);
     c = a.c;
-    thr = 8.f / a.c;
+    thr = RowMax::threshold(a.c);
     const int hh = lane >> 5;
     const char* src = a.q + (long)min(row, a.T - 1) * a.ldq + head * a.hsq;
 #pragma unroll
