@@ -353,6 +353,68 @@ def test_scales_that_leave_no_difference_between_scores(scale):
         within(ops.paged_attention(q, kc, vc, table, lens, scale=scale), want, bound, 'paged')
 
 
+def first_of_all(s, limits):
+    """The key of each row's largest score among those it sees, and whether it stands out by more than 32 bits round: a sum of up to 128
+    products is off by at most 24 steps of the magnitudes' sum, which is some five times the largest score."""
+    s = s.masked_fill(torch.arange(s.shape[1])[None] >= torch.as_tensor(limits)[:, None], -math.inf)
+    top = s.topk(min(2, s.shape[1]), 1)
+    clear = torch.ones(s.shape[0], dtype=torch.bool)
+    if s.shape[1] > 1:
+        clear = top.values[:, 0] - top.values[:, 1] > 2.0 ** -16 * s.masked_fill(s.isinf(), 0).abs().amax(1)
+        assert clear.sum() >= 0.98 * len(clear) - 1
+    return top.indices[:, 0], clear
+
+
+@pytest.mark.parametrize('dtype', DTYPES, ids=IDS)
+@pytest.mark.parametrize('lengths,hq,d', [([40, 1, 35], 2, 32), ([350, 70], 2, 64), ([40, 30, 9] * 28, 16, 64), ([1300], 16, 128)],
+                         ids=['split', 'far', 'wide', 'pairs'])
+def test_scores_far_beyond_the_range_of_exponents(dtype, lengths, hq, d):
+    """Scores of 10^9 (fp16) to 10^21: each row takes the value of its largest score's key, exactly."""
+    c, big, d = cum(lengths), 1.5e4 if dtype == torch.float16 else 1e10, 64 if len(lengths) == 1 and dtype == torch.float32 else d
+    q, k = (randn(c[-1], hq, d, dtype=torch.float32, seed=320 + i).mul_(big).clamp_(-6e4 if big < 1e5 else -1e12, 6e4 if big < 1e5 else 1e12).to(dtype)
+            for i in range(2))
+    v = randn(c[-1], hq, d, dtype=dtype, seed=322)
+    out = ops.packed_attention(q, k, v, cu_tensor(c), frame=1, scale=1.0)
+    for h in (0, hq - 1):
+        for a, b in zip(c[:-1], c[1:]):
+            at, clear = first_of_all(q[a:b, h].double().cpu() @ k[a:b, h].double().cpu().t(), range(1, b - a + 1))
+            assert torch.equal(out[a:b, h].cpu()[clear], v[a:b, h].cpu()[at[clear]]), (h, a)
+
+
+@pytest.mark.parametrize('dtype', DTYPES, ids=IDS)
+@pytest.mark.parametrize('lengths,width', [([99, 1, 0, 40], 0), ([2500, 3], 300)])
+def test_paged_scores_far_beyond_the_range_of_exponents(dtype, lengths, width):
+    big = 1.5e4 if dtype == torch.float16 else 1e10
+    q, kc, vc, table, lens = make_paged(lengths, 2, 16, 2, 1, 64, dtype, 330)
+    table = torch.cat([table, torch.full((len(lengths), width), -1, dtype=torch.int32, device=DEV)], 1)
+    q, kc = ((x.float() * big).clamp(-6e4 if big < 1e5 else -1e12, 6e4 if big < 1e5 else 1e12).to(dtype) for x in (q / 1.5, kc))
+    out = ops.paged_attention(q, kc, vc, table, lens, scale=1.0)
+    for b, n in enumerate(lengths):
+        pages = table[b, :-(-n // 16)].long()
+        k, v = (x[pages].flatten(0, 1)[:n, 0].cpu() for x in (kc, vc))
+        for i in range(2):
+            for h in range(2):
+                if n - 2 + i < 0:
+                    assert (out[b, i, h] == 0).all()
+                    continue
+                at, clear = first_of_all((q[b, i, h].double().cpu() @ k.double().t())[None], [n - 1 + i])
+                assert not clear or torch.equal(out[b, i, h].cpu(), v[at[0]]), (b, i, h)
+
+
+@pytest.mark.parametrize('dtype', DTYPES[:2], ids=IDS[:2])
+def test_a_key_of_the_lowest_values(dtype):
+    """A key filled with the type's lowest value has a score of some 10^36: all of the weight, or none of it, by the sign of the query's sum."""
+    n, d = 90, 32
+    q, k, v = (randn(n, 1, d, dtype=dtype, seed=340 + i, scale=s) for i, s in enumerate((1e-3, 1.0, 1.0)))
+    k[0] = torch.finfo(dtype).min
+    out = ops.packed_attention(q, k, v, cu_tensor([0, n]), frame=1)
+    first = q[:, 0].double().sum(1).cpu() < 0
+    first[0] = True                                                # it sees nothing else
+    assert torch.equal(out[:, 0].cpu()[first], v[0].cpu().expand(n, d)[first])
+    rest = OS.attend(q[1:, 0], k[1:, 0], v[1:, 0], range(1, n), d ** -0.5, dtype)
+    within(out[1:, 0].cpu()[~first[1:]], rest['out'][~first[1:]], rest['out_b'][~first[1:]], 'without it')
+
+
 def test_packed_attention_nothing_to_do():
     z = torch.zeros(0, 2, 32, device=DEV).requires_grad_()
     out = ops.packed_attention(z, z, z, cu_tensor([0, 0]), frame=1)

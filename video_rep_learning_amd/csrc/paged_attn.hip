@@ -179,6 +179,7 @@ __device__ __forceinline__ void walk_unit(const PagedArgs& a, const Piece& u, in
     mx = pair_max(mx);
     float alpha;
     if (st.grow(mx, a.c, thr, alpha)) {
+      bad |= st.steep(m < a.R);
 #pragma unroll
       for (int dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
@@ -226,7 +227,7 @@ __device__ __forceinline__ void walk_unit(const PagedArgs& a, const Piece& u, in
     }
     there = next;
   }
-  if (bad) {                                          // a value that is not finite beside masked places: visible pairs only
+  if (bad) {                                          // a value that is not finite beside masked places, or steep scores: visible pairs only
 #pragma unroll
     for (int dt = 0; dt < DP / 32; ++dt) o[dt] = zero16();
     st = RowMax();
@@ -239,11 +240,8 @@ __device__ __forceinline__ void walk_unit(const PagedArgs& a, const Piece& u, in
         const long at = ((long)pg * a.page + key % a.page) * row_bytes;
         const float s = slow_dot<O, DP>(qf, kb + at, a.D, hh);
         if (key >= hi) continue;
-        const float to = fmaxf(st.m, s);
-        const float alpha = st.m == NEG_INF ? 0.f : __builtin_amdgcn_exp2f((st.m - to) * a.c);
-        st.m = to;
-        st.nm = to == NEG_INF ? 0.f : -to * a.c;
-        const float p = __builtin_amdgcn_exp2f(fmaf(s, a.c, st.nm));
+        float alpha;
+        const float p = st.add(s, a.c, alpha);
         st.l = fmaf(st.l, alpha, hh == 0 ? p : 0.f);
 #pragma unroll
         for (int dt = 0; dt < DP / 32; ++dt)

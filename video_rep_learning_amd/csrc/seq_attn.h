@@ -640,6 +640,17 @@ struct RowMax {
     l *= alpha;
     return true;
   }
+  // The exponents s c + nm all carry the rounding of nm, which cancels against the row's sum; beyond this size it could push them out of
+  // the formats' range (one step of nm is 2 there), so the wave takes its slow form, whose exponents are (s - m) c.
+  __device__ __forceinline__ bool steep(bool kept) const { return __builtin_amdgcn_ballot_w64(kept && fabsf(nm) > 16777216.f) != 0; }
+  // the slow forms' step: one more score; its weight, and what everything so far is multiplied with
+  __device__ __forceinline__ float add(float s, float c, float& alpha) {
+    const float to = fmaxf(m, s);
+    alpha = m == NEG_INF ? 0.f : __builtin_amdgcn_exp2f((m - to) * c);
+    m = to;
+    nm = to == NEG_INF ? 0.f : -to * c;
+    return __builtin_amdgcn_exp2f((to == NEG_INF ? s : s - to) * c);
+  }
 };
 
 // union of the four waves' spans (a barrier inside)

@@ -42,7 +42,7 @@ struct Fwd {
   float c, thr;
   int lane;
   uint32_t rpart, cpart;
-  bool bad = false;        // a tile with masked places held a value that is not finite
+  bool bad = false;        // a tile with masked places held a value that is not finite, or the scores are steep
 
   __device__ __forceinline__ void start(const FwdArgs& a, int head, int row, int lane_) {
     lane = lane_;
@@ -82,6 +82,7 @@ struct Fwd {
     mx = pair_max(mx);
     float alpha;
     if (st.grow(mx, c, thr, alpha)) {
+      bad |= st.steep(own.hi > own.lo);
 #pragma unroll
       for (int dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
@@ -105,11 +106,8 @@ struct Fwd {
       for (int key = k0; key < min(k0 + 32, end); ++key) {
         const float s = slow_dot<O, DP>(qf, kb + (long)key * a.ldk, a.D, lane >> 5);
         if (key < own.lo || key >= own.hi) continue;
-        const float to = fmaxf(st.m, s);
-        const float alpha = st.m == NEG_INF ? 0.f : __builtin_amdgcn_exp2f((st.m - to) * c);
-        st.m = to;
-        st.nm = to == NEG_INF ? 0.f : -to * c;
-        const float p = __builtin_amdgcn_exp2f(fmaf(s, c, st.nm));
+        float alpha;
+        const float p = st.add(s, c, alpha);
         st.l = fmaf(st.l, alpha, lane < 32 ? p : 0.f);                  // the pair's sum is taken at the end
 #pragma unroll
         for (int dt = 0; dt < DP / 32; ++dt)
