@@ -265,6 +265,34 @@ def test_packed_attention_gradients_hide_other_sequences_from_pairs_of_waves(dty
             within(x[c[1]:c[1] + 4], want[nm][c[1]:c[1] + 4], want[nm + '_b'][c[1]:c[1] + 4], '%s of the next sequence' % nm)
 
 
+@pytest.mark.parametrize('lengths,hq,hk,d,dtypes', [([500, 450, 500], 12, 6, 64, DTYPES), ([450, 35] + [100] * 37, 8, 4, 64, DTYPES),
+                                                    ([2600, 45], 16, 8, 128, DTYPES[1:2]), ([2600, 45], 16, 8, 120, DTYPES[2:]),
+                                                    ([2600, 45], 16, 16, 64, DTYPES[:1])],
+                         ids=['split, two heads a workgroup', 'wide, two heads a workgroup', 'pairs bf16', 'pairs fp16', 'pairs fp32'])
+def test_key_gradients_past_a_bad_query(lengths, hq, hk, d, dtypes):
+    """A query or output gradient that is not finite early in a long sequence: the keys behind it, some of them in its own tile, are not
+    seen by it and keep their gradients, which their waves take again over their whole walk; an output gradient with one infinite
+    channel leaves the other channels of every dV as they are."""
+    c, at = cum(lengths), 100
+    for dtype in dtypes:
+        q, k, v, do = (randn(c[-1], h, d, dtype=dtype, seed=350 + i) for i, h in enumerate((hq, hk, hk, hq)))
+        want = OS.packed(q, k, v, c, 1, do=do)
+        rows, keys = torch.arange(c[-1]) != at, torch.arange(c[-1]) > at
+        other = [i for i in range(d) if i != 5]
+        for which, bad in (('q', math.nan), ('q', math.inf), ('do', math.nan), ('do', -math.inf)):
+            q2, do2 = q.clone(), do.clone()
+            if which == 'q':
+                q2[at] = bad
+            else:
+                do2[at, :, 5] = bad
+            got = run_packed(q2, k, v, cu_tensor(c), 1, do2)
+            for x, nm, keep in zip(got, ('out', 'dq', 'dk', 'dv'), (rows, rows, keys, keys)):
+                within(x[keep], want[nm][keep], want[nm + '_b'][keep], '%s behind a bad %s' % (nm, which))
+            if which == 'do':
+                within(got[0], want['out'], want['out_b'], 'out')
+                within(got[3][..., other], want['dv'][..., other], want['dv_b'][..., other], 'the other channels of dv')
+
+
 def test_packed_attention_gradient_against_differences():
     """Central differences of the fp32 forward: f = sum w * out.  The forward is off by its bounds, so f by b = sum |w| bound, the quotient
     by b / h; the step's own error is h^2 / 6 of the third derivative, taken from halving the step."""
