@@ -7,6 +7,7 @@ import torch
 HALF_STEP = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}   # one rounding, relative
 TINY = {torch.float32: 2.0 ** -149, torch.bfloat16: 2.0 ** -133, torch.float16: 2.0 ** -24}      # one step below the normal range
 U32 = 2.0 ** -24
+FLUSH = 2.0 ** -126          # the device's power of two gives 0 below this, its matrix instructions may take and leave 0 there
 
 
 def rotate(x, pos, freqs, sections, interleaved=False, inverse=False):
@@ -46,11 +47,15 @@ def attend(q, k, v, limits, scale, dtype, do=None, low=False):
     and its power of two round a few times more; so a probability is off by 2 * es relative (numerator and denominator), es the
     score's absolute error + 8 steps.  Probabilities and dS round once to a 16-bit operand (up).  A sum over n terms is off by at most
     (n / 16 + 40) steps of 32 bits of the sum of magnitudes.  delta reads the stored, rounded output.  low: a probability enters its
-    product as the 16-bit operand and the rounded rest (at most up of it, so the two are off by up * up)."""
+    product as the 16-bit operand and the rounded rest (at most up of it, so the two are off by up * up).
+
+    Weights are powers of two of s - m, m no larger than the row's maximum, so their sum is at least 1 and a weight that is flushed to 0
+    takes at most FLUSH from a probability; so does every term of a sum that lies below it."""
     q, k, v = (t.detach().double().cpu() for t in (q, k, v))
     n, L, D = q.shape[0], k.shape[0], q.shape[1]
     u = HALF_STEP[dtype]
     up, tiny = (0.0, 0.0) if dtype == torch.float32 else (u * u if low else u, TINY[dtype])
+    lost = max(tiny * 0.5, FLUSH)
     seen = torch.arange(L)[None] < torch.as_tensor(limits)[:, None]
     if L == 0:
         z = torch.zeros(n, D, dtype=torch.float64)
@@ -69,7 +74,7 @@ def attend(q, k, v, limits, scale, dtype, do=None, low=False):
     es = ((D / 8 + 8) * big + 8 * (1 + big)) * U32                       # absolute, of a natural exponent
     ep = 2 * es + (L / 16 + 40) * U32 + 2.0 ** -22                          # relative, of a probability
     ones = seen.double()
-    out_b = (p * (up + ep)) @ v.abs() + tiny * 0.5 * (ones @ v.abs()) / 1.0 + (L / 16 + 40) * U32 * (p @ v.abs())
+    out_b = (p * (up + ep)) @ v.abs() + lost * (ones @ v.abs()) + FLUSH * L + (L / 16 + 40) * U32 * (p @ v.abs())
     out_b = out_b + u * (out.abs() + out_b) + TINY[dtype]
     r = dict(out=out, out_b=out_b)
     if do is None:
@@ -78,17 +83,17 @@ def attend(q, k, v, limits, scale, dtype, do=None, low=False):
     dp = do @ v.t()
     delta = (do * out).sum(1, keepdim=True)
     ds = p * (dp - delta)
-    pb = p * (up + ep) + tiny * 0.5 * ones
+    pb = p * (up + ep) + lost * ones
     N = n / 16 + 40
     dv = p.t() @ do
-    dv_b = pb.t() @ do.abs() + N * U32 * (p.t() @ do.abs())
+    dv_b = pb.t() @ do.abs() + FLUSH * n + N * U32 * (p.t() @ do.abs())
     delta_b = (do.abs() * (out_b + D * U32 * out.abs())).sum(1, keepdim=True)
     dp_b = (D / 8 + 8) * U32 * (do.abs() @ v.abs().t())
-    ds_b = p * (dp_b + delta_b + 2 * U32 * (dp.abs() + delta.abs())) + (p * ep) * (dp - delta).abs()
-    ds_b = ds_b + up * (ds.abs() + ds_b) + tiny * 0.5 * ones
+    ds_b = p * (dp_b + delta_b + 2 * U32 * (dp.abs() + delta.abs())) + (p * ep + FLUSH * ones) * (dp - delta).abs()
+    ds_b = ds_b + up * (ds.abs() + ds_b) + lost * ones
     dq, dk = ds @ k * scale, ds.t() @ q * scale
-    dq_b = (ds_b @ k.abs() + (L / 16 + 40) * U32 * (ds.abs() @ k.abs())) * scale
-    dk_b = (ds_b.t() @ q.abs() + N * U32 * (ds.abs().t() @ q.abs())) * scale
+    dq_b = (ds_b @ k.abs() + FLUSH * L + (L / 16 + 40) * U32 * (ds.abs() @ k.abs())) * scale
+    dk_b = (ds_b.t() @ q.abs() + FLUSH * n + N * U32 * (ds.abs().t() @ q.abs())) * scale
     r.update(dq=dq, dk=dk, dv=dv, dq_b=dq_b + u * (dq.abs() + dq_b) + TINY[dtype], dk_b=dk_b, dv_b=dv_b)   # dk, dv: rounded after the group's sum
     return r
 

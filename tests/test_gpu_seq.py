@@ -366,6 +366,34 @@ def test_one_token_or_one_head_in_any_memory_order(dtype, t, h, d):
     assert all(torch.equal(a, b) for a, b in zip(want, all_of_them(*xs)))
 
 
+RISING = [('short', 4, 2, 40, 1), ('edges', 2, 1, 80, 0), ('long', 3, 1, 64, 5), ('far', 2, 1, 64, 1), ('far', 1, 1, 32, 0), ('wide', 16, 16, 32, 1),
+          ('wide', 16, 8, 128, 0), ('swarm', 2, 1, 32, 1), ('pairs', 16, 8, 128, 1), ('pairs', 16, 16, 64, 1)]
+
+
+def rising(x, lengths, height, seed):
+    """Keys whose products with rising_queries() climb by `height` over each sequence."""
+    u = torch.randn(x.shape[-1], generator=torch.Generator().manual_seed(seed)).sign().to(DEV)
+    step = torch.cat([torch.arange(n) / max(n, 1) for n in lengths]).to(DEV)
+    return (x.float() * 0.7 + step[:, None, None] * height / x.shape[-1] * u).to(x.dtype), u
+
+
+@pytest.mark.parametrize('dtype', DTYPES, ids=IDS)
+@pytest.mark.parametrize('scale', [0.6, 0.03], ids=['large scale', 'small scale'])
+@pytest.mark.parametrize('lengths,hq,hk,d,frame', RISING)
+def test_packed_attention_with_scores_that_rise_along_the_keys(dtype, scale, lengths, hq, hk, d, frame):
+    """A scale of the caller's, and scores that climb by 60 over a sequence: most rows take a new maximum again and again, in every form."""
+    lens = LENGTHS[lengths]
+    c = cum(lens)
+    q, k, v = (randn(c[-1], h, d, dtype=dtype, seed=360 + i) for i, h in enumerate((hq, hk, hk)))
+    k, u = rising(k, lens, 60 / scale, 364)
+    q = (q.float() * 0.3 + u).to(dtype)
+    do = randn(c[-1], hq, d, dtype=dtype, seed=365)
+    got = run_packed(q, k, v, cu_tensor(c), frame, do, scale=scale)
+    want = OS.packed(q, k, v, c, frame, scale=scale, do=do)
+    for x, nm in zip(got, ('out', 'dq', 'dk', 'dv')):
+        within(x, want[nm], want[nm + '_b'], nm)
+
+
 @pytest.mark.parametrize('scale', [1e-39, 3e-38, 1e-20])
 def test_scales_that_leave_no_difference_between_scores(scale):
     """Every visible key weighs the same, in each form."""
@@ -525,6 +553,22 @@ def test_paged_attention(dtype, lengths, new, page, hq, hk, d, frame):
     within(ops.paged_attention(q, kc, vc, wide, lens.long(), frame=frame), want, bound, 'wide table')
     qt = q.transpose(1, 2).contiguous().transpose(1, 2)
     assert torch.equal(ops.paged_attention(qt, kc, vc, table, lens, frame=frame), out)
+
+
+@pytest.mark.parametrize('dtype', DTYPES, ids=IDS)
+@pytest.mark.parametrize('scale', [0.6, 0.03], ids=['large scale', 'small scale'])
+@pytest.mark.parametrize('lengths,new,page,hq,hk,d,frame', [PAGED[i] for i in (1, 3, 5, 7, 8, 10, 11)])
+def test_paged_attention_with_scores_that_rise_along_the_keys(dtype, scale, lengths, new, page, hq, hk, d, frame):
+    q, kc, vc, table, lens = make_paged(lengths, new, page, hq, hk, d, dtype, 370)
+    for b, n in enumerate(lengths):
+        for j in range(-(-n // page)):
+            m, pg = min(page, n - j * page), int(table[b, j])
+            u = torch.randn(d, generator=torch.Generator().manual_seed(371)).sign().to(DEV)
+            step = (torch.arange(j * page, j * page + m, device=DEV) / n)[:, None, None]
+            kc[pg, :m] = (kc[pg, :m].float() * 0.7 + step * (60 / scale / d) * u).to(dtype)
+    q = (q.float() * 0.2 + torch.randn(d, generator=torch.Generator().manual_seed(371)).sign().to(DEV)).to(dtype)
+    want, bound = OS.paged(q, kc, vc, table, lens, frame, scale=scale, low=True)
+    within(ops.paged_attention(q, kc, vc, table, lens, frame=frame, scale=scale), want, bound, 'out')
 
 
 @pytest.mark.parametrize('dtype', DTYPES, ids=IDS)
