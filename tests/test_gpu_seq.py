@@ -176,6 +176,24 @@ def test_packed_attention_and_its_gradients(dtype, lengths, hq, hk, d, frame):
         assert torch.equal(ops.packed_attention(q, k, v, cu_tensor(c), frame=frame), got[0])       # the same without statistics
 
 
+@pytest.mark.parametrize('dtype,lengths,hq,hk,d,frame', [
+    (torch.bfloat16, [6000, 70], 8, 4, 64, 1),       # 408 workgroups of 128 rows: all on the card at once, two rounds there and back
+    (torch.bfloat16, [2600, 45], 12, 4, 96, 1),      # 288: the second round is a part of one
+    (torch.float16, [4200, 130], 15, 5, 80, 6),      # 555, all heads' tiles in turn
+    (torch.float32, [5200], 3, 1, 32, 1),            # the split form, eight waves a tile
+    (torch.bfloat16, [6500], 8, 2, 128, 0),          # walks of the whole sequence, two waves in turn only where causal
+    (torch.bfloat16, [6500], 8, 2, 128, 1)], ids=['there and back', 'part of a round', 'heads in turn', 'split', 'all keys', 'pairs'])
+def test_long_sequences(dtype, lengths, hq, hk, d, frame):
+    """Thousands of tokens, one group of heads of them compared."""
+    c, g, at = cum(lengths), hq // hk, hk - 1
+    q, k, v, do = (randn(c[-1], h, d, dtype=dtype, seed=380 + i) for i, h in enumerate((hq, hk, hk, hq)))
+    got = run_packed(q, k, v, cu_tensor(c), frame, do)
+    hs, ks = slice(at * g, at * g + g), slice(at, at + 1)
+    want = OS.packed(q[:, hs], k[:, ks], v[:, ks], c, frame, do=do[:, hs])
+    for x, nm in zip(got, ('out', 'dq', 'dk', 'dv')):
+        within(x[:, hs if nm in ('out', 'dq') else ks], want[nm], want[nm + '_b'], nm)
+
+
 @pytest.mark.parametrize('dtype', DTYPES, ids=IDS)
 @pytest.mark.parametrize('frame,behind,hq,hk', [(0, 61, 4, 2), (1, 61, 4, 2), (4, 61, 4, 2), (1, 4100, 16, 16)])
 def test_packed_attention_leaves_rows_of_no_sequence_alone(dtype, frame, behind, hq, hk):
