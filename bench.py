@@ -464,6 +464,7 @@ def main():
         dist.all_gather_object(ranks_seen, me)
 
     from video_rep_learning_amd import _lib
+    from video_rep_learning_amd.utils.distributed import reduce_tensor
     from video_rep_learning_amd.utils import presets
     from video_rep_learning_amd.utils.optimizer import construct_optimizer
     from video_rep_learning_amd.models import build_model
@@ -544,7 +545,7 @@ def main():
                 'exposed_allreduce_ms_per_step': None if (ex := reducer.exposed_ms()) is None else round(ex, 4), 'reducer_active': True}
     tmax = torch.tensor([dt], device=dev, dtype=torch.float64)
     if world > 1:
-        dist.all_reduce(tmax, op=dist.ReduceOp.MAX)
+        reduce_tensor(tmax, op=dist.ReduceOp.MAX)
     dt = tmax.item()
     # ---- the same loop, extended to a settled state: every rank derives the same step count from the all-reduced time ----
     sustained = None
@@ -558,7 +559,7 @@ def main():
         dt2 = time.perf_counter() - t0
         t2 = torch.tensor([dt2], device=dev, dtype=torch.float64)
         if world > 1:
-            dist.all_reduce(t2, op=dist.ReduceOp.MAX)
+            reduce_tensor(t2, op=dist.ReduceOp.MAX)
         sustained = {'steps': n2, 'seconds': round(t2.item(), 4), 'ms_per_step': round(t2.item() / n2 * 1e3, 3)}
     stage('roofline steps')
     last_loss = float(loss.item())

@@ -209,6 +209,50 @@ def test_two_ranks_on_two_gpus_over_rccl_equal_one_process(gather):
     assert worst[1] <= 2e-2, worst
 
 
+# ---------------------------------------------------------------------------------------------- gloo and device tensors
+def test_gloo_is_given_host_memory_only(monkeypatch):
+    """Every collective of the data-parallel step on device tensors, over a one-rank gloo group (identities)."""
+    from video_rep_learning_amd import ops
+    from video_rep_learning_amd.utils import distributed as du
+
+    def host_only(name):
+        real = getattr(dist, name)
+
+        def call(*args, **kw):
+            for t in args:
+                for x in t if isinstance(t, (list, tuple)) else [t]:
+                    assert not (torch.is_tensor(x) and x.is_cuda), '%s over gloo on a device tensor' % name
+            return real(*args, **kw)
+        monkeypatch.setattr(dist, name, call)
+    for name in ('all_reduce', 'all_gather', 'all_gather_into_tensor'):
+        host_only(name)
+    monkeypatch.setenv('MVF_FORCE_REDUCER', '1')
+    dist.init_process_group('gloo', init_method='tcp://127.0.0.1:%d' % _free_port(), rank=0, world_size=1)
+    try:
+        x = torch.randn(6, 5, device='cuda')
+        want = x.clone()
+        assert torch.equal(du.all_reduce([x])[0], want) and torch.equal(du.all_gather([x])[0], want)
+        y = x.clone().requires_grad_()
+        z = du.gather_rows(y)
+        z.backward(x)
+        assert torch.equal(z, want) and torch.equal(y.grad, want)
+        du.reduce_tensor(x, op=dist.ReduceOp.MAX)
+        assert torch.equal(x, want)
+        mean, var = torch.randn(8, device='cuda'), torch.rand(8, device='cuda') + 0.1
+        for equal in (True, False):
+            m, v, n = ops.sync_bn_stats(mean, var, 12, equal_counts=equal)
+            assert n == 12 and (m - mean).abs().max() <= 2.0 ** -22 * mean.abs().max() and (v - var).abs().max() <= 2.0 ** -22 * var.max()
+        params = [torch.nn.Parameter(torch.randn(7, 3, device='cuda')), torch.nn.Parameter(torch.randn(5, device='cuda'))]
+        flat = du.FlatBuffers(params)
+        red = du.GradReducer(flat)
+        sum((p * p).sum() for p in params).backward()
+        assert red.finish() == 1.0
+        for p in params:
+            assert torch.equal(p.grad, 2 * p.detach())
+    finally:
+        dist.destroy_process_group()
+
+
 # ---------------------------------------------------------------------------------------------- RCCL, one rank
 def _forced_worker(rank, world, port, ret, gather):
     """One process, one GPU: a plain step first, then the same step on a ONE-rank `nccl` (= RCCL) process group with

@@ -16,6 +16,7 @@ from torch.autograd.graph import increment_version
 
 from . import _lib
 from ._lib import call, ptr, stream, F32, BF16, FP8, F16
+from .utils.distributed import gather_tensor, reduce_tensor
 
 
 def _dt(dtype):
@@ -518,17 +519,14 @@ def sync_bn_stats(mean, var, count, group=None, equal_counts=False, running=None
             local = syncbn_local_buffer(C, count, mean.device)
             local[:C].copy_(mean)
             local[C:2 * C].copy_(var)
-        gathered = torch.empty(world * (2 * C + 1), device=mean.device, dtype=torch.float32)   # flat: gloo's form of the call takes no 2-D output
-        dist.all_gather_into_tensor(gathered, local, group=group)
+        gathered = gather_tensor(local, group)
         gm = torch.empty(C, device=mean.device, dtype=torch.float32)
         gv = torch.empty_like(gm)
         rm, rv, mom = running if running is not None else (None, None, 0.0)
         call('mvf_syncbn_merge', ptr(gathered), world, C, float(count), ptr(gm), ptr(gv), ptr(rm), ptr(rv), float(mom), stream())
         return gm, gv, float(count) * world
     local = torch.cat([mean, var, mean.new_tensor([float(count)])])
-    gathered = [torch.empty_like(local) for _ in range(world)]
-    dist.all_gather(gathered, local, group=group)
-    st = torch.stack(gathered)
+    st = gather_tensor(local, group)
     n = st[:, -1:]
     if equal_counts:
         total = float(count) * world
@@ -602,7 +600,7 @@ class _BatchNormTrain(torch.autograd.Function):
         if slots is not None:
             grad_ready(*owners)
         if world > 0:
-            dist.all_reduce(s, group=group)          # collective C3 of SURVEY.md
+            reduce_tensor(s, group)                  # collective C3 of SURVEY.md
         dx = torch.empty_like(x)
         call('mvf_bn_bwd_apply', ptr(dy), ptr(x), ptr(mean), ptr(var), ptr(g), ptr(b), s[0].data_ptr(),
              s[1].data_ptr(), ptr(dx), R, C, eps, int(relu), count, stream())
@@ -1306,7 +1304,7 @@ class _RowLinChain(torch.autograd.Function):
             if sync_sums is not None:
                 # SyncBatchNorm backward: sum dZ and sum dZ xhat over ALL ranks' rows (collective C3 of SURVEY.md) before the previous
                 # stage's launch applies them; dgamma / dbeta stay local (the gradient all-reduce averages them like every parameter)
-                dist.all_reduce(sync_sums, group=stages[i - 1].sync[0])
+                reduce_tensor(sync_sums, stages[i - 1].sync[0])
             probs.append((gT, R['xT'], st.w, st.b, N, Kin))
             keep.append(gT)
             dcur = dX

@@ -64,12 +64,48 @@ def synchronize():
         dist.barrier()
 
 
+# gloo takes host memory only: given device tensors it makes streams of a higher priority and copies from threads of its own, which has
+# hung with several ranks on one device and has ended a rank at its exit.  Device tensors go through host memory here, synchronously.
+def _through_host(t, group=None):
+    return t.is_cuda and dist.get_backend(group) == 'gloo'
+
+
+class _HostReduce:
+    """The asynchronous form of an all-reduce through host memory: wait() brings the sums back."""
+
+    def __init__(self, t, group, op):
+        self.t, self.host = t, t.cpu()
+        self.work = dist.all_reduce(self.host, op=op, group=group, async_op=True)
+
+    def wait(self):
+        self.work.wait()
+        self.t.copy_(self.host)
+
+
+def reduce_tensor(t, group=None, async_op=False, op=dist.ReduceOp.SUM):
+    """dist.all_reduce (in place) of a host or device tensor; async_op: returns what wait() is called on."""
+    if not _through_host(t, group):
+        return dist.all_reduce(t, op=op, group=group, async_op=async_op)
+    work = _HostReduce(t, group, op)
+    if async_op:
+        return work
+    work.wait()
+
+
+def gather_tensor(t, group=None):
+    """dist.all_gather of equal shapes: [world, *t.shape], on t's device."""
+    src = t.cpu() if _through_host(t, group) else t.contiguous()
+    out = torch.empty(dist.get_world_size(group) * t.numel(), dtype=t.dtype, device=src.device)     # (gloo's form takes one dimension)
+    dist.all_gather_into_tensor(out, src.reshape(-1), group=group)
+    return out.view(-1, *t.shape).to(t.device)
+
+
 def all_reduce(tensors, average=True):
     """In-place all-reduce of a list of tensors, optionally averaged (distributed.py:38-54)."""
     if not collectives_active():
         return tensors
     for t in tensors:
-        dist.all_reduce(t, async_op=False)
+        reduce_tensor(t)
     if average:
         ws = dist.get_world_size()
         for t in tensors:
@@ -81,12 +117,7 @@ def all_gather(tensors):
     """Non-differentiable tensor all-gather + cat(dim 0) (distributed.py:16-35)."""
     if not collectives_active():
         return tensors
-    out = []
-    for t in tensors:
-        parts = [torch.empty_like(t) for _ in range(dist.get_world_size())]
-        dist.all_gather(parts, t.contiguous())
-        out.append(torch.cat(parts, dim=0))
-    return out
+    return [gather_tensor(t).flatten(0, 1) for t in tensors]
 
 
 class _GatherRows(torch.autograd.Function):
@@ -96,11 +127,8 @@ class _GatherRows(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x):
-        ws, rk = dist.get_world_size(), dist.get_rank()
-        parts = [torch.empty_like(x) for _ in range(ws)]
-        dist.all_gather(parts, x.contiguous())
-        ctx.rows, ctx.rank = x.shape[0], rk
-        return torch.cat(parts, dim=0)
+        ctx.rows, ctx.rank = x.shape[0], dist.get_rank()
+        return gather_tensor(x).flatten(0, 1)
 
     @staticmethod
     def backward(ctx, g):
@@ -226,7 +254,7 @@ class GradReducer:
 
     def _launch(self, b):
         s, e = self.buckets[b]
-        self.works[b] = dist.all_reduce(self.flat.flat_g[s:e], op=dist.ReduceOp.SUM, group=self.group, async_op=True)
+        self.works[b] = reduce_tensor(self.flat.flat_g[s:e], group=self.group, async_op=True)
 
     def _make_hook(self, i, from_kernel):
         def hook(_param):
