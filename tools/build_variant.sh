@@ -9,7 +9,7 @@ set -e
 R=$(cd $(dirname $0)/.. && pwd)
 C=$R/video_rep_learning_amd/csrc
 python3 -c "import sys; sys.path.insert(0, '$R'); from video_rep_learning_amd.csrc import build; build.build()"
-HIPCC="/opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -fPIC -std=c++17 -Wno-unused-result -mllvm -amdgpu-atomic-optimizer-strategy=None -I$C -I$R/include"
+HIPCC="/opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -fPIC -std=c++17 -Wno-unused-result -mllvm -amdgpu-atomic-optimizer-strategy=None -Xclang -target-feature -Xclang -packed-fp32-ops -I$C -I$R/include"
 name=$1
 if [[ "$2" == *.hip ]]; then
   srcs="$2"; shift 2; flags="$*"; out=$C/libmvf_hip_$name.so

@@ -11,15 +11,11 @@ LIB = os.path.join(HERE, 'libmvf_hip.so')
 HIPCC = os.environ.get('HIPCC', '/opt/rocm/bin/hipcc')
 # atomic optimizer off: it rewrites a one-lane ticket atomic (gemm_tc256) into a wave-aggregated one whose result is
 # read back at once (s_waitcnt vmcnt(0) right behind the atomic)
+# packed fp32 off: hipcc makes v_pk_add / mul / fma_f32 out of ordinary float code, and some of their forms have given wrong results on this
+# part now and then (training step of the default benchmark 10.63 -> 10.73 ms)
 FLAGS = ['--offload-arch=gfx950', '-O3', '-fPIC', '-std=c++17', '-Wno-unused-result',
-         '-mllvm', '-amdgpu-atomic-optimizer-strategy=None',
+         '-mllvm', '-amdgpu-atomic-optimizer-strategy=None', '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops',
          '-I' + HERE, '-I' + os.path.join(HERE, '..', '..', 'include')] + os.environ.get('MVF_EXTRA_FLAGS', '').split()
-
-# hipcc makes v_pk_add / mul / fma_f32 out of ordinary float code, and some of their forms have given wrong results on this part now and
-# then.  These sources are compiled without them; the older ones keep the instructions (and bits) that their tests' ReLU-kink
-# comparisons were settled with: without packed fp32 one small-model gradient check lands on another side of two kinks.
-UNPACKED = ['-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
-UNPACKED_SOURCES = ('rotary.hip', 'seq_attn.hip', 'seq_attn_bwd.hip', 'paged_attn.hip')
 
 
 def sources():
@@ -42,8 +38,7 @@ def _stale(target, deps):
 def _compile(src, force):
     obj = os.path.join(HERE, 'build', os.path.basename(src)[:-4] + '.o')
     if force or _stale(obj, [src, os.path.abspath(__file__)] + headers()):      # (this file: the flags)
-        flags = FLAGS + (UNPACKED if os.path.basename(src) in UNPACKED_SOURCES else [])
-        r = subprocess.run([HIPCC] + flags + ['-c', src, '-o', obj], capture_output=True, text=True)
+        r = subprocess.run([HIPCC] + FLAGS + ['-c', src, '-o', obj], capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError('hipcc failed on %s:\n%s' % (src, r.stderr[-4000:]))
     return obj

@@ -107,8 +107,7 @@ __device__ __forceinline__ float gelu_erf(float x) { return 0.5f * x * (1.0f + e
 // epilogue is VALU-bound: 1750 VALU instructions per wave and tile) took a quarter more.  The max / fma form has no
 // cancellation on either side of 0 (0.5 x (1 + erf) loses the negative tail to the rounding of 1 + erf).
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
-// two elements at a time, written on 2-vectors: the polynomial, the squarings and the last fma are v_pk_fma_f32 / v_pk_mul_f32
-// (left to the SLP vectoriser, the literal constants of the scalar form end up in v_fmaak_f32 and nothing is packed)
+// two elements at a time, written on 2-vectors (csrc/build.py's flags keep them out of packed fp32 instructions)
 __device__ __forceinline__ f32x2_t gelu_erf_fast2(f32x2_t x) {
   const f32x2_t z = {fabsf(x.x) * 0.70710678118654752440f, fabsf(x.y) * 0.70710678118654752440f};   // |.| is a source modifier
   const f32x2_t a6 = {0.0000430638f, 0.0000430638f}, a5 = {0.0002765672f, 0.0002765672f}, a4 = {0.0001520143f, 0.0001520143f},

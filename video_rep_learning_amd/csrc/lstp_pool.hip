@@ -53,6 +53,16 @@ template <> struct Ld16<bf16_t> {
 
 // ---- pass 1: scores[f*N+n, j] = sum_c x[f,n,c] * vec[f|0, j, c] --------------------------------------------
 // grid (F, ysplit); a wave walks tokens of its frame two at a time; vec of the frame sits in LDS ([nq][C] f32).
+// fp32 rows: products rounded one by one, the same bits whichever instructions take them; 16-bit rows' products are fused into the sum
+template <typename T>
+__device__ __forceinline__ float dot4(const float* v, const float4& w) {
+  if constexpr (sizeof(T) == 4) {
+#pragma clang fp contract(off)
+    return v[0] * w.x + v[1] * w.y + v[2] * w.z + v[3] * w.w;
+  } else {
+    return v[0] * w.x + v[1] * w.y + v[2] * w.z + v[3] * w.w;
+  }
+}
 template <typename T>
 __global__ __launch_bounds__(256) void lstp_scores_kernel(PoolArgs a) {
   extern __shared__ __attribute__((aligned(16))) float svec[];  // [nq][C]
@@ -88,8 +98,8 @@ __global__ __launch_bounds__(256) void lstp_scores_kernel(PoolArgs a) {
 #pragma unroll
             for (int e = 0; e < E; e += 4) {
               const float4 w4 = *reinterpret_cast<const float4*>(wv + e);
-              acc0[j] += v0[e] * w4.x + v0[e + 1] * w4.y + v0[e + 2] * w4.z + v0[e + 3] * w4.w;
-              acc1[j] += v1[e] * w4.x + v1[e + 1] * w4.y + v1[e + 2] * w4.z + v1[e + 3] * w4.w;
+              acc0[j] += dot4<T>(v0 + e, w4);
+              acc1[j] += dot4<T>(v1 + e, w4);
             }
           }
         }

@@ -384,7 +384,7 @@ __global__ __launch_bounds__(NW * 64, OCC) void vit_attn_bf16_flash_kernel(AttnA
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      float mx = -1e30f;     // 3-input maxima and packed fp32 arithmetic: see attn_tiles
+      float mx = -1e30f;     // 3-input maxima and arithmetic on pairs: see attn_tiles
 #pragma unroll
       for (int kt = 0; kt < KTB; ++kt) mx = max3f(max3f(mx, s[i][kt][0], s[i][kt][1]), s[i][kt][2], s[i][kt][3]);
       mx = fmaxf(mx, __shfl_xor(mx, 16, 64));

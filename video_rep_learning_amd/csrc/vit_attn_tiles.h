@@ -21,8 +21,8 @@ struct AttnArgs {
   int npad;         // the backward of trainable blocks (vit_attn_bwd.hip); NULL on the frozen path
 };
 
-// v_max3_f32 / packed fp32 arithmetic (v_pk_fma_f32, v_pk_add_f32: two floats per lane and instruction at the full VALU rate),
-// written so that hipcc selects them itself: inline asm would hide the MFMA-result -> VALU-read wait states from its hazard pass
+// v_max3_f32, written so that hipcc selects it itself: inline asm would hide the MFMA-result -> VALU-read wait states from its hazard pass;
+// arithmetic on pairs, which csrc/build.py's flags keep out of packed instructions
 __device__ __forceinline__ float max3f(float a, float b, float c) { return __builtin_fmaxf(__builtin_fmaxf(a, b), c); }
 __device__ __forceinline__ f32x2_t pk_fma(f32x2_t a, f32x2_t b, f32x2_t c) { return __builtin_elementwise_fma(a, b, c); }
 __device__ __forceinline__ f32x2_t pk_add(f32x2_t a, f32x2_t b) { return a + b; }

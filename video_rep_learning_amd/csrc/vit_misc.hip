@@ -87,6 +87,7 @@ __global__ __launch_bounds__(256) void layernorm_kernel(const float* __restrict_
   for (int i = 0; i < MAXV; ++i) {
     const int q = lane + i * 64;
     if (q < nv) {
+#pragma clang fp contract(off)                // squares rounded one by one: the same bits whichever instructions take them
       const float a = v[i].x - mean, bb = v[i].y - mean, c = v[i].z - mean, d = v[i].w - mean;
       ss += a * a + bb * bb + c * c + d * d;
     }
