@@ -624,6 +624,24 @@ def test_paged_attention_rounds_once(dtype, lengths, new, page, hq, hk, d, frame
     within(ops.paged_attention(q, kc, vc, table, lens, frame=frame), want, bound, 'out')
 
 
+@pytest.mark.parametrize('dtype', DTYPES, ids=IDS)
+@pytest.mark.parametrize('bad', [math.inf, -math.inf])
+@pytest.mark.parametrize('length,width', [(97, 0), (3000, 0)])
+def test_paged_attention_carries_infinite_values(dtype, bad, length, width):
+    """An infinite value among the visible ones is that row's result in its channel, in the middle of a walk as beside masked places."""
+    for at in (40, length - 1):
+        q, kc, vc, table, lens = make_paged([length], 2, 16, 4, 2, 32, dtype, 135)
+        want, bound = OS.paged(q, kc, vc, table, lens, 1)
+        # weights of this key in all rows, far from what 16 bits flush
+        pg, row = int(table[0, at // 16]), at % 16
+        vc[pg, row, :, 5] = bad
+        out = ops.paged_attention(q, kc, vc, table, lens, frame=1)
+        sees = [i for i in range(2) if at < length - 1 + i]
+        assert (out[0, sees][..., 5] == bad).all()
+        other = [i for i in range(32) if i != 5]
+        within(out[..., other], want[..., other], bound[..., other], 'other channels')
+
+
 def test_paged_attention_far_pages():
     """Pages behind 2^31 elements of the cache, written by rotary_append and read back."""
     page, hk, d = 64, 8, 128

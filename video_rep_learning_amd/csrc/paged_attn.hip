@@ -227,6 +227,7 @@ __device__ __forceinline__ void walk_unit(const PagedArgs& a, const Piece& u, in
     }
     there = next;
   }
+  if constexpr (LOW<O>) bad |= not_finite(o, m < a.R);
   if (bad) {                                          // a value that is not finite beside masked places, or steep scores: visible pairs only
 #pragma unroll
     for (int dt = 0; dt < DP / 32; ++dt) o[dt] = zero16();

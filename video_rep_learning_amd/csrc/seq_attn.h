@@ -220,6 +220,17 @@ __device__ __forceinline__ bool tile_nonfinite(uint32_t img, int lane) {
   for (int i = 0; i < I::C / 2; ++i) bad |= O::nonfinite(lds_read<u32x4_t>(img + (i * 64 + lane) * 16));
   return __builtin_amdgcn_ballot_w64(bad) != 0;
 }
+// The second operand of LOW may be 0 or of the other sign, so an infinity of the streamed rows can come out as NaN: where sums that took it
+// are not finite (in lanes that are kept), the wave goes over its rows again too.
+template <int N>
+__device__ __forceinline__ bool not_finite(const f32x16_t (&x)[N], bool kept) {
+  float t = 0.f;
+#pragma unroll
+  for (int dt = 0; dt < N; ++dt)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) t = fmaf(x[dt][e], 0.f, t);
+  return __builtin_amdgcn_ballot_w64(kept && t != 0.f) != 0;      // (a NaN is not equal to 0)
+}
 // the slow forms' pieces: a dot product of a row in fragments with a row in memory (whole in both lanes of a pair), and acc += w * row
 template <class O, int DP>
 __device__ __forceinline__ float slow_dot(const typename O::Frag (&f)[DP / 16], const char* row, int D, int hh) {
