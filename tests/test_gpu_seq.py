@@ -176,6 +176,23 @@ def test_packed_attention_and_its_gradients(dtype, lengths, hq, hk, d, frame):
         assert torch.equal(ops.packed_attention(q, k, v, cu_tensor(c), frame=frame), got[0])       # the same without statistics
 
 
+@pytest.mark.parametrize('lengths,h,d,frame,small', [([2000, 30], 2, 64, 1, 8), ([1500], 3, 32, 0, 10), ([400, 700] * 6, 8, 64, 0, 8),
+                                                     ([2600, 45], 16, 128, 1, 6), ([40, 3], 2, 64, 1, 12)], ids=['split', 'all keys', 'wide', 'pairs', 'short'])
+def test_fp16_gradients_far_below_one(lengths, h, d, frame, small):
+    """Output gradients of 2^-6 to 2^-12: dS lies where fp16 has few bits or none, the gradients themselves do not."""
+    c, dtype = cum(lengths), torch.float16
+    q, k, v = (randn(c[-1], h, d, dtype=dtype, seed=395 + i) for i in range(3))
+    do = randn(c[-1], h, d, dtype=dtype, seed=399, scale=2.0 ** -small)
+    got = run_packed(q, k, v, cu_tensor(c), frame, do)
+    for x, nm in zip(got[1:], ('dq', 'dk', 'dv')):
+        x = x[:, -1:]
+        y = OS.packed(q[:, -1:], k[:, -1:], v[:, -1:], c, frame, do=do[:, -1:])[nm]
+        # roundings of the operand, of the result and of the output that delta reads, none above 2^-11, random in sign; elements below
+        # 2^-14 round to steps of 2^-24
+        error = (x.double().cpu() - y).norm()
+        assert error <= 3 * 2.0 ** -11 / math.sqrt(3) * y.norm() + 2.0 ** -25 * math.sqrt(y.numel()), (nm, error / y.norm())
+
+
 @pytest.mark.parametrize('dtype,lengths,hq,hk,d,frame', [
     (torch.bfloat16, [6000, 70], 8, 4, 64, 1),       # 408 workgroups of 128 rows: all on the card at once, two rounds there and back
     (torch.bfloat16, [2600, 45], 12, 4, 96, 1),      # 288: the second round is a part of one

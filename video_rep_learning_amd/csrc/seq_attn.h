@@ -664,6 +664,10 @@ struct RowMax {
   }
 };
 
+// The backward's probabilities in fp16 carry this power of two (in the rows' exponent offsets, so it costs nothing): of sequences of ten
+// thousands of tokens they lie where fp16 has few bits, and they are at most 1.
+constexpr int PSHIFT = 15;
+
 // union of the four waves' spans (a barrier inside)
 __device__ __forceinline__ Span block_span(const WaveSpan& ws, int* s_span, int lane, int wave, int nw) {
   if (lane == 0) { s_span[2 * wave] = ws.any.hi > 0 ? ws.any.lo : 0x7fffffff; s_span[2 * wave + 1] = ws.any.hi; }

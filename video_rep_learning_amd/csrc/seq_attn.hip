@@ -123,11 +123,11 @@ struct Fwd {
 };
 
 // What the backward needs to have the same probabilities again.  fp32: the exponent's offset and 1 / l, applied as in the forward (one
-// log2-sum would round at the size of its integer part: 1e-6 of a probability); 16-bit: one offset that holds both.
+// log2-sum would round at the size of its integer part: 1e-6 of a probability); 16-bit: one offset that holds both (fp16: and PSHIFT).
 template <int DT>
 __device__ __forceinline__ void store_stat(const FwdArgs& a, int head, int row, float nm, float l, bool some) {
   const size_t at = (size_t)head * a.T + row;
-  a.stat[at] = !some ? NEG_INF : DT == MVF_F32 ? nm : nm - __builtin_amdgcn_logf(l);
+  a.stat[at] = !some ? NEG_INF : DT == MVF_F32 ? nm : nm - __builtin_amdgcn_logf(l) + (DT == MVF_F16 ? PSHIFT : 0);
   a.stat[(size_t)a.Hq * a.T + at] = some ? 1.0f / l : 0.f;
 }
 

@@ -29,7 +29,8 @@ struct BwdArgs {
   int parts;                           // workgroups that share a group's heads
   char *dq, *dk, *dv;                  // [T, Hq, D], [T, Hk, D] x 2
   int T, Hq, Hk, D, frame, ntiles, level;
-  float c, scale;
+  float c, scale;                      // scale * log2(e); scale over 2^PSHIFT
+  float pinv;                          // 1 over 2^PSHIFT
 };
 
 // a row as the B operand's fragments.  (A row of no sequence may hold anything: it stays in its own lanes and is not stored.)
@@ -61,6 +62,45 @@ __device__ __forceinline__ void store_rows(char* base, size_t row_elems, const f
 
 // the fp32 format of the partial sums
 typedef Op<MVF_F32> Part;
+
+// fp16 holds 2^-14 to 2^16 with all of its bits, and dS = P (dP - delta) of a long sequence lies below.  A column (an owned row, the pair of
+// lanes that holds it) therefore enters its product multiplied with a power of two of its own, which follows the largest dS so
+// far: it is brought to 2^10 .. 2^11, and again only when one passes 2^15 (the sums follow; all of this is exact).
+template <int DT>
+struct DsScale {
+  float f = 0x1p30f;       // smaller dS than 2^-15 leave it
+  template <int N>
+  __device__ __forceinline__ void fit(f32x16_t& x, f32x16_t (&acc)[N]) {
+    if constexpr (DT == MVF_F16) {
+      float mx = 0.f, top[5];
+#pragma unroll
+      for (int e = 0; e < 5; ++e) top[e] = fmaxf(fmaxf(fabsf(x[3 * e]), fabsf(x[3 * e + 1])), fabsf(x[3 * e + 2]));
+      mx = fmaxf(fmaxf(fmaxf(top[0], top[1]), top[2]), fmaxf(fmaxf(top[3], top[4]), fabsf(x[15])));
+      if (__builtin_expect(__builtin_amdgcn_ballot_w64(mx * f > 32768.f) != 0, 0)) {
+        mx = pair_max(mx);
+        const float to = mx * f > 32768.f && mx < -NEG_INF ? ldexpf(1.f, 11 - __builtin_amdgcn_frexp_expf(mx)) : f;
+        const float by = to / f;                  // (powers of two)
+        f = to;
+#pragma unroll
+        for (int dt = 0; dt < N; ++dt)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) acc[dt][e] *= by;
+      }
+#pragma unroll
+      for (int e = 0; e < 16; ++e) x[e] *= f;
+    }
+  }
+  template <int N>
+  __device__ __forceinline__ void undo(f32x16_t (&acc)[N]) const {
+    if constexpr (DT == MVF_F16) {
+      const float by = 1.f / f;
+#pragma unroll
+      for (int dt = 0; dt < N; ++dt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[dt][e] *= by;
+    }
+  }
+};
 
 // The waves' sums of the same 32 rows, added in order, out as [row][D].  All threads; barriers inside.
 template <class O, int DP>
@@ -98,6 +138,7 @@ struct Dq {
   int lane;
   uint32_t rpart, cpart;
   bool bad = false;        // a tile with masked places held a value that is not finite
+  DsScale<DT> ds;
 
   __device__ __forceinline__ void start(const BwdArgs& a, int head, int row, int lane_, bool write_delta) {
     lane = lane_;
@@ -149,6 +190,7 @@ struct Dq {
         s[e] = key >= own.lo && key < own.hi ? s[e] : 0.f;
       }
     }
+    ds.fit(s, dq);
     accumulate<O, DP>(dq, s, ck);
   }
   __device__ __forceinline__ void slow(const BwdArgs& a, const char* kb, const char* vb, int first, int step, int end) {
@@ -207,6 +249,7 @@ __global__ __launch_bounds__(256 * H, DT == MVF_F32 && DP > 32 ? H : 2) void pac
     for (int t = wave >> 2; t < R::KB / 32; t += H) f.any_tile(ws, ik + t * 32 * I::RB, ik + R::IMG + t * 32 * I::RB, b0 + 32 * t);
     buf = buf == 2 ? 0 : buf + 1;
   }
+  f.ds.undo(f.dq);
   if (f.bad) f.slow(a, kb, vb, span.lo + 32 * (wave >> 2), 32 * H, ws.any.hi);
   if constexpr (H == 2) {
     __syncthreads();
@@ -255,6 +298,7 @@ __global__ __launch_bounds__(256, 1) void packed_attn_dq_split_kernel(BwdArgs a)
     if (S::NB == 2) buf ^= 1;
     else if (more) issue(key0 + 128, 0);
   }
+  f.ds.undo(f.dq);
   if (f.bad) f.slow(a, kb, vb, ws.any.lo + wave * 32, 128, ws.any.hi);
   if (f.own.hi == 0) {           // rows of no sequence rode along in unmasked tiles
 #pragma unroll
@@ -279,6 +323,7 @@ struct Dkv {
   int lane;
   uint32_t rpart, cpart;
   bool bad = false;        // a tile with masked places held a value that is not finite
+  DsScale<DT> ds;
 
   __device__ __forceinline__ void start(const BwdArgs& a, int kh, int row, int lane_, char* own_v) {
     lane = lane_;
@@ -338,6 +383,7 @@ struct Dkv {
       }
     }
     accumulate<O, DP>(dv, s, cd);
+    ds.fit(dp, dk);
     accumulate<O, DP>(dk, dp, cq);
   }
   // over tiles it = first, first + step, ... of (head h0 + .. of g, 32-query tile, of which a head has a multiple of `per`)
@@ -434,6 +480,7 @@ __global__ __launch_bounds__(256 * H, DT == MVF_F32 && DP > 32 ? H : 2) void pac
     b0 += R::KB;
     if (b0 >= span.hi) b0 = span.lo;
   }
+  f.ds.undo(f.dk);
   if (f.bad) f.slow(a, kh, row, h0, g, {span.lo, ws.any.hi}, wave >> 2, H, H);
   if constexpr (H == 2) {
     char* half = smem + (wave & 3) * HALF<DP> + lane * 16;
@@ -452,15 +499,15 @@ __global__ __launch_bounds__(256 * H, DT == MVF_F32 && DP > 32 ? H : 2) void pac
     const size_t plane = (size_t)a.T * a.Hk * a.D;
     char* base = reinterpret_cast<char*>(a.part + 2 * part * plane);
     store_rows<Part, DP>(base, at, f.dk, a.scale, f.own.hi > 0, a.D, lane >> 5);
-    store_rows<Part, DP>(base, plane + at, f.dv, 1.f, f.own.hi > 0, a.D, lane >> 5);
+    store_rows<Part, DP>(base, plane + at, f.dv, a.pinv, f.own.hi > 0, a.D, lane >> 5);
   } else {
     store_rows<O, DP>(a.dk, at, f.dk, a.scale, f.own.hi > 0, a.D, lane >> 5);
-    store_rows<O, DP>(a.dv, at, f.dv, 1.f, f.own.hi > 0, a.D, lane >> 5);
+    store_rows<O, DP>(a.dv, at, f.dv, a.pinv, f.own.hi > 0, a.D, lane >> 5);
   }
 }
 
 template <int DT, int DP, bool PAD>
-__global__ __launch_bounds__(256, 1) void packed_attn_dkv_split_kernel(BwdArgs a) {
+__global__ __launch_bounds__(256, DT != MVF_F32 && DP <= 64 ? 2 : 1) void packed_attn_dkv_split_kernel(BwdArgs a) {
   typedef Op<DT> O;
   typedef SplitTiles<O, DP, 4> S;
   constexpr int NF = planes(DT) * 32, NSP = (NF + 63) / 64, SB = NSP * 256;
@@ -502,6 +549,7 @@ __global__ __launch_bounds__(256, 1) void packed_attn_dkv_split_kernel(BwdArgs a
     if (S::NB == 2) buf ^= 1;
     else if (more) issue(it + 4, 0);
   }
+  f.ds.undo(f.dk);
   if (f.bad) f.slow(a, kh, row, h0, g, ws.any, wave, 4);
   if (f.own.hi == 0) {
 #pragma unroll
@@ -513,10 +561,10 @@ __global__ __launch_bounds__(256, 1) void packed_attn_dkv_split_kernel(BwdArgs a
     const size_t plane = (size_t)a.T * a.Hk * a.D;
     float* base = a.part + 2 * part * plane + (size_t)kh * a.D;
     store_joined<Part, DP>(so, f.dk, reinterpret_cast<char*>(base), row0, rows, (long)a.Hk * a.D, a.scale, a.D, wave, lane);
-    store_joined<Part, DP>(so, f.dv, reinterpret_cast<char*>(base + plane), row0, rows, (long)a.Hk * a.D, 1.f, a.D, wave, lane);
+    store_joined<Part, DP>(so, f.dv, reinterpret_cast<char*>(base + plane), row0, rows, (long)a.Hk * a.D, a.pinv, a.D, wave, lane);
   } else {
     store_joined<O, DP>(so, f.dk, a.dk + (size_t)kh * a.D * O::SZ, row0, rows, (long)a.Hk * a.D, a.scale, a.D, wave, lane);
-    store_joined<O, DP>(so, f.dv, a.dv + (size_t)kh * a.D * O::SZ, row0, rows, (long)a.Hk * a.D, 1.f, a.D, wave, lane);
+    store_joined<O, DP>(so, f.dv, a.dv + (size_t)kh * a.D * O::SZ, row0, rows, (long)a.Hk * a.D, a.pinv, a.D, wave, lane);
   }
 }
 
@@ -638,6 +686,6 @@ extern "C" int mvf_packed_attn_bwd(int dtype, const void* q, long ldq, long hsq,
   MVF_CHECK_ARG(tile_bound<32>(T, n_seqs) * Hk * parts < (1l << 30) && (size_t)T * Hk * D / 512 < (1ul << 31));
   BwdArgs a = {(const char*)q, (const char*)k, (const char*)v, s[0], s[1], s[2], s[3], s[4], s[5], cu_seqlens, n_seqs, (const char*)out,
                (const char*)d_out, stat, delta, delta + ((size_t)Hq * T + 3) / 4 * 4, parts, (char*)dq, (char*)dk, (char*)dv, T, Hq, Hk, D,
-               frame, 0, 0, scale * LOG2E, scale};
+               frame, 0, 0, scale * LOG2E, scale * (dtype == MVF_F16 ? 1.f / (1 << PSHIFT) : 1.f), dtype == MVF_F16 ? 1.f / (1 << PSHIFT) : 1.f};
   return dtype == MVF_F32 ? launch_d<MVF_F32>(a, st) : dtype == MVF_BF16 ? launch_d<MVF_BF16>(a, st) : launch_d<MVF_F16>(a, st);
 }
