@@ -660,6 +660,12 @@ int mvf_rotary_append(int dtype, const void* q, long ldq, long hsq, const void* 
 int mvf_packed_attn_fwd(int dtype, const void* q, long ldq, long hsq, const void* k, long ldk, long hsk, const void* v, long ldv, long hsv,
                         const int* cu_seqlens, int n_seqs, void* out, float* stat, int T, int Hq, int Hk, int D, int frame, float scale,
                         hipStream_t stream);
+/* The same, and rest (NULL, or [T, Hq, D] of the same 16-bit type; not touched in fp32): what the rounding of out took away.  The backward
+ * takes rowsum(d_out out) from both: the rounding of out is small beside out, but not beside what the gradients of short sequences
+ * leave of that sum. */
+int mvf_packed_attn_fwd_rest(int dtype, const void* q, long ldq, long hsq, const void* k, long ldk, long hsk, const void* v, long ldv,
+                             long hsv, const int* cu_seqlens, int n_seqs, void* out, void* rest, float* stat, int T, int Hq, int Hk, int D,
+                             int frame, float scale, hipStream_t stream);
 /* Its gradients: out, d_out [T, Hq, D], stat as the forward left it; dq [T, Hq, D], dk, dv [T, Hk, D] (summed over the query heads of a
  * group in a fixed order; no atomics).  workspace: mvf_packed_attn_bwd_workspace_bytes, not shared between calls that can run at the
  * same time. */
@@ -668,6 +674,10 @@ int mvf_packed_attn_bwd(int dtype, const void* q, long ldq, long hsq, const void
                         const int* cu_seqlens, int n_seqs, const void* out, const void* d_out, const float* stat, void* workspace,
                         size_t ws_bytes, void* dq, void* dk, void* dv, int T, int Hq, int Hk, int D, int frame, float scale,
                         hipStream_t stream);
+int mvf_packed_attn_bwd_rest(int dtype, const void* q, long ldq, long hsq, const void* k, long ldk, long hsk, const void* v, long ldv,
+                             long hsv, const int* cu_seqlens, int n_seqs, const void* out, const void* rest, const void* d_out,
+                             const float* stat, void* workspace, size_t ws_bytes, void* dq, void* dk, void* dv, int T, int Hq, int Hk,
+                             int D, int frame, float scale, hipStream_t stream);
 /* Attention of the last n_new tokens of each of B streams, positions lengths[b] - n_new .. lengths[b] - 1, over the stream's pages.
  * q: element (b, i, h, d) at b * q_batch + i * q_token + h * q_head + d; out [B, n_new, Hq, D]; block_table [B][table_width].  A position
  * before 0 sees nothing (unless frame = 0) and gets zeros.  workspace: mvf_paged_attn_workspace_bytes (0: NULL will do), not shared between

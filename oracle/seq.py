@@ -40,7 +40,7 @@ def limit(p, frame, length):
     return length if frame == 0 else max(0, min(length, (p // frame + 1) * frame))
 
 
-def attend(q, k, v, limits, scale, dtype, do=None, low=False):
+def attend(q, k, v, limits, scale, dtype, do=None, low=False, fine=False):
     """One head: q [n, D], k, v [L, D], limits [n] keys seen by each row; do [n, D].  -> dict of 64-bit results and of bounds.
 
     The bounds follow the kernels' roundings.  A score is a 32-bit sum of D products (at most D / 8 + 8 dependent additions); the exponent
@@ -50,11 +50,15 @@ def attend(q, k, v, limits, scale, dtype, do=None, low=False):
     product as the 16-bit operand and the rounded rest (at most up of it, so the two are off by up * up).
 
     Weights are powers of two of s - m, m no larger than the row's maximum, so their sum is at least 1 and a weight that is flushed to 0
-    takes at most FLUSH from a probability; so does every term of a sum that lies below it."""
+    takes at most FLUSH from a probability; so does every term of a sum that lies below it.
+
+    fine: the training pass over short sequences.  Probabilities and dS enter their products with their rests (up * up); delta reads the
+    output and the rounded rest of its rounding; fp16 operands carry powers of two, so that probabilities lose 2^-40 at most and dS 2^-35
+    of its column's largest (2^-33 here: one head's largest for its group's)."""
     q, k, v = (t.detach().double().cpu() for t in (q, k, v))
     n, L, D = q.shape[0], k.shape[0], q.shape[1]
     u = HALF_STEP[dtype]
-    up, tiny = (0.0, 0.0) if dtype == torch.float32 else (u * u if low else u, TINY[dtype])
+    up, tiny = (0.0, 0.0) if dtype == torch.float32 else (u * u if low or fine else u, TINY[dtype])
     lost = max(tiny * 0.5, FLUSH)
     seen = torch.arange(L)[None] < torch.as_tensor(limits)[:, None]
     if L == 0:
@@ -75,6 +79,7 @@ def attend(q, k, v, limits, scale, dtype, do=None, low=False):
     ep = 2 * es + (L / 16 + 40) * U32 + 2.0 ** -22                          # relative, of a probability
     ones = seen.double()
     out_b = (p * (up + ep)) @ v.abs() + lost * (ones @ v.abs()) + FLUSH * L + (L / 16 + 40) * U32 * (p @ v.abs())
+    unrounded = out_b
     out_b = out_b + u * (out.abs() + out_b) + TINY[dtype]
     r = dict(out=out, out_b=out_b)
     if do is None:
@@ -83,14 +88,18 @@ def attend(q, k, v, limits, scale, dtype, do=None, low=False):
     dp = do @ v.t()
     delta = (do * out).sum(1, keepdim=True)
     ds = p * (dp - delta)
+    lost_s = lost
+    if fine:
+        lost, lost_s = 2.0 ** -40, 2.0 ** -33 * ds.abs().max() + FLUSH
     pb = p * (up + ep) + lost * ones
     N = n / 16 + 40
     dv = p.t() @ do
     dv_b = pb.t() @ do.abs() + FLUSH * n + N * U32 * (p.t() @ do.abs())
-    delta_b = (do.abs() * (out_b + D * U32 * out.abs())).sum(1, keepdim=True)
+    read = unrounded + up * (out.abs() + unrounded) + TINY[dtype] if fine else out_b
+    delta_b = (do.abs() * (read + D * U32 * out.abs())).sum(1, keepdim=True)
     dp_b = (D / 8 + 8) * U32 * (do.abs() @ v.abs().t())
     ds_b = p * (dp_b + delta_b + 2 * U32 * (dp.abs() + delta.abs())) + (p * ep + FLUSH * ones) * (dp - delta).abs()
-    ds_b = ds_b + up * (ds.abs() + ds_b) + lost * ones
+    ds_b = ds_b + up * (ds.abs() + ds_b) + lost_s * ones
     dq, dk = ds @ k * scale, ds.t() @ q * scale
     dq_b = (ds_b @ k.abs() + FLUSH * L + (L / 16 + 40) * U32 * (ds.abs() @ k.abs())) * scale
     dk_b = (ds_b.t() @ q.abs() + FLUSH * n + N * U32 * (ds.abs().t() @ q.abs())) * scale
@@ -98,8 +107,9 @@ def attend(q, k, v, limits, scale, dtype, do=None, low=False):
     return r
 
 
-def packed(q, k, v, cu, frame, scale=None, do=None):
-    """Attention over packed sequences: q [T, Hq, D], k, v [T, Hk, D], cu: list of bounds -> dict of [T, H, D] results and bounds."""
+def packed(q, k, v, cu, frame, scale=None, do=None, fine=False):
+    """Attention over packed sequences: q [T, Hq, D], k, v [T, Hk, D], cu: list of bounds -> dict of [T, H, D] results and bounds.  fine: as
+    in attend()."""
     T, Hq, D = q.shape
     Hk, dt = k.shape[1], q.dtype
     g, scale = Hq // Hk, D ** -0.5 if scale is None else scale
@@ -111,7 +121,7 @@ def packed(q, k, v, cu, frame, scale=None, do=None):
     for a, b in zip(cu[:-1], cu[1:]):
         limits = [limit(p, frame, b - a) for p in range(b - a)]
         for h in range(Hq):
-            one = attend(q[a:b, h], k[a:b, h // g], v[a:b, h // g], limits, scale, dt, None if do is None else do[a:b, h])
+            one = attend(q[a:b, h], k[a:b, h // g], v[a:b, h // g], limits, scale, dt, None if do is None else do[a:b, h], fine=fine)
             for nm in names:
                 i = h // g if nm in ('dk', 'dv') else h
                 r[nm][a:b, i] += one[nm]

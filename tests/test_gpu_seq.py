@@ -176,6 +176,22 @@ def test_packed_attention_and_its_gradients(dtype, lengths, hq, hk, d, frame):
         assert torch.equal(ops.packed_attention(q, k, v, cu_tensor(c), frame=frame), got[0])       # the same without statistics
 
 
+@pytest.mark.parametrize('dtype', DTYPES[1:], ids=IDS[1:])
+@pytest.mark.parametrize('lengths,h,d,frame', [([2, 2, 3, 1, 2], 1, 40, 1), ([2] * 20, 3, 80, 0), ([31, 5, 128, 2, 64], 2, 64, 1), ([4] * 30, 2, 128, 3),
+                                               ([100, 3, 20] * 8, 2, 96, 1), ([40, 2, 9] * 40, 12, 64, 1), ([30, 3, 128] * 20, 16, 32, 0)],
+                         ids=['pairs', 'couples', 'split', 'fours', 'split 96', 'wide', 'wide 32'])
+def test_gradients_of_short_sequences_keep_their_bits(dtype, lengths, h, d, frame):
+    """What is left of dP - delta in short sequences is small beside both: delta must not come from the rounded output alone, and dS must
+    not lose what 16 bits take."""
+    c = cum(lengths)
+    q, k, v = (randn(c[-1], h, d, dtype=dtype, seed=390 + i, scale=s) for i, s in enumerate((1.5, 1.0, 1.0)))
+    do = randn(c[-1], h, d, dtype=dtype, seed=394)
+    got = run_packed(q, k, v, cu_tensor(c), frame, do)
+    want = OS.packed(q, k, v, c, frame, do=do, fine=True)
+    for x, nm in zip(got, ('out', 'dq', 'dk', 'dv')):
+        within(x, want[nm], want[nm + '_b'], nm)
+
+
 @pytest.mark.parametrize('lengths,h,d,frame,small', [([2000, 30], 2, 64, 1, 8), ([1500], 3, 32, 0, 10), ([400, 700] * 6, 8, 64, 0, 8),
                                                      ([2600, 45], 16, 128, 1, 6), ([40, 3], 2, 64, 1, 12)], ids=['split', 'all keys', 'wide', 'pairs', 'short'])
 def test_fp16_gradients_far_below_one(lengths, h, d, frame, small):
@@ -657,6 +673,15 @@ def test_paged_attention_carries_infinite_values(dtype, bad, length, width):
         assert (out[0, sees][..., 5] == bad).all()
         other = [i for i in range(32) if i != 5]
         within(out[..., other], want[..., other], bound[..., other], 'other channels')
+
+
+@pytest.mark.parametrize('dtype', DTYPES, ids=IDS)
+@pytest.mark.parametrize('n', [20, 90, 300])
+def test_value_gradients_carry_infinite_output_gradients(dtype, n):
+    q, k, v, do = (randn(n, 2, 32, dtype=dtype, seed=400 + i, scale=0.5) for i in range(4))
+    do[n // 2, :, 5] = math.inf
+    got = run_packed(q, k, v, cu_tensor([0, n]), 1, do)
+    assert (got[3][:n // 2 + 1, :, 5] == math.inf).all() and torch.isfinite(got[3][n // 2 + 1:]).all()
 
 
 def test_paged_attention_far_pages():

@@ -241,6 +241,22 @@ def test_packed_entry_points_refuse(lib, name, value):
     assert lib.mvf_packed_attn_bwd(*head, P, P, P, 1 << 40, P, P, P, *tail, None) == 10001
 
 
+def test_packed_entry_points_with_rest_refuse_what_the_others_do(lib):
+    def fwd(rest=P, **kw):
+        a = dict(FWD, **kw)
+        v = list(a.values())
+        at = list(a).index('out') + 1
+        return lib.mvf_packed_attn_fwd_rest(*v[:at], rest, *v[at:], None)
+
+    def bwd(rest=P, d_out=P, ws=1 << 40, **kw):
+        a = dict(FWD, **kw)
+        head = [a[n] for n in ('dtype', 'q', 'ldq', 'hsq', 'k', 'ldk', 'hsk', 'v', 'ldv', 'hsv', 'cu', 'n', 'out')]
+        return lib.mvf_packed_attn_bwd_rest(*head, rest, d_out, P, P, ws, P, P, P, *(a[n] for n in ('T', 'Hq', 'Hk', 'D', 'frame', 'scale')), None)
+    for name, value in BAD_ATTN:
+        assert fwd(**{name: value}) == 10001 and bwd(**{name: value}) == 10001, name
+    assert fwd(rest=P + 8) == 10001 and bwd(rest=P + 8) == 10001 and bwd(d_out=None) == 10001 and bwd(ws=8) == 10001
+
+
 @pytest.mark.parametrize('d', [0, 12, 136, -8])
 def test_head_sizes_are_declined(lib, d):
     assert lib.mvf_packed_attn_fwd(*dict(FWD, D=d).values(), None) == 10002

@@ -123,8 +123,10 @@ SIGNATURES = {
     'mvf_rotary': 'ipllpll' + 'pip' + 'iiiii' + 'pp' + 'iiiip',
     'mvf_rotary_append': 'ipllpllpll' + 'pip' + 'iiii' + 'ppp' + 'pii' + 'pp' + 'ii' + 'iiiip',
     'mvf_packed_attn_fwd': 'ipllpllpll' + 'pi' + 'pp' + 'iiiiifp',
+    'mvf_packed_attn_fwd_rest': 'ipllpllpll' + 'pi' + 'ppp' + 'iiiiifp',
     'mvf_packed_attn_bwd_workspace_bytes': 'iiiiii',
     'mvf_packed_attn_bwd': 'ipllpllpll' + 'pi' + 'ppppz' + 'ppp' + 'iiiiifp',
+    'mvf_packed_attn_bwd_rest': 'ipllpllpll' + 'pi' + 'pppppz' + 'ppp' + 'iiiiifp',
     'mvf_paged_attn_workspace_bytes': 'iiiiiii',
     'mvf_paged_attn': 'iplllppppppz' + 'iiiiiiiiifp',
     'mvf_augment_workspace_bytes': 'iii',

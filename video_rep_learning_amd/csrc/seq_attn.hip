@@ -10,7 +10,7 @@
 //   split:  a workgroup owns 32 rows, each wave walks every fourth (or eighth) 32-key tile by itself, the partial softmaxes are joined at
 //           the end: four times as many workgroups and a quarter of the dependent steps, for four times the key traffic.
 // The weights are rounded to the operands' format for the second product (relative 2^-9 in bf16, random in sign, so the sum is off by that
-// much of its size, as the rounding of the result is); their sum is taken before, in 32 bits.
+// much of its size, as the rounding of the result is; not in short walks: short_walk()); their sum is taken before, in 32 bits.
 // Measured: 2 x 8192 causal bf16, 16 query heads of 128 on 4: 0.60 ms, 916 TFLOP/s of visible pairs (a large bf16 matrix product: 1130 to
 // 1150); 32 x 785, 12 of 64: 114 us, 530; 8 x 1440 fp32 causal by 6, 8 of 32: 119 us, 72 (a large fp32 product: 148).  Bound by the waves'
 // own chains: at D 96 the matrix pipe is busy 24 % of the cycles, the vector unit 31 %, and 32 % of the waves' time goes into waits.
@@ -29,7 +29,41 @@ struct FwdArgs {
   float* stat;                         // NULL, or [2][Hq][T]: see finish()
   int T, Hq, Hk, D, frame, ntiles, level;
   float c;                             // scale * log2(e)
+  char* rest;                          // NULL, or (16-bit types) [T, Hq, D]: what out's rounding took away
 };
+
+// four channels of a row of the result
+template <class O>
+__device__ __forceinline__ void store_out(const FwdArgs& a, size_t at, float x, float y, float z, float w) {
+  typedef typename O::E E;
+  E* out = reinterpret_cast<E*>(a.out) + at;
+  if (O::SZ == 2 && a.rest != nullptr) O::store4_rest(out, reinterpret_cast<E*>(a.rest) + at, x, y, z, w);
+  else O::store4(out, x, y, z, w);
+}
+
+// 32 channels of a wave's rows, the first `left` of them: 16-bit formats trade quarters between the lanes of a pair, 16 bytes a store
+template <class O>
+__device__ __forceinline__ void store_tile(const FwdArgs& a, size_t at, int left, const f32x16_t& x, int lane) {
+  const int hh = lane >> 5;
+  if constexpr (O::SZ == 2) {
+#pragma unroll
+    for (int e = 0; e < 4; e += 2) {
+      u32x4_t out, rest;
+      O::pack8_rest(x, e, out, rest);
+      const int d = 8 * (e + hh);
+      if (d < left) {
+        *reinterpret_cast<u32x4_t*>(reinterpret_cast<typename O::E*>(a.out) + at + d) = out;
+        if (a.rest != nullptr) *reinterpret_cast<u32x4_t*>(reinterpret_cast<typename O::E*>(a.rest) + at + d) = rest;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int d = 8 * e + 4 * hh;
+      if (d < left) O::store4(reinterpret_cast<typename O::E*>(a.out) + at + d, x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
+    }
+  }
+}
 
 template <int DT, int DP>
 struct Fwd {
@@ -43,6 +77,7 @@ struct Fwd {
   int lane;
   uint32_t rpart, cpart;
   bool bad = false;        // a tile with masked places held a value that is not finite, or the scores are steep
+  bool low = false;        // the weights' second operand: see accumulate()
 
   __device__ __forceinline__ void start(const FwdArgs& a, int head, int row, int lane_) {
     lane = lane_;
@@ -93,7 +128,7 @@ struct Fwd {
       s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], c, st.nm));
       st.l += s[e];
     }
-    accumulate<O, DP>(o, s, cl);
+    accumulate_if<O, DP>(low, o, s, cl);
   }
   // the same rows over 32-key tiles first, first + step, ..., one visible pair at a time
   __device__ __forceinline__ void slow(const FwdArgs& a, const char* kb, const char* vb, int first, int step, int end) {
@@ -133,7 +168,7 @@ __device__ __forceinline__ void store_stat(const FwdArgs& a, int head, int row, 
 
 // H = 2: eight waves, two for each 32 rows, which take every block's tiles in turn and join their halves at the end
 template <int DT, int DP, bool PAD, int H>
-__global__ __launch_bounds__(256 * H, DT == MVF_F32 && DP > 64 ? H : 2) void packed_attn_fwd_kernel(FwdArgs a) {
+__global__ __launch_bounds__(256 * H, DT == MVF_F32 && DP > 64 ? H : DT != MVF_F32 && DP == 128 && H == 1 ? 3 : 2) void packed_attn_fwd_kernel(FwdArgs a) {
   typedef Op<DT> O;
   typedef Img<O, DP> I;
   typedef Ring<O, DP, 3, 4 * H> R;
@@ -150,6 +185,7 @@ __global__ __launch_bounds__(256 * H, DT == MVF_F32 && DP > 64 ? H : 2) void pac
   f.start(a, head, row, lane);                 // (a row of no sequence may hold anything: it stays in its own lanes and is not stored)
   f.own = keys_of(sequence_of(own, a.cu, a.n_seqs, a.T, row), a.frame, row);
   const WaveSpan ws = wave_span(f.own);
+  f.low = short_walk(ws);
   if constexpr (PAD) clear_lds(smem, R::NB * R::BUF);
   const Span span = block_span(ws, s_span, lane, wave, 4 * H);
   const int g = a.Hq / a.Hk;
@@ -171,6 +207,7 @@ __global__ __launch_bounds__(256 * H, DT == MVF_F32 && DP > 64 ? H : 2) void pac
     for (int t = wave >> 2; t < R::KB / 32; t += H) f.any_tile(ws, ik + t * 32 * I::RB, ik + R::IMG + t * 32 * I::RB, b0 + 32 * t);
     buf = buf == 2 ? 0 : buf + 1;
   }
+  if (O::SZ == 2 && f.low) f.bad |= not_finite(f.o, f.own.hi > f.own.lo);
   if (f.bad) f.slow(a, kb, vb, span.lo + 32 * (wave >> 2), 32 * H, ws.any.hi);
   if constexpr (H == 2) {
     __syncthreads();
@@ -201,17 +238,13 @@ __global__ __launch_bounds__(256 * H, DT == MVF_F32 && DP > 64 ? H : 2) void pac
   const bool some = f.own.hi > f.own.lo && l != 0.f;          // (l is NaN where a score was)
   const float inv = some ? 1.0f / l : 0.f;
   if (a.stat != nullptr && lane < 32) store_stat<DT>(a, head, row, f.st.nm, l, some);
-  typename O::E* dst = reinterpret_cast<typename O::E*>(a.out) + ((size_t)row * a.Hq + head) * a.D;
+  const size_t at = ((size_t)row * a.Hq + head) * a.D;
 #pragma unroll
-  for (int dt = 0; dt < DP / 32; ++dt)
+  for (int dt = 0; dt < DP / 32; ++dt) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int d = 32 * dt + 8 * e + 4 * (lane >> 5);
-      if (d < a.D) {
-        if (some) O::store4(dst + d, f.o[dt][4 * e] * inv, f.o[dt][4 * e + 1] * inv, f.o[dt][4 * e + 2] * inv, f.o[dt][4 * e + 3] * inv);
-        else O::store4(dst + d, 0.f, 0.f, 0.f, 0.f);
-      }
-    }
+    for (int e = 0; e < 16; ++e) f.o[dt][e] = some ? f.o[dt][e] * inv : 0.f;
+    store_tile<O>(a, at + 32 * dt, a.D - 32 * dt, f.o[dt], lane);
+  }
 }
 
 template <int DT, int DP, bool PAD, int NW>
@@ -231,6 +264,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void packed_attn_fwd_split_kernel(
   f.start(a, head, row, lane);                 // (a row of no sequence may hold anything: it stays in its own lanes and is not stored)
   f.own = keys_of(sequence_of(own, a.cu, a.n_seqs, a.T, row), a.frame, row);
   const WaveSpan ws = wave_span(f.own);
+  f.low = short_walk(ws);
   if constexpr (PAD) clear_lds(smem, NW * S::NB * S::BUF);
   const int g = a.Hq / a.Hk;
 #pragma unroll
@@ -253,6 +287,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void packed_attn_fwd_split_kernel(
     if (S::NB == 2) buf ^= 1;
     else if (more) issue(key0 + 32 * NW, 0);
   }
+  if (O::SZ == 2 && f.low) f.bad |= not_finite(f.o, f.own.hi > f.own.lo);
   if (f.bad) f.slow(a, kb, vb, ws.any.lo + wave * 32, 32 * NW, ws.any.hi);
   if (f.own.hi == 0) {           // rows of no sequence rode along in unmasked tiles
     f.st = RowMax();
@@ -266,8 +301,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void packed_attn_fwd_split_kernel(
     const bool some = l != 0.f;
     const float inv = some ? 1.0f / l : 0.f;
     if (stat && d == 0) store_stat<DT>(a, head, row0 + i, -mx, l, some);
-    O::store4(reinterpret_cast<typename O::E*>(a.out) + ((size_t)(row0 + i) * a.Hq + head) * a.D + d, acc[0] * inv, acc[1] * inv,
-              acc[2] * inv, acc[3] * inv);
+    store_out<O>(a, ((size_t)(row0 + i) * a.Hq + head) * a.D + d, acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
   });
 }
 
@@ -319,6 +353,13 @@ int launch_d(const FwdArgs& a, hipStream_t st) {
 extern "C" int mvf_packed_attn_fwd(int dtype, const void* q, long ldq, long hsq, const void* k, long ldk, long hsk, const void* v,
                                    long ldv, long hsv, const int* cu_seqlens, int n_seqs, void* out, float* stat, int T, int Hq, int Hk,
                                    int D, int frame, float scale, hipStream_t st) {
+  return mvf_packed_attn_fwd_rest(dtype, q, ldq, hsq, k, ldk, hsk, v, ldv, hsv, cu_seqlens, n_seqs, out, nullptr, stat, T, Hq, Hk, D, frame,
+                                  scale, st);
+}
+
+extern "C" int mvf_packed_attn_fwd_rest(int dtype, const void* q, long ldq, long hsq, const void* k, long ldk, long hsk, const void* v,
+                                        long ldv, long hsv, const int* cu_seqlens, int n_seqs, void* out, void* rest, float* stat, int T,
+                                        int Hq, int Hk, int D, int frame, float scale, hipStream_t st) {
   MVF_CHECK_ARG(dtype == MVF_F32 || dtype == MVF_BF16 || dtype == MVF_F16);
   MVF_CHECK_ARG(q && k && v && cu_seqlens && out && T > 0 && n_seqs > 0 && Hk > 0 && Hq > 0 && Hq % Hk == 0 && frame >= 0);
   MVF_CHECK_ARG(scale > 0.f && scale < 1e30f && T < (1 << 30) && tile_bound<32>(T, n_seqs) * Hq < (1l << 30));
@@ -326,8 +367,8 @@ extern "C" int mvf_packed_attn_fwd(int dtype, const void* q, long ldq, long hsq,
   const long sz = dtype == MVF_F32 ? 4 : 2;
   const long s[6] = {ldq * sz, hsq * sz, ldk * sz, hsk * sz, ldv * sz, hsv * sz};
   for (long x : s) MVF_CHECK_ARG(x > 0 && x % 16 == 0);
-  MVF_CHECK_ARG((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) & 15) == 0);
+  MVF_CHECK_ARG((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out | (uintptr_t)rest) & 15) == 0);
   FwdArgs a = {(const char*)q, (const char*)k, (const char*)v, s[0], s[1], s[2], s[3], s[4], s[5], cu_seqlens, n_seqs, (char*)out, stat,
-               T, Hq, Hk, D, frame, 0, 0, scale * LOG2E};
+               T, Hq, Hk, D, frame, 0, 0, scale * LOG2E, (char*)rest};
   return dtype == MVF_F32 ? launch_d<MVF_F32>(a, st) : dtype == MVF_BF16 ? launch_d<MVF_BF16>(a, st) : launch_d<MVF_F16>(a, st);
 }

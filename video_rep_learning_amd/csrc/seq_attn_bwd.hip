@@ -5,9 +5,10 @@
 //   dK/dV:  owns 32 keys per wave, streams Q and dO of every head of the group (the sum over the group stays in registers)
 // Each in the three forms of the forward: wide (four waves of 32 rows share the streamed blocks), pairs (eight waves do) and split (one
 // 32-row tile, every wave walks its own quarter of the streamed tiles, the four sums are added at the end in a fixed order).
-// P and dS are rounded to the operands' format where they enter a product; the sums, delta and the row statistics are 32 bits.  In bf16 dS
-// (2^-9 relative, random in sign) and the rounding of the result give an error of sqrt(2) 1.7e-3 = 2.4e-3 of the gradient's size, and delta,
-// taken from the rounded output, the rest of the measured 2.5e-3.
+// P and dS are rounded to the operands' format where they enter a product (whole in short walks: short_walk()); the sums, delta and the row
+// statistics are 32 bits.  delta is taken from the output and what its rounding took away: from the rounded output alone it leaves
+// gradients of short sequences off by up to 30 roundings, of long ones by 1.55.  Errors in bf16: 1.7e-3 of the gradient's size in short
+// walks, one rounding, and in long ones, with dS's own (2^-9 relative, random in sign), sqrt(2) of that, 2.4e-3.
 // Measured, 2 x 8192 causal bf16, 16 query heads of 128 on 4: dQ 0.86 ms (960 TFLOP/s of its three products), dK / dV 1.29 ms (850 of its
 // four) and 25 us for the sum of the parts.  Bound by registers: dK / dV holds 2 x 32 x 128 sums and a wave's K rows, so two waves a SIMD
 // are all that fit, and their waits are not all covered.
@@ -22,7 +23,7 @@ struct BwdArgs {
   long ldq, hsq, ldk, hsk, ldv, hsv;   // token and head strides in BYTES
   const int* cu;
   int n_seqs;
-  const char *out, *d_out;             // [T, Hq, D]
+  const char *out, *rest, *d_out;      // [T, Hq, D]; rest may be NULL
   const float* stat;                   // [2][Hq][T] of the forward
   float* delta;                        // [Hq][T]
   float* part;                         // parts > 1: [parts][2 (dk, dv)][T][Hk][D]
@@ -127,6 +128,10 @@ __device__ __forceinline__ void store_joined(float* so, const f32x16_t (&x)[DP /
 }
 
 // ------------------------------------------------------------------------------------------------ dQ
+// Small heads take dS whole in long walks too: their keys' weighted mean is large beside the keys' spread, dS (whose sum is 0) takes it out of
+// the gradient but not out of dS's roundings (dQ of heads of 16 to 40: 1.5 to 1.6 of one rounding, whole 1.1; of 64: 1.47, for 9 % of the
+// backward's time).
+constexpr int SMALL_HEAD = 48;
 template <int DT, int DP>
 struct Dq {
   typedef Op<DT> O;
@@ -139,6 +144,7 @@ struct Dq {
   uint32_t rpart, cpart;
   bool bad = false;        // a tile with masked places held a value that is not finite
   DsScale<DT> ds;
+  bool low = false;        // dS's second operand: see accumulate()
 
   __device__ __forceinline__ void start(const BwdArgs& a, int head, int row, int lane_, bool write_delta) {
     lane = lane_;
@@ -157,6 +163,16 @@ struct Dq {
       if (d < a.D) x = *reinterpret_cast<const typename O::Frag*>(a.out + orow + d * O::SZ);
 #pragma unroll
       for (int j = 0; j < 8; ++j) dl = fmaf(O::get(dof[ks], j), O::get(x, j), dl);
+    }
+    if (O::SZ == 2 && a.rest != nullptr) {
+#pragma unroll
+      for (int ks = 0; ks < DP / 16; ++ks) {
+        const int d = 16 * ks + 8 * hh;
+        typename O::Frag x = {};
+        if (d < a.D) x = *reinterpret_cast<const typename O::Frag*>(a.rest + orow + d * O::SZ);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) dl = fmaf(O::get(dof[ks], j), O::get(x, j), dl);
+      }
     }
     dl = pair_sum(dl);
     const size_t at = (size_t)head * a.T + rr;
@@ -191,7 +207,7 @@ struct Dq {
       }
     }
     ds.fit(s, dq);
-    accumulate<O, DP>(dq, s, ck);
+    accumulate_if<O, DP>(low, dq, s, ck);
   }
   __device__ __forceinline__ void slow(const BwdArgs& a, const char* kb, const char* vb, int first, int step, int end) {
 #pragma unroll
@@ -230,6 +246,7 @@ __global__ __launch_bounds__(256 * H, DT == MVF_F32 && DP > 32 ? H : 2) void pac
   f.start(a, head, row, lane, row < own.end && wave < 4);
   f.own = keys_of(sequence_of(own, a.cu, a.n_seqs, a.T, row), a.frame, row);
   const WaveSpan ws = wave_span(f.own);
+  f.low = short_walk(ws) || a.D <= SMALL_HEAD;
   if constexpr (PAD) clear_lds(smem, R::NB * R::BUF);
   const Span span = block_span(ws, s_span, lane, wave, 4 * H);
   const int g = a.Hq / a.Hk;
@@ -250,6 +267,7 @@ __global__ __launch_bounds__(256 * H, DT == MVF_F32 && DP > 32 ? H : 2) void pac
     buf = buf == 2 ? 0 : buf + 1;
   }
   f.ds.undo(f.dq);
+  if (O::SZ == 2 && f.low) f.bad |= not_finite(f.dq, f.own.hi > f.own.lo);
   if (f.bad) f.slow(a, kb, vb, span.lo + 32 * (wave >> 2), 32 * H, ws.any.hi);
   if constexpr (H == 2) {
     __syncthreads();
@@ -278,6 +296,7 @@ __global__ __launch_bounds__(256, 1) void packed_attn_dq_split_kernel(BwdArgs a)
   f.start(a, head, row, lane, wave == 0 && row < own.end);
   f.own = keys_of(sequence_of(own, a.cu, a.n_seqs, a.T, row), a.frame, row);
   const WaveSpan ws = wave_span(f.own);
+  f.low = short_walk(ws) || a.D <= SMALL_HEAD;
   if constexpr (PAD) clear_lds(smem, 4 * S::NB * S::BUF);
   const int g = a.Hq / a.Hk;
   const char *kb = a.k + head / g * a.hsk, *vb = a.v + head / g * a.hsv;
@@ -299,6 +318,7 @@ __global__ __launch_bounds__(256, 1) void packed_attn_dq_split_kernel(BwdArgs a)
     else if (more) issue(key0 + 128, 0);
   }
   f.ds.undo(f.dq);
+  if (O::SZ == 2 && f.low) f.bad |= not_finite(f.dq, f.own.hi > f.own.lo);
   if (f.bad) f.slow(a, kb, vb, ws.any.lo + wave * 32, 128, ws.any.hi);
   if (f.own.hi == 0) {           // rows of no sequence rode along in unmasked tiles
 #pragma unroll
@@ -310,7 +330,8 @@ __global__ __launch_bounds__(256, 1) void packed_attn_dq_split_kernel(BwdArgs a)
 
 // ------------------------------------------------------------------------------------------------ dK, dV
 // VL: the wave's own V rows as an image in LDS instead of registers: 16-bit D = 128 then fits two waves on a SIMD, whose products and
-// exponentials overlap (2 x 8192 causal, 16 heads on 4: 1.29 ms; one wave with everything in registers: 2.2).
+// exponentials overlap (2 x 8192 causal, 16 heads on 4: 1.29 ms; one wave with everything in registers: 2.2).  There is no room for second
+// operands there: 2 x 2048 112 us, with them behind their branch 122.
 template <int DT, int DP, bool VL>
 struct Dkv {
   typedef Op<DT> O;
@@ -324,6 +345,7 @@ struct Dkv {
   uint32_t rpart, cpart;
   bool bad = false;        // a tile with masked places held a value that is not finite
   DsScale<DT> ds;
+  bool low = false;        // dS's second operand: see accumulate()
 
   __device__ __forceinline__ void start(const BwdArgs& a, int kh, int row, int lane_, char* own_v) {
     lane = lane_;
@@ -382,9 +404,9 @@ struct Dkv {
         dp[e] = sees ? dp[e] : 0.f;
       }
     }
-    accumulate<O, DP>(dv, s, cd);
+    accumulate_if<O, DP>(!VL && low, dv, s, cd);
     ds.fit(dp, dk);
-    accumulate<O, DP>(dk, dp, cq);
+    accumulate_if<O, DP>(!VL && low, dk, dp, cq);
   }
   // over tiles it = first, first + step, ... of (head h0 + .. of g, 32-query tile, of which a head has a multiple of `per`)
   __device__ __forceinline__ void slow(const BwdArgs& a, int kh, int row, int h0, int g, Span any, int first, int step, int per = 1) {
@@ -448,6 +470,7 @@ __global__ __launch_bounds__(256 * H, DT == MVF_F32 && DP > 32 ? H : 2) void pac
   f.start(a, kh, row, lane, smem + R::NB * (R::BUF + SB) + (wave & 3) * 32 * I::RB);      // (two waves write the same V rows)
   f.own = queries_of(sequence_of(own, a.cu, a.n_seqs, a.T, row), a.frame, row);
   const WaveSpan ws = wave_span(f.own);
+  f.low = short_walk(ws);
   if constexpr (PAD) clear_lds(smem, R::NB * R::BUF);
   const Span span = block_span(ws, s_span, lane, wave, 4 * H);
   const int g = a.Hq / a.Hk / a.parts, h0 = kh * (a.Hq / a.Hk) + part * g;
@@ -481,6 +504,7 @@ __global__ __launch_bounds__(256 * H, DT == MVF_F32 && DP > 32 ? H : 2) void pac
     if (b0 >= span.hi) b0 = span.lo;
   }
   f.ds.undo(f.dk);
+  if (O::SZ == 2 && !VL && f.low) f.bad |= not_finite(f.dk, f.own.hi > f.own.lo) | not_finite(f.dv, f.own.hi > f.own.lo);
   if (f.bad) f.slow(a, kh, row, h0, g, {span.lo, ws.any.hi}, wave >> 2, H, H);
   if constexpr (H == 2) {
     char* half = smem + (wave & 3) * HALF<DP> + lane * 16;
@@ -523,6 +547,7 @@ __global__ __launch_bounds__(256, DT != MVF_F32 && DP <= 64 ? 2 : 1) void packed
   f.start(a, kh, row, lane, nullptr);
   f.own = queries_of(sequence_of(own, a.cu, a.n_seqs, a.T, row), a.frame, row);
   const WaveSpan ws = wave_span(f.own);
+  f.low = short_walk(ws);
   if constexpr (PAD) clear_lds(smem, 4 * S::NB * S::BUF);
   const int g = a.Hq / a.Hk / a.parts, h0 = kh * (a.Hq / a.Hk) + part * g, nt = (ws.any.hi - ws.any.lo + 31) >> 5, total = nt * g;
   const uint32_t lds = lds_addr(smem) + wave * S::NB * S::BUF, stat0 = lds_addr(smem) + 4 * S::NB * S::BUF + wave * S::NB * SB;
@@ -550,6 +575,7 @@ __global__ __launch_bounds__(256, DT != MVF_F32 && DP <= 64 ? 2 : 1) void packed
     else if (more) issue(it + 4, 0);
   }
   f.ds.undo(f.dk);
+  if (O::SZ == 2 && f.low) f.bad |= not_finite(f.dk, f.own.hi > f.own.lo) | not_finite(f.dv, f.own.hi > f.own.lo);
   if (f.bad) f.slow(a, kh, row, h0, g, ws.any, wave, 4);
   if (f.own.hi == 0) {
 #pragma unroll
@@ -670,6 +696,14 @@ extern "C" int mvf_packed_attn_bwd(int dtype, const void* q, long ldq, long hsq,
                                    long ldv, long hsv, const int* cu_seqlens, int n_seqs, const void* out, const void* d_out,
                                    const float* stat, void* workspace, size_t ws_bytes, void* dq, void* dk, void* dv, int T, int Hq, int Hk,
                                    int D, int frame, float scale, hipStream_t st) {
+  return mvf_packed_attn_bwd_rest(dtype, q, ldq, hsq, k, ldk, hsk, v, ldv, hsv, cu_seqlens, n_seqs, out, nullptr, d_out, stat, workspace,
+                                  ws_bytes, dq, dk, dv, T, Hq, Hk, D, frame, scale, st);
+}
+
+extern "C" int mvf_packed_attn_bwd_rest(int dtype, const void* q, long ldq, long hsq, const void* k, long ldk, long hsk, const void* v,
+                                        long ldv, long hsv, const int* cu_seqlens, int n_seqs, const void* out, const void* rest,
+                                        const void* d_out, const float* stat, void* workspace, size_t ws_bytes, void* dq, void* dk,
+                                        void* dv, int T, int Hq, int Hk, int D, int frame, float scale, hipStream_t st) {
   MVF_CHECK_ARG(dtype == MVF_F32 || dtype == MVF_BF16 || dtype == MVF_F16);
   MVF_CHECK_ARG(q && k && v && cu_seqlens && out && d_out && stat && workspace && dq && dk && dv);
   MVF_CHECK_ARG(T > 0 && n_seqs > 0 && Hk > 0 && Hq > 0 && Hq % Hk == 0 && frame >= 0);
@@ -679,13 +713,13 @@ extern "C" int mvf_packed_attn_bwd(int dtype, const void* q, long ldq, long hsq,
   const long s[6] = {ldq * sz, hsq * sz, ldk * sz, hsk * sz, ldv * sz, hsv * sz};
   for (long x : s) MVF_CHECK_ARG(x > 0 && x % 16 == 0);
   MVF_CHECK_ARG((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out | (uintptr_t)d_out | (uintptr_t)dq | (uintptr_t)dk |
-                  (uintptr_t)dv | (uintptr_t)workspace) & 15) == 0);
+                  (uintptr_t)dv | (uintptr_t)workspace | (uintptr_t)rest) & 15) == 0);
   MVF_CHECK_ARG(ws_bytes >= mvf_packed_attn_bwd_workspace_bytes(dtype, T, n_seqs, Hq, Hk, D));
   float* delta = (float*)workspace;
   const int parts = head_parts(T, n_seqs, Hq, Hk, dtype);
   MVF_CHECK_ARG(tile_bound<32>(T, n_seqs) * Hk * parts < (1l << 30) && (size_t)T * Hk * D / 512 < (1ul << 31));
   BwdArgs a = {(const char*)q, (const char*)k, (const char*)v, s[0], s[1], s[2], s[3], s[4], s[5], cu_seqlens, n_seqs, (const char*)out,
-               (const char*)d_out, stat, delta, delta + ((size_t)Hq * T + 3) / 4 * 4, parts, (char*)dq, (char*)dk, (char*)dv, T, Hq, Hk, D,
+               (const char*)rest, (const char*)d_out, stat, delta, delta + ((size_t)Hq * T + 3) / 4 * 4, parts, (char*)dq, (char*)dk, (char*)dv, T, Hq, Hk, D,
                frame, 0, 0, scale * LOG2E, scale * (dtype == MVF_F16 ? 1.f / (1 << PSHIFT) : 1.f), dtype == MVF_F16 ? 1.f / (1 << PSHIFT) : 1.f};
   return dtype == MVF_F32 ? launch_d<MVF_F32>(a, st) : dtype == MVF_BF16 ? launch_d<MVF_BF16>(a, st) : launch_d<MVF_F16>(a, st);
 }

@@ -2405,26 +2405,27 @@ def _packed_fwd(q, k, v, cu, frame, scale, need_stat):
     T, Hq, D = q.shape
     out = torch.empty(T, Hq, D, device=q.device, dtype=q.dtype)
     stat = torch.empty(2, Hq, T, device=q.device, dtype=torch.float32) if need_stat else None
+    rest = torch.empty_like(out) if need_stat and q.dtype != torch.float32 else None       # what the rounding of out takes away
     if T:
-        _launch('mvf_packed_attn_fwd', q, _SEQ_DT[q.dtype], q.data_ptr(), *q.stride()[:2], k.data_ptr(), *k.stride()[:2], v.data_ptr(),
-                *v.stride()[:2], cu.data_ptr(), cu.shape[0] - 1, out.data_ptr(), stat.data_ptr() if need_stat else None, T, Hq, k.shape[1], D,
-                frame, scale)
-    return out, stat
+        _launch('mvf_packed_attn_fwd_rest', q, _SEQ_DT[q.dtype], q.data_ptr(), *q.stride()[:2], k.data_ptr(), *k.stride()[:2], v.data_ptr(),
+                *v.stride()[:2], cu.data_ptr(), cu.shape[0] - 1, out.data_ptr(), None if rest is None else rest.data_ptr(),
+                stat.data_ptr() if need_stat else None, T, Hq, k.shape[1], D, frame, scale)
+    return out, stat, rest
 
 
 class _PackedAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, cu, frame, scale):
         q, k, v = _aligned(q), _aligned(k), _aligned(v)
-        out, stat = _packed_fwd(q, k, v, cu, frame, scale, True)
-        ctx.save_for_backward(q, k, v, cu, out, stat)
+        out, stat, rest = _packed_fwd(q, k, v, cu, frame, scale, True)
+        ctx.save_for_backward(q, k, v, cu, out, stat, rest)
         ctx.cfg = (frame, scale)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, d_out):
-        q, k, v, cu, out, stat = ctx.saved_tensors
+        q, k, v, cu, out, stat, rest = ctx.saved_tensors
         frame, scale = ctx.cfg
         T, Hq, D = q.shape
         d_out = d_out.contiguous()
@@ -2435,8 +2436,9 @@ class _PackedAttention(torch.autograd.Function):
             code, n = _SEQ_DT[q.dtype], cu.shape[0] - 1
             need = _lib.load().mvf_packed_attn_bwd_workspace_bytes(code, T, n, Hq, k.shape[1], D)
             ws = torch.empty(need, device=q.device, dtype=torch.uint8)
-            _launch('mvf_packed_attn_bwd', q, code, q.data_ptr(), *q.stride()[:2], k.data_ptr(), *k.stride()[:2], v.data_ptr(),
-                    *v.stride()[:2], cu.data_ptr(), n, out.data_ptr(), d_out.data_ptr(), stat.data_ptr(), ws.data_ptr(), need,
+            _launch('mvf_packed_attn_bwd_rest', q, code, q.data_ptr(), *q.stride()[:2], k.data_ptr(), *k.stride()[:2], v.data_ptr(),
+                    *v.stride()[:2], cu.data_ptr(), n, out.data_ptr(), None if rest is None else rest.data_ptr(), d_out.data_ptr(),
+                    stat.data_ptr(), ws.data_ptr(), need,
                     dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), T, Hq, k.shape[1], D, frame, scale)
         return dq, dk, dv, None, None, None
 
