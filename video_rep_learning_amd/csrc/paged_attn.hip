@@ -5,8 +5,8 @@
 // them: HBM-bound on 2 len Hk D elements per stream.  A workgroup's four waves walk 32-key tiles of their own (staged by the wave
 // itself, two tiles ahead: no barrier in the loop, 128 KB in flight per compute unit at 16-bit D 128) and meet once per unit; long
 // streams are further cut over workgroups, whose partial sums a second launch joins in a fixed order.  A page id outside the cache holds no
-// keys.  Measured: 12 streams of 32768, bf16, 8 key heads of 128: 297 us, 5.4 TB/s (a copy of 2 GiB: 4.9); 64 of 4096, 4 heads: 105 us,
-// 5.1 TB/s; 64 of 1 to 4096 (66 MB): 26 us, of which the first tile's chain of loads (length, page ids, rows) and the join are 12.
+// keys.  Measured: 12 streams of 32768, bf16, 8 key heads of 128: 300 us, 5.4 TB/s (a copy of 2 GiB: 4.9); 64 of 4096, 4 heads: 105 us,
+// 5.1 TB/s; 64 of 1 to 4096 (50 MB): 27 us, of which the first tile's chain of loads (length, page ids, rows) and the join are 12.
 #include "mvf_hip_internal.h"
 #include "seq_attn.h"
 

@@ -6,8 +6,8 @@
 // dropped terms are 2e-9 and 1e-10 there.
 // The appending form writes the turned keys and the values into pages of a cache instead: token t of stream seq[t] at index[t] goes to
 // row index % page of page table[seq][index / page].
-// Measured: 50176 tokens, 12 + 12 heads of 64, bf16: 66 us, 4.7 TB/s (a copy of 2 GiB: 4.9); 24 prompts into their pages, 16 + 2 x 2 heads of
-// 128: 78 us, 5.4 TB/s; 48 tokens in fp32: 7 us, a launch.
+// Measured: 50176 tokens, 12 + 12 heads of 64, bf16: 67 us, 4.6 TB/s (a copy of 2 GiB: 4.9); 24 prompts into their pages, 16 + 2 x 2 heads of
+// 128, 354 MB: 78 us, 4.5 TB/s; 48 tokens in fp32: 7 us, a launch.
 #include "mvf_hip_internal.h"
 #include "seq_attn.h"
 

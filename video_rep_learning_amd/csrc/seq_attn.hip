@@ -11,7 +11,7 @@
 //           the end: four times as many workgroups and a quarter of the dependent steps, for four times the key traffic.
 // The weights are rounded to the operands' format for the second product (relative 2^-9 in bf16, random in sign, so the sum is off by that
 // much of its size, as the rounding of the result is; not in short walks: short_walk()); their sum is taken before, in 32 bits.
-// Measured: 2 x 8192 causal bf16, 16 query heads of 128 on 4: 0.60 ms, 916 TFLOP/s of visible pairs (a large bf16 matrix product: 1130 to
+// Measured: 2 x 8192 causal bf16, 16 query heads of 128 on 4: 0.60 ms, 911 TFLOP/s of visible pairs (a large bf16 matrix product: 1130 to
 // 1150); 32 x 785, 12 of 64: 114 us, 530; 8 x 1440 fp32 causal by 6, 8 of 32: 119 us, 72 (a large fp32 product: 148).  Bound by the waves'
 // own chains: at D 96 the matrix pipe is busy 24 % of the cycles, the vector unit 31 %, and 32 % of the waves' time goes into waits.
 #include "mvf_hip_internal.h"

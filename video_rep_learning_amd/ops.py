@@ -2448,8 +2448,9 @@ def packed_attention(q, k, v, cu_seqlens, frame=0, scale=None):
     Hk: query head h reads key head h // (Hq // Hk)), sequence b in rows cu_seqlens[b] .. cu_seqlens[b + 1] -> [T, Hq, D].
     frame = 0: a token sees its whole sequence; frame = n: its own and all earlier groups of n tokens of it (1: causal by token; the
     number of entities: causal by frame).  Rows of no sequence give zeros and get zero gradients.  fp32, bf16 or fp16, D a multiple of 8
-    up to 128; scale: 1 / sqrt(D).  Differentiable (once) in q, k, v, the same bits every time.  In the backward the weights and dS are operands
-    of products in the tensors' type: fp16 wants a scaled loss, as everywhere."""
+    up to 128; scale: 1 / sqrt(D).  Differentiable (once) in q, k, v, the same bits every time.  16-bit tensors: where a token sees more than
+    128 others, softmax weights (and dS, their gradients) enter products rounded to the tensors' type, which leaves outputs and gradients
+    within one and a half roundings; sums are 32 bits.  The backward computes the scores again: it wants |scale q . k| below 1e5."""
     _heads(q, 'q')
     _heads(k, 'k', q.shape[0], q.shape[2])
     _heads(v, 'v', q.shape[0], q.shape[2])
@@ -2471,7 +2472,8 @@ def paged_attention(q, k_cache, v_cache, block_table, lengths, frame=1, scale=No
     """Attention of the last n tokens of each stream over its pages of the cache: q [B, n, Hq, D] are the queries of positions
     lengths[b] - n .. lengths[b] - 1 (whose keys and values are in the cache already: rotary_append), k_cache, v_cache
     [pages, page, Hk, D], block_table [B, pages of a stream], lengths [B] -> [B, n, Hq, D].  frame as in packed_attention; a stream of
-    length 0 gives zeros.  For inference: no gradient."""
+    length 0 gives zeros, and so does a position before 0 (unless frame = 0).  A length beyond the table's pages is cut to them; a page outside
+    the cache holds no keys.  16-bit results are one rounding of a 32-bit sum.  For inference: no gradient."""
     if q.dim() != 4 or 0 in q.shape[1:] or q.shape[3] % 8 or q.shape[3] > 128:
         raise ValueError('q: expected [streams, new tokens, heads, head size (a multiple of 8 up to 128)], got %s' % (tuple(q.shape),))
     code = _seq_operands(q, k_cache, v_cache)
