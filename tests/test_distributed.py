@@ -200,3 +200,20 @@ def _loss_allreduce(rank, world):
 def test_loss_allreduce_average():
     out = spawn(_loss_allreduce)
     assert [o[0] for o in out] == [1.5, 1.5] and out[0][1] == 2 and out[0][2] and not out[1][2]
+
+
+def test_collectives_take_any_shape_and_order():
+    """gather_tensor and reduce_tensor on a group of one: empty tensors, no dimensions, strides of their own, whole numbers."""
+    dist.init_process_group('gloo', store=dist.HashStore(), rank=0, world_size=1)
+    try:
+        for t in (torch.zeros(0, 3), torch.tensor(2.5), torch.arange(6).view(2, 3).t(), torch.randn(4, 2, 3)[:, 1], torch.zeros(2, 0, dtype=torch.int64)):
+            got = du.gather_tensor(t)
+            assert got.shape == (1,) + t.shape and torch.equal(got[0], t)
+        x = torch.randn(5)
+        y = x.clone()
+        du.reduce_tensor(y)
+        work = du.reduce_tensor(y, async_op=True, op=dist.ReduceOp.MAX)
+        work.wait()
+        assert torch.equal(x, y)
+    finally:
+        dist.destroy_process_group()

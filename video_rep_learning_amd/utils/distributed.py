@@ -95,9 +95,10 @@ def reduce_tensor(t, group=None, async_op=False, op=dist.ReduceOp.SUM):
 def gather_tensor(t, group=None):
     """dist.all_gather of equal shapes: [world, *t.shape], on t's device."""
     src = t.cpu() if _through_host(t, group) else t.contiguous()
-    out = torch.empty(dist.get_world_size(group) * t.numel(), dtype=t.dtype, device=src.device)     # (gloo's form takes one dimension)
+    world = dist.get_world_size(group)
+    out = torch.empty(world * t.numel(), dtype=t.dtype, device=src.device)       # (gloo's form takes one dimension)
     dist.all_gather_into_tensor(out, src.reshape(-1), group=group)
-    return out.view(-1, *t.shape).to(t.device)
+    return out.view(world, *t.shape).to(t.device)
 
 
 def all_reduce(tensors, average=True):
