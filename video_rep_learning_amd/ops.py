@@ -2385,18 +2385,20 @@ def rotary_append(q, k, v, pos, freqs, sections, k_cache, v_cache, block_table, 
         return qo
     if 0 in table.shape or max(table.shape) >= 2 ** 31:
         raise ValueError('block_table is empty or too large: %s' % (tuple(table.shape),))
-    kc, vc, size, width = k_cache.data_ptr(), v_cache.data_ptr(), k_cache.numel() * q.element_size(), q.element_size()
-    if abs(kc - vc) < size:
+    kc, vc, width, Hk = k_cache.data_ptr(), v_cache.data_ptr(), q.element_size(), k.shape[1]
+    size = k_cache.numel() * width
+    if -size < kc - vc < size:
         raise ValueError('k_cache and v_cache share memory')
-    for t in (q, k, v):
+    args = []
+    for t, heads in ((q, Hq), (k, Hk), (v, Hk)):
         lo, (ld, hs, _) = t.data_ptr(), t.stride()
-        hi = lo + ((T - 1) * ld + (t.shape[1] - 1) * hs + D) * width
+        hi = lo + ((T - 1) * ld + (heads - 1) * hs + D) * width
         if lo < kc + size and hi > kc or lo < vc + size and hi > vc:
             raise ValueError('an operand lies in the memory of a cache, which is written while it is read')
-    _launch('mvf_rotary_append', q, code, q.data_ptr(), *q.stride()[:2], k.data_ptr(), *k.stride()[:2], v.data_ptr(), *v.stride()[:2],
-            pos.data_ptr(), _POS_DT[pos.dtype], freqs.data_ptr(), *sections, bool(interleaved), qo.data_ptr(), k_cache.data_ptr(),
-            v_cache.data_ptr(), table.data_ptr(), table.shape[1], table.shape[0], seq.data_ptr(), index.data_ptr(), k_cache.shape[0],
-            k_cache.shape[1], T, Hq, k.shape[1], D)
+        args += lo, ld, hs
+    _launch('mvf_rotary_append', q, code, *args, pos.data_ptr(), _POS_DT[pos.dtype], freqs.data_ptr(), *sections, bool(interleaved),
+            qo.data_ptr(), kc, vc, table.data_ptr(), table.shape[1], table.shape[0], seq.data_ptr(), index.data_ptr(), k_cache.shape[0],
+            k_cache.shape[1], T, Hq, Hk, D)
     increment_version((k_cache, v_cache))           # what autograd keeps of them is out of date
     return qo
 
