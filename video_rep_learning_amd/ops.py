@@ -600,7 +600,7 @@ class _BatchNormTrain(torch.autograd.Function):
         if slots is not None:
             grad_ready(*owners)
         if world > 0:
-            reduce_tensor(s, group)                  # collective C3 of SURVEY.md
+            reduce_tensor(s, group)                  # over all ranks
         dx = torch.empty_like(x)
         call('mvf_bn_bwd_apply', ptr(dy), ptr(x), ptr(mean), ptr(var), ptr(g), ptr(b), s[0].data_ptr(),
              s[1].data_ptr(), ptr(dx), R, C, eps, int(relu), count, stream())
